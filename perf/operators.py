@@ -4,9 +4,9 @@
 (none where it is negative): out[n] = base[n] + scale[a] B[a] (A[a] x[n]), with A[a] the first rank[a] rows of [most, K] and B[a] the first
 rank[a] columns of [M, most]; base is what the shared projection gave.
 
-`draw`: one token per row of logits from a given random number u, after temperature, top-k, top-p and min-p.  With w_i = exp((l_i - max) / T):
-the k largest logits are kept (ties: the lower index), of these in falling order those before which the share of w is under top_p, of these
-the ones with w >= max(min_p, 2^-64); the token is the first kept one, in vocabulary order, whose running sum of w exceeds u times the sum of
+`draw`: one token per row of logits from a given random number u, after temperature, top-k, top-p and min-p.  With w_i = exp((l_i - max) / T),
+and 0 for less than 2^-40: the k largest logits are kept (ties: the lower index), of these in falling order those before which the share of w is
+under top_p, of these the ones with w > 0 and w >= min_p; the token is the first kept one, in vocabulary order, whose running sum of w exceeds u times the sum of
 all kept.  T = 0 takes the largest logit.  The second output is the token's log-probability among the kept ones.
 """
 import math
@@ -128,8 +128,9 @@ def _draw_plain(s):
     l, at = torch.sort(s["logits"], dim=1, descending=True, stable=True)  # equal logits stay in the order of their indices
     l = l.double()  # borders between two tokens are nearer to each other than 32 bits tell apart
     w = torch.exp((l - l[:, :1]) / torch.where(T > 0, T, 1.0))
+    w = torch.where(w >= 2.0**-40, w, 0.0)
     place = torch.arange(V, device=l.device)[None, :]
-    keep = (place < torch.where(k > 0, k, V)) & (w >= torch.clamp(m, 2.0**-64, 1.0))
+    keep = (place < torch.where(k > 0, k, V)) & (w >= torch.clamp(m, 2.0**-40, 1.0))
     of_k = torch.where(place < torch.where(k > 0, k, V), w, 0.0)
     upto = torch.cumsum(of_k, 1)
     keep &= (upto - of_k < p * upto[:, -1:]) | (p <= 0) | (p >= 1)
@@ -189,7 +190,9 @@ def exact(case, seed):
         k = int(s["params"][n, 1:2].view(torch.int32)) or len(l)
         fall = torch.argsort(-l.double(), stable=True)[: 1 if T == 0 else k]
         z = (l[fall].double() - l[fall[0]].double()) / (T or 1.0)
-        fall, z = fall[z >= max(-64 * math.log(2), math.log(m) if m > 0 else -math.inf)], z
+        fall, z = fall[z >= -40 * math.log(2)], z[z >= -40 * math.log(2)]
+        if m > 0:
+            fall = fall[z >= math.log(m)]
         if 0 < p < 1:
             share = torch.cumsum(torch.softmax(z, 0), 0)
             fall = fall[: 1 + int((share < p).sum())]
