@@ -211,6 +211,45 @@ int rsv_op_sample(int device, const float* logits, int64_t rows, int64_t V, cons
 int rsv_op_sample_static(int device, void* stream, const float* logits_dev, int64_t rows, int64_t V, const float* sampler8_dev,
                          const uint32_t* hist_dev, int64_t hist_stride, uint32_t* out_dev);
 
+/* ---- operators on the caller's device memory ------------------------------------------------------
+ * As rsv_op_sample_static: every array is DEVICE memory of `device`, the launch goes to `stream` (a cudaStream_t, NULL = default
+ * stream) and returns without synchronising, nothing is allocated and no work area is shared, so calls on different streams may
+ * run at the same time and a call may be captured into a CUDA graph.  The caller's current device stays current.  They have no
+ * counterpart in the reference. */
+enum { RSV_F32 = 0, RSV_F16 = 1, RSV_BF16 = 2 };
+
+/* One token per row of logits[rows][V] (rows row_stride elements apart) from the caller's random numbers.  params4_dev[rows * 4]: rows of
+ * [temperature T, bits(top_k), top_p, min_p]; uniforms_dev[rows]: u in [0, 1).  With w_i = exp((l_i - max) / T), and 0 for less than 2^-40:
+ *   - the top_k largest logits are kept (equal ones: the lower index first, so exactly top_k; 0 or >= V: all);
+ *   - of these, in falling order, those before which the sum of w is under top_p times the sum over all of them (<= 0 or >= 1: all);
+ *   - of these, the ones with w > 0 and w >= min_p (<= 0: all; over 1 counts as 1);
+ *   - the token is the first kept one, in vocabulary order, whose running sum of w exceeds u times the sum of all kept ones.
+ * T <= 0 takes the largest logit (the lowest of equal ones).  u < 0 and NaN count as 0, u >= 1 takes the last kept token.
+ * tokens_dev[rows]; logprobs_dev[rows] (may be NULL) is the natural logarithm of the token's share of the kept sum.  Logits of -inf are never
+ * drawn; where there is nothing else the token is 0xFFFFFFFF and the log-probability -inf; a row with a NaN gives 0xFFFFFFFF and NaN.
+ * Weights and sums are whole numbers of 64 bits, so the result does not depend on how rows are split or batched.  V <= 2^22; rows <= 2^28 - 1. */
+int rsv_draw_tokens(int device, void* stream, int dtype, const void* logits_dev, int64_t rows, int64_t V, int64_t row_stride, const float* params4_dev,
+                    const float* uniforms_dev, uint32_t* tokens_dev, float* logprobs_dev);
+
+/* Low-rank adapters of many requests.  Slot s holds A [rank, K] in the first rank rows of a[s] ([max_rank, K], rows a_row and slots a_slot
+ * elements apart) and B [M, rank] in the first rank columns of b[s] ([M, max_rank], rows b_row apart, slots b_slot); what lies behind a slot's
+ * rank is never used.  dtype: RSV_F16 or RSV_BF16.  ranks[slots] NULL: max_rank each; scales[slots] NULL: 1.  max_rank <= 256, slots <= 65536. */
+typedef struct {
+    int32_t dtype;
+    int64_t slots, max_rank, K, M;
+    const void* a;
+    int64_t a_slot, a_row;
+    const void* b;
+    int64_t b_slot, b_row;
+    const int32_t* ranks;
+    const float* scales;
+} rsv_adapters;
+/* out[n] = base[n] + scale[s] B[s] (A[s] x[n]) with s = index_dev[n], for rows x[rows][K], base and out [rows][M] (strides in elements; xtype RSV_F32 or
+ * the adapters' dtype, for all three).  A row whose index is negative (or >= slots) has no adapter: out[n] = base[n].  base is what the shared projection
+ * gave, NULL counts as zeros, and it may be out itself; no other overlap of out is allowed.  Sums are fp32, rounded to out's type once. */
+int rsv_adapters_apply(int device, void* stream, const rsv_adapters* ad, int xtype, const void* x_dev, int64_t x_stride, int64_t rows,
+                       const int32_t* index_dev, const void* base_dev, int64_t base_stride, void* out_dev, int64_t out_stride);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,7 @@ there is no CPU path here: loading a model without the native library or without
 import ctypes as _c
 import json as _json
 import os as _os
+import sys as _sys
 
 import numpy as _np
 
@@ -16,7 +17,7 @@ LIB_CUDA = _os.path.join(_PKG, "librsv_b200.so")
 LIB_SYNTH = _os.path.join(_PKG, "librsv_synth.so")
 
 __all__ = ["ModelBuilder", "Bundle", "State", "Scheduler", "SamplerParams", "RnnInput", "RnnOption", "ModelInfo", "RsvError", "write_synthetic", "SHAPES",
-           "quantize_int8", "op_dequant_int8", "op_linear", "op_wkv7", "op_argmax", "op_sample", "native", "ABI_SYMBOLS"]
+           "quantize_int8", "op_dequant_int8", "op_linear", "op_wkv7", "op_argmax", "op_sample", "draw_params", "draw_tokens", "Adapters", "native", "ABI_SYMBOLS"]
 
 
 class RsvError(RuntimeError):
@@ -33,6 +34,7 @@ ABI_SYMBOLS = [
     "rsv_prof_enable", "rsv_prof_clear", "rsv_prof_dump", "rsv_launch_count", "rsv_timer_start", "rsv_timer_stop", "rsv_synchronize",
     "rsv_sched_new", "rsv_sched_free", "rsv_sched_submit", "rsv_sched_step", "rsv_sched_poll", "rsv_sched_result", "rsv_sched_sync",
     "rsv_sched_stats", "rsv_quantize_int8", "rsv_op_dequant_int8", "rsv_op_linear", "rsv_op_wkv7", "rsv_op_argmax", "rsv_op_sample", "rsv_op_sample_static",
+    "rsv_draw_tokens", "rsv_adapters_apply",
 ]
 
 
@@ -120,6 +122,8 @@ def native():
         L.rsv_op_wkv7.argtypes = [_c.c_int, _c.c_int, i64, i64, i64] + [vp] * 15
         L.rsv_op_sample.argtypes = [_c.c_int, vp, i64, i64, vp, vp, i64, vp]
         L.rsv_op_sample_static.argtypes = [_c.c_int, vp, vp, i64, i64, vp, vp, i64, vp]
+        L.rsv_draw_tokens.argtypes = [_c.c_int, vp, _c.c_int, vp, i64, i64, i64, vp, vp, vp, vp]
+        L.rsv_adapters_apply.argtypes = [_c.c_int, vp, vp, _c.c_int, vp, i64, i64, vp, vp, i64, vp, i64]
         _native = L
     return _native
 
@@ -551,6 +555,106 @@ def op_sample(logits, sampler_rows, hist=None, device=0):
     else:
         _check(native().rsv_op_sample(device, _ptr(lg), lg.shape[0], lg.shape[1], _ptr(rows), None, 0, _ptr(out)))
     return out
+
+
+# ---- operators on device memory: torch CUDA tensors (anything with data_ptr, shape, stride, dtype and device), on their framework's current stream ----
+_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+_WORDS = ("torch.int32", "torch.uint32")
+
+
+def _stream_of(device, stream):
+    """The handle of `stream` (a torch stream or an integer), by default torch's current stream of the device."""
+    if stream is None:
+        return _sys.modules["torch"].cuda.current_stream(device).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _rows_of(name, t, dtypes, cols=None, rows=None):
+    """(rows, columns, row stride) of a matrix whose columns follow each other."""
+    if t.device.type != "cuda":
+        raise RsvError(f"{name}: a CUDA tensor is needed")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise RsvError(f"{name}: a matrix with contiguous rows is needed")
+    if str(t.dtype) not in dtypes:
+        raise RsvError(f"{name}: dtype {t.dtype} is not one of {', '.join(dtypes)}")
+    if (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows):
+        raise RsvError(f"{name}: shape {tuple(t.shape)}, wanted {(rows, cols)}")
+    return t.shape[0], t.shape[1], t.stride(0)
+
+
+def _vector(name, t, dtypes, n, device):
+    if t.device != device or not t.is_contiguous() or tuple(t.shape) != (n,) or str(t.dtype) not in dtypes:
+        raise RsvError(f"{name}: a contiguous vector of {n} values of {' or '.join(dtypes)} on {device} is needed")
+    return t.data_ptr()
+
+
+def draw_params(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Parameter rows of `draw_tokens` as a float32 array [rows, 4]; the arguments are numbers or sequences, broadcast against each other."""
+    T, k, p, m = _np.broadcast_arrays(*(_np.atleast_1d(v) for v in (temperature, top_k, top_p, min_p)))
+    if (k < 0).any():
+        raise RsvError("draw_params: top_k must not be negative")
+    out = _np.empty((T.size, 4), dtype=_np.float32)
+    out[:, 0], out[:, 2], out[:, 3] = T, p, m
+    out.view(_np.uint32)[:, 1] = _np.minimum(k, 0xFFFFFFFF)
+    return out
+
+
+def draw_tokens(logits, params, uniforms, tokens, logprobs=None, stream=None):
+    """Draws tokens[r] from row r of logits [rows, V] (float32, float16 or bfloat16) with the random number uniforms[r] in [0, 1), after the row's temperature,
+    top-k, top-p and min-p (`params` [rows, 4] float32, as draw_params lays them out); logprobs[r]: the log-probability among what was kept.  Rules, ties and
+    rows that have no token (-1 in an int32 tensor): rsv_draw_tokens in include/rsv_b200.h.  Queued on the stream, returns at once."""
+    rows, V, ld = _rows_of("logits", logits, _DTYPES)
+    dev = logits.device
+    if _rows_of("params", params, ("torch.float32",), 4, rows)[2] != 4 and rows > 1 or params.device != dev:
+        raise RsvError(f"params: a contiguous tensor on {dev} is needed")
+    _check(native().rsv_draw_tokens(dev.index, _stream_of(dev, stream), _DTYPES[str(logits.dtype)], logits.data_ptr(), rows, V, ld, params.data_ptr(),
+                                    _vector("uniforms", uniforms, ("torch.float32",), rows, dev), _vector("tokens", tokens, _WORDS, rows, dev),
+                                    None if logprobs is None else _vector("logprobs", logprobs, ("torch.float32",), rows, dev)))
+    return tokens
+
+
+class _AdaptersC(_c.Structure):
+    _fields_ = [("dtype", _c.c_int32), ("slots", _c.c_int64), ("max_rank", _c.c_int64), ("K", _c.c_int64), ("M", _c.c_int64), ("a", _c.c_void_p), ("a_slot", _c.c_int64),
+                ("a_row", _c.c_int64), ("b", _c.c_void_p), ("b_slot", _c.c_int64), ("b_row", _c.c_int64), ("ranks", _c.c_void_p), ("scales", _c.c_void_p)]
+
+
+class Adapters:
+    """Low-rank adapters of many requests beside one shared projection: slot s is A[s] [rank, K] and B[s] [M, rank] (rsv_adapters in include/rsv_b200.h).
+
+    A [slots, max_rank, K] and B [slots, M, max_rank], float16 or bfloat16; ranks [slots] int32 (default: max_rank each) and scales [slots] float32 (default: 1).
+    The tensors are used where they lie and may be written to between calls on the same stream, to bring in another adapter for instance."""
+
+    def __init__(self, A, B, ranks=None, scales=None):
+        if A.dim() != 3 or B.dim() != 3 or A.device.type != "cuda" or B.device != A.device:
+            raise RsvError("Adapters: A and B must be three-dimensional CUDA tensors on one device")
+        if str(A.dtype) not in ("torch.float16", "torch.bfloat16") or B.dtype != A.dtype:
+            raise RsvError("Adapters: A and B must both be float16 or both bfloat16")
+        slots, most, K = A.shape
+        if B.shape[0] != slots or B.shape[2] != most:
+            raise RsvError(f"Adapters: B of shape {tuple(B.shape)} does not go with A of shape {tuple(A.shape)}")
+        if (K > 1 and A.stride(2) != 1) or (most > 1 and B.stride(2) != 1):
+            raise RsvError("Adapters: the last dimensions of A and B must be contiguous")
+        self.device, self.dtype = A.device, A.dtype
+        self.slots, self.max_rank, self.K, self.M = slots, most, K, B.shape[1]
+        self._keep = (A, B, ranks, scales)
+        self._c = _AdaptersC(_DTYPES[str(A.dtype)], slots, most, K, self.M, A.data_ptr(), A.stride(0), A.stride(1), B.data_ptr(), B.stride(0), B.stride(1),
+                             None if ranks is None else _vector("ranks", ranks, ("torch.int32",), slots, A.device),
+                             None if scales is None else _vector("scales", scales, ("torch.float32",), slots, A.device))
+        self._ref = _c.byref(self._c)
+        self._xtypes = ("torch.float32", str(A.dtype))
+
+    def apply(self, x, index, out, base=None, stream=None):
+        """out[n] = base[n] + scale B (A x[n]) with the adapter index[n] (int32; negative: none).  x [rows, K], out and base [rows, M] of one type: float32 or the
+        adapters'.  base None: zeros; base may be out.  Queued on the stream, returns at once."""
+        rows, _, ldx = _rows_of("x", x, self._xtypes, self.K)
+        dev, xt = self.device, str(x.dtype)
+        ldo = _rows_of("out", out, (xt,), self.M, rows)[2]
+        ldb = _rows_of("base", base, (xt,), self.M, rows)[2] if base is not None else 0
+        if x.device != dev or out.device != dev or (base is not None and base.device != dev):
+            raise RsvError(f"Adapters.apply: all tensors must be on {dev}")
+        _check(native().rsv_adapters_apply(dev.index, _stream_of(dev, stream), self._ref, _DTYPES[xt], x.data_ptr(), ldx, rows,
+                                           _vector("index", index, ("torch.int32",), rows, dev), None if base is None else base.data_ptr(), ldb, out.data_ptr(), ldo))
+        return out
 
 
 # ---- synthetic checkpoints (csrc/synth.cpp) ----
