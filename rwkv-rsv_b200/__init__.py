@@ -560,31 +560,40 @@ def op_sample(logits, sampler_rows, hist=None, device=0):
 # ---- operators on device memory: torch CUDA tensors (anything with data_ptr, shape, stride, dtype and device), on their framework's current stream ----
 _DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
 _WORDS = ("torch.int32", "torch.uint32")
+_types = {}  # torch dtype -> the C interface's number; a call takes a few microseconds, so a dtype's name is made once
+
+
+def _type_of(t):
+    n = _types.get(t.dtype)
+    if n is None:
+        n = _types[t.dtype] = _DTYPES.get(str(t.dtype), -1 if str(t.dtype) not in _WORDS else 8)
+    return n
 
 
 def _stream_of(device, stream):
     """The handle of `stream` (a torch stream or an integer), by default torch's current stream of the device."""
     if stream is None:
-        return _sys.modules["torch"].cuda.current_stream(device).cuda_stream
+        torch = _sys.modules["torch"]
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(device) if raw else torch.cuda.current_stream(device).cuda_stream
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _rows_of(name, t, dtypes, cols=None, rows=None):
-    """(rows, columns, row stride) of a matrix whose columns follow each other."""
-    if t.device.type != "cuda":
-        raise RsvError(f"{name}: a CUDA tensor is needed")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise RsvError(f"{name}: a matrix with contiguous rows is needed")
-    if str(t.dtype) not in dtypes:
-        raise RsvError(f"{name}: dtype {t.dtype} is not one of {', '.join(dtypes)}")
-    if (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows):
-        raise RsvError(f"{name}: shape {tuple(t.shape)}, wanted {(rows, cols)}")
-    return t.shape[0], t.shape[1], t.stride(0)
+def _rows_of(name, t, types, cols=None, rows=None, device=None):
+    """Row stride of a matrix whose columns follow each other, of one of these types and sizes, on the device."""
+    R, C = t.shape if t.dim() == 2 else (-1, -1)
+    at, (down, right) = t.get_device(), t.stride() if R >= 0 else (0, 0)
+    if R < 0 or at < 0 or (device is not None and at != device) or (right != 1 and C > 1) or _type_of(t) not in types or (cols is not None and C != cols) or (rows is not None and R != rows):
+        raise RsvError(f"{name}: {tuple(t.shape)} of {t.dtype} on {t.device} with strides {t.stride()}; wanted is a CUDA tensor [{'rows' if rows is None else rows}, "
+                       f"{'columns' if cols is None else cols}] of {' or '.join(k for k, v in _DTYPES.items() if v in types)} with contiguous rows" +
+                       ("" if device is None else f" on cuda:{device}"))
+    return down
 
 
-def _vector(name, t, dtypes, n, device):
-    if t.device != device or not t.is_contiguous() or tuple(t.shape) != (n,) or str(t.dtype) not in dtypes:
-        raise RsvError(f"{name}: a contiguous vector of {n} values of {' or '.join(dtypes)} on {device} is needed")
+def _vector(name, t, kind, n, device):
+    """Address of a contiguous vector of n values of that kind on the device."""
+    if t.get_device() != device or _type_of(t) != kind or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise RsvError(f"{name}: {tuple(t.shape)} of {t.dtype} on {t.device}; wanted is a contiguous vector of {n} values of {'float32' if kind == 0 else 'int32'} on cuda:{device}")
     return t.data_ptr()
 
 
@@ -603,13 +612,13 @@ def draw_tokens(logits, params, uniforms, tokens, logprobs=None, stream=None):
     """Draws tokens[r] from row r of logits [rows, V] (float32, float16 or bfloat16) with the random number uniforms[r] in [0, 1), after the row's temperature,
     top-k, top-p and min-p (`params` [rows, 4] float32, as draw_params lays them out); logprobs[r]: the log-probability among what was kept.  Rules, ties and
     rows that have no token (-1 in an int32 tensor): rsv_draw_tokens in include/rsv_b200.h.  Queued on the stream, returns at once."""
-    rows, V, ld = _rows_of("logits", logits, _DTYPES)
-    dev = logits.device
-    if _rows_of("params", params, ("torch.float32",), 4, rows)[2] != 4 and rows > 1 or params.device != dev:
-        raise RsvError(f"params: a contiguous tensor on {dev} is needed")
-    _check(native().rsv_draw_tokens(dev.index, _stream_of(dev, stream), _DTYPES[str(logits.dtype)], logits.data_ptr(), rows, V, ld, params.data_ptr(),
-                                    _vector("uniforms", uniforms, ("torch.float32",), rows, dev), _vector("tokens", tokens, _WORDS, rows, dev),
-                                    None if logprobs is None else _vector("logprobs", logprobs, ("torch.float32",), rows, dev)))
+    ld = _rows_of("logits", logits, (0, 1, 2))
+    rows, V = logits.shape
+    dev = logits.get_device()
+    if _rows_of("params", params, (0,), 4, rows, dev) != 4 and rows > 1:
+        raise RsvError("params: a contiguous tensor is needed")
+    _check(native().rsv_draw_tokens(dev, _stream_of(dev, stream), _type_of(logits), logits.data_ptr(), rows, V, ld, params.data_ptr(), _vector("uniforms", uniforms, 0, rows, dev),
+                                    _vector("tokens", tokens, 8, rows, dev), None if logprobs is None else _vector("logprobs", logprobs, 0, rows, dev)))
     return tokens
 
 
@@ -634,26 +643,21 @@ class Adapters:
             raise RsvError(f"Adapters: B of shape {tuple(B.shape)} does not go with A of shape {tuple(A.shape)}")
         if (K > 1 and A.stride(2) != 1) or (most > 1 and B.stride(2) != 1):
             raise RsvError("Adapters: the last dimensions of A and B must be contiguous")
-        self.device, self.dtype = A.device, A.dtype
         self.slots, self.max_rank, self.K, self.M = slots, most, K, B.shape[1]
-        self._keep = (A, B, ranks, scales)
-        self._c = _AdaptersC(_DTYPES[str(A.dtype)], slots, most, K, self.M, A.data_ptr(), A.stride(0), A.stride(1), B.data_ptr(), B.stride(0), B.stride(1),
-                             None if ranks is None else _vector("ranks", ranks, ("torch.int32",), slots, A.device),
-                             None if scales is None else _vector("scales", scales, ("torch.float32",), slots, A.device))
-        self._ref = _c.byref(self._c)
-        self._xtypes = ("torch.float32", str(A.dtype))
+        self.device, self._dev, self._keep = A.device, A.get_device(), (A, B, ranks, scales)
+        self._c = _AdaptersC(_type_of(A), slots, most, K, self.M, A.data_ptr(), A.stride(0), A.stride(1), B.data_ptr(), B.stride(0), B.stride(1),
+                             None if ranks is None else _vector("ranks", ranks, 8, slots, self._dev), None if scales is None else _vector("scales", scales, 0, slots, self._dev))
+        self._ref, self._types = _c.byref(self._c), (0, _type_of(A))
 
     def apply(self, x, index, out, base=None, stream=None):
         """out[n] = base[n] + scale B (A x[n]) with the adapter index[n] (int32; negative: none).  x [rows, K], out and base [rows, M] of one type: float32 or the
         adapters'.  base None: zeros; base may be out.  Queued on the stream, returns at once."""
-        rows, _, ldx = _rows_of("x", x, self._xtypes, self.K)
-        dev, xt = self.device, str(x.dtype)
-        ldo = _rows_of("out", out, (xt,), self.M, rows)[2]
-        ldb = _rows_of("base", base, (xt,), self.M, rows)[2] if base is not None else 0
-        if x.device != dev or out.device != dev or (base is not None and base.device != dev):
-            raise RsvError(f"Adapters.apply: all tensors must be on {dev}")
-        _check(native().rsv_adapters_apply(dev.index, _stream_of(dev, stream), self._ref, _DTYPES[xt], x.data_ptr(), ldx, rows,
-                                           _vector("index", index, ("torch.int32",), rows, dev), None if base is None else base.data_ptr(), ldb, out.data_ptr(), ldo))
+        dev, rows, xt = self._dev, x.shape[0], _type_of(x)
+        ldx = _rows_of("x", x, self._types, self.K, None, dev)
+        ldo = _rows_of("out", out, (xt,), self.M, rows, dev)
+        ldb = _rows_of("base", base, (xt,), self.M, rows, dev) if base is not None else 0
+        _check(native().rsv_adapters_apply(dev, _stream_of(dev, stream), self._ref, xt, x.data_ptr(), ldx, rows, _vector("index", index, 8, rows, dev),
+                                           None if base is None else base.data_ptr(), ldb, out.data_ptr(), ldo))
         return out
 
 

@@ -8,11 +8,11 @@
 
 namespace rsv {
 
-// rint(2^F) V fits 63 bits, and a weight 51
+// V weights of up to 2^F fit 62 bits, and the up to 384 of a thread 53: those are summed in fp64
 static int draw_bits(int64_t V) {
     int lg = 0;
     while ((int64_t(1) << lg) < V) ++lg;
-    return lg > 12 ? 62 - lg : 50;
+    return lg > 16 ? 62 - lg : 46;  // (384 a thread: V from 2^19 on, F = 43)
 }
 
 template <typename T>
@@ -22,18 +22,18 @@ static void launch_draw(cudaStream_t stream, int device, int64_t rows, const Dra
     const int64_t places = (int64_t)A.V + (aligned ? 0 : N - 1);
     int S = 1;
     while (S < kDcMaxCtas && (int64_t)S * most < places) S *= 2;
-    if ((int64_t)S * most < places) {
+    if ((int64_t)S * (kDcMostSliceBytes / (int64_t)sizeof(T)) < places + S * unit) {
         draw_plain_kernel<T><<<(unsigned)rows, kDwThreads, 0, stream>>>(A);
         RSV_CUDA(cudaGetLastError());
         return;
     }
     // few rows: over more CTAs, as long as the GPU has room for them
-    while (S < kDcMaxCtas && rows * S * 2 <= 296 && places > (int64_t)S * unit) S *= 2;
+    while (S < kDcMaxCtas && rows * S * 2 <= 592 && places > (int64_t)S * unit) S *= 2;
     const int slice = (int)((places + (int64_t)S * unit - 1) / ((int64_t)S * unit)) * unit;
     const size_t smem = sizeof(DcShared) + std::max((size_t)slice * sizeof(T), sizeof(DwPlainShared));
     static bool configured[64] = {false};
     if (device >= 64 || !configured[device]) {
-        RSV_CUDA(cudaFuncSetAttribute(draw_cluster_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(DcShared) + kDcSliceBytes)));
+        RSV_CUDA(cudaFuncSetAttribute(draw_cluster_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(DcShared) + kDcMostSliceBytes)));
         if (device < 64) configured[device] = true;
     }
     cudaLaunchConfig_t cfg = {};

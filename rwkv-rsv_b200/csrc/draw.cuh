@@ -19,7 +19,7 @@
 
 namespace rsv {
 
-constexpr int kDwThreads = 512;
+constexpr int kDwThreads = 256;
 constexpr int kDwWarps = kDwThreads / 32;
 constexpr int kDwMaxLogV = 22;
 constexpr uint32_t kDwNone = 0xFFFFFFFFu;  // the token of a row that has none
@@ -49,50 +49,70 @@ __device__ __forceinline__ float dw_value(uint32_t key) { return __uint_as_float
 // What a row asks for, and its largest logit once that is known.
 struct DwRow {
     double c, ymin, mxd;  // log2(e) / T; the least y that min-p keeps
-    float mx, top_p;
+    float T, mx, top_p, min_p;
     uint32_t top_k;  // 0: all
     int F;
     bool greedy;
 };
-__device__ __forceinline__ DwRow dw_row(const DrawArgs& A, int row) {
+__device__ __forceinline__ DwRow dw_asked(const DrawArgs& A, int row) {
     const float* p = A.params4 + (size_t)row * 4;
-    const float T = p[0], m = p[3];
     const uint32_t k = __float_as_uint(p[1]);
     DwRow r;
-    r.greedy = !(T > 0.f);
-    r.c = 1.4426950408889634074 / (double)T;
+    r.T = p[0];
+    r.greedy = !(r.T > 0.f);
     r.top_k = k < (uint32_t)A.V ? k : 0u;
     r.top_p = p[2] > 0.f && p[2] < 1.f ? p[2] : 0.f;
-    r.ymin = m > 0.f ? fmax(log2((double)fminf(m, 1.f)), -40.0) : -40.0;
+    r.min_p = p[3] > 0.f ? fminf(p[3], 1.f) : 0.f;
     r.F = A.F;
-    r.mx = 0.f, r.mxd = 0.0;
+    r.c = r.ymin = r.mxd = 0.0;
+    r.mx = 0.f;
     return r;
 }
-// (The largest logit may be infinite, and T too: what is NaN then counts as nothing.)
-__device__ __forceinline__ double dw_y(const DwRow& r, float l) { return l == r.mx ? 0.0 : ((double)l - r.mxd) * r.c; }
+__device__ __forceinline__ double dw_rate(float T) { return 1.4426950408889634074 / (double)T; }
+__device__ __forceinline__ double dw_least(float min_p) { return min_p > 0.f ? fmax(log2((double)min_p), -40.0) : -40.0; }
+// (The difference first: at a low temperature max and l alone would be too large to subtract.)
+__device__ __forceinline__ double dw_y(const DwRow& r, float l) { return ((double)l - r.mxd) * r.c; }
 
-// rint(2^(y + F)) for -40 <= y <= 0.  2^y = 2^n 2^(j/16) 2^f with |f| <= 1/32: a table of sixteen and the Taylor polynomial of e^(f ln 2) to the sixth
-// power (the next term is under 4e-16).
-__device__ __forceinline__ u64 dw_fixed(double y, int F, const double* tab16) {
-    const double big = 6755399441055744.0 / 16.0;  // 1.5 2^48: a sum's last place is 1/16
-    const double t = y + big, f = (y - (t - big)) * 0.69314718055994530942;
+// rint(2^(y + F)) for y = (l - max) c from -40 to 0.  2^y = 2^n 2^(j/16) 2^f with |f| <= 1/32: a table of 2^(F + j/16) and the Taylor polynomial of
+// e^(f ln 2) to the fifth power, with the powers of ln 2 in its coefficients (the next term is under 1.5e-13 of the weight).  Kernels that sum weights
+// are bound by these eleven fp64 operations and their surroundings (64 of them a cycle and SM).
+__device__ __forceinline__ double dw_whole(const DwRow& r, float l, const double* tab16) {
+    const double big = 6755399441055744.0 / 16.0, round = 4503599627370496.0, d = (double)l - r.mxd;  // 1.5 2^48: a sum's last place is 1/16; 2^52: it is 1
+    const double t = fma(d, r.c, big), f = fma(d, r.c, -(t - big));
     const int n16 = __double2loint(t);
-    double p = fma(f, 1.0 / 720.0, 1.0 / 120.0);
-    p = fma(p, f, 1.0 / 24.0);
-    p = fma(p, f, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
+    double p = fma(f, 0.0013333558146428443, 0.0096181291076284769);
+    p = fma(p, f, 0.055504108664821583);
+    p = fma(p, f, 0.24022650695910072);
+    p = fma(p, f, 0.69314718055994529);
     p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0) * tab16[n16 & 15];
-    p = __hiloint2double(__double2hiint(p) + (((n16 >> 4) + F) << 20), __double2loint(p));
-    return (u64)__double_as_longlong(p + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;  // (p < 2^51)
+    const double w = tab16[n16 & 15];
+    return fma(p, __hiloint2double(__double2hiint(w) + (n16 & ~15) * 65536, __double2loint(w)), round) - round;
 }
+__device__ __forceinline__ u64 dw_fixed(const DwRow& r, float l, const double* tab16) { return (u64)dw_whole(r, l, tab16); }
 // The weight of a logit; 0 for y < -40.
-__device__ __forceinline__ u64 dw_weight(const DwRow& r, float l, const double* tab16) {
-    const double y = dw_y(r, l);
-    return y >= -40.0 ? dw_fixed(y, r.F, tab16) : 0ull;
-}
-__device__ __forceinline__ void dw_fill_table(double* tab16) {
-    if (threadIdx.x < 16) tab16[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
+__device__ __forceinline__ u64 dw_weight(const DwRow& r, float l, const double* tab16) { return dw_y(r, l) >= -40.0 ? dw_fixed(r, l, tab16) : 0ull; }
+// 2^(j/16)
+__constant__ double kDwTable[16] = {1.0,
+                                    1.0442737824274138,
+                                    1.0905077326652577,
+                                    1.1387886347566916,
+                                    1.189207115002721,
+                                    1.241857812073484,
+                                    1.2968395546510096,
+                                    1.3542555469368927,
+                                    1.4142135623730951,
+                                    1.4768261459394993,
+                                    1.5422108254079407,
+                                    1.6104903319492543,
+                                    1.681792830507429,
+                                    1.7562521603732995,
+                                    1.8340080864093424,
+                                    1.9152065613971474};
+__device__ __forceinline__ void dw_fill_table(double* tab16, int F) {
+    if (threadIdx.x < 16) {
+        const double t = kDwTable[threadIdx.x];
+        tab16[threadIdx.x] = __hiloint2double(__double2hiint(t) + (F << 20), __double2loint(t));
+    }
 }
 // top_p of the sum: the sum before a token is under it exactly where it is under the next whole number
 __device__ __forceinline__ u64 dw_share(float top_p, u64 total) {
@@ -113,6 +133,7 @@ __device__ __forceinline__ float dw_logprob(const DwRow& r, float l, u64 total) 
     return (float)(dw_y(r, l) * 0.69314718055994530942 - log((double)total * exp2(-(double)r.F)));
 }
 
+static_assert(kDwThreads == 256, "a thread per bin of a radix pass");
 // ---- a row by one CTA, from global memory -----------------------------------------------------------------
 struct DwPlainShared {
     double tab[16];
@@ -138,8 +159,10 @@ template <typename T>
 __device__ __noinline__ void dw_row_plain(const DrawArgs& A, int row, DwPlainShared& sh) {
     const T* lg = reinterpret_cast<const T*>(A.logits) + (size_t)row * A.ld;
     const int V = A.V, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    DwRow r = dw_row(A, row);
-    dw_fill_table(sh.tab);
+    DwRow r = dw_asked(A, row);
+    r.c = dw_rate(r.T);
+    r.ymin = dw_least(r.min_p);
+    dw_fill_table(sh.tab, r.F);
     // ---- the largest logit
     float mx = -INFINITY;
     bool nan = false;
@@ -160,10 +183,17 @@ __device__ __noinline__ void dw_row_plain(const DrawArgs& A, int row, DwPlainSha
     }
     r.mx = mx;
     r.mxd = (double)mx;
+    // where there are infinite logits only they are drawn, all alike
+    const bool infinite = mx == INFINITY;
+    if (infinite) r.mx = 0.f, r.mxd = 0.0;
+    const auto logit = [&](int i) {
+        const float l = dw_f32(lg[i]);
+        return infinite ? (l == INFINITY ? 0.f : -INFINITY) : l;
+    };
     if (r.greedy) {
         uint32_t best = kDwNone;
         for (int i = tid; i < V; i += kDwThreads)
-            if (dw_f32(lg[i]) == mx) best = min(best, (uint32_t)i);
+            if (logit(i) == r.mx) best = min(best, (uint32_t)i);
         best = __reduce_min_sync(0xffffffffu, best);
         if (lane == 0) atomicMin(&sh.best, best);
         __syncthreads();
@@ -177,10 +207,10 @@ __device__ __noinline__ void dw_row_plain(const DrawArgs& A, int row, DwPlainSha
 #pragma unroll 1
         for (int shift = 24; shift >= 0; shift -= 8) {
             __syncthreads();
-            if (tid < 256) sh.hist[tid] = 0;
+            sh.hist[tid] = 0;
             __syncthreads();
             for (int i = tid; i < V; i += kDwThreads) {
-                const uint32_t key = dw_key(dw_f32(lg[i]));
+                const uint32_t key = dw_key(logit(i));
                 if ((key & mask) == prefix) atomicAdd(reinterpret_cast<uint32_t*>(&sh.hist[(key >> shift) & 255u]), 1u);
             }
             __syncthreads();
@@ -201,7 +231,7 @@ __device__ __noinline__ void dw_row_plain(const DrawArgs& A, int row, DwPlainSha
     if (r.top_p > 0.f) {
         u64 sum = 0;
         for (int i = tid; i < V; i += kDwThreads) {
-            const float l = dw_f32(lg[i]);
+            const float l = logit(i);
             if (dw_key(l) > cut) sum += dw_weight(r, l, sh.tab);
         }
         const u64 wcut = equals ? dw_weight(r, dw_value(cut), sh.tab) * equals : 0ull;  // the kept ones of those at the cut
@@ -211,10 +241,10 @@ __device__ __noinline__ void dw_row_plain(const DrawArgs& A, int row, DwPlainSha
 #pragma unroll 1
         for (int shift = 24; shift >= 0; shift -= 8) {
             __syncthreads();
-            if (tid < 256) sh.hist[tid] = 0;
+            sh.hist[tid] = 0;
             __syncthreads();
             for (int i = tid; i < V; i += kDwThreads) {
-                const float l = dw_f32(lg[i]);
+                const float l = logit(i);
                 const uint32_t key = dw_key(l);
                 if ((key & mask) == prefix && key > cut) atomicAdd(&sh.hist[(key >> shift) & 255u], dw_weight(r, l, sh.tab));
             }
@@ -239,20 +269,20 @@ __device__ __noinline__ void dw_row_plain(const DrawArgs& A, int row, DwPlainSha
     // ---- the sum of the kept ones
     u64 sum = 0;
     for (int i = tid; i < V; i += kDwThreads) {
-        const float l = dw_f32(lg[i]);
+        const float l = logit(i);
         const double y = dw_y(r, l);
-        if (dw_key(l) > cut && y >= r.ymin) sum += dw_fixed(y, r.F, sh.tab);
+        if (dw_key(l) > cut && y >= r.ymin) sum += dw_fixed(r, l, sh.tab);
     }
     u64 total = dw_block_sum(sum, sh);
     if (equals && dw_y(r, dw_value(cut)) >= r.ymin) total += dw_weight(r, dw_value(cut), sh.tab) * equals;
     const u64 U = dw_target(A.u[row], total);
-    // ---- the draw, 512 tokens at a time in vocabulary order
+    // ---- the draw, 256 tokens at a time in vocabulary order
     u64 run = 0;
     uint32_t seen = 0;
 #pragma unroll 1
     for (int i0 = 0; i0 < V; i0 += kDwThreads) {
         const int i = i0 + tid;
-        const float l = i < V ? dw_f32(lg[i]) : -INFINITY;
+        const float l = i < V ? logit(i) : -INFINITY;
         const uint32_t key = dw_key(l);
         const bool eq = i < V && key == cut;
         const uint32_t ballot = __ballot_sync(0xffffffffu, eq);
@@ -265,7 +295,7 @@ __device__ __noinline__ void dw_row_plain(const DrawArgs& A, int row, DwPlainSha
             seen += sh.wcnt[j];
         }
         const double y = dw_y(r, l);
-        u64 w = i < V && y >= r.ymin && (key > cut || (eq && place < equals)) ? dw_fixed(y, r.F, sh.tab) : 0ull, incl = w;
+        u64 w = i < V && y >= r.ymin && (key > cut || (eq && place < equals)) ? dw_fixed(r, l, sh.tab) : 0ull, incl = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 t = __shfl_up_sync(0xffffffffu, incl, o);

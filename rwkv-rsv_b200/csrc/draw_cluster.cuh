@@ -2,46 +2,62 @@
 //
 // The logits are read from global memory once, with their maximum; everything else works on shared memory.  The cut that top-k and top-p make is
 // found without sorting the row:
-//   list    Every thread keeps the largest of its own logits.  The k-th largest of a CTA's 512 such maxima is a lower bound of the row's k-th largest
-//           logit, and so is the smallest over the CTAs of the (k / CTAs)-th; the logits from the larger of the two on are collected (k and a few more),
-//           sorted by value and index, and the cut lies among them.  With top-p and no top-k the 256 largest are tried first: their weight tells
-//           whether the cut lies among them.
-//   region  Otherwise a histogram of (max - l) in 2048 linear bins says near which bin the cut lies; the logits of that bin and its neighbours are
+//   list    Every thread keeps the largest of its own logits.  The k-th largest of a CTA's 256 such maxima is a lower bound of the row's k-th largest
+//           logit, and so is the smallest over the CTAs of the (k / CTAs)-th; the logits from the larger of the two on are collected (k and a few more) and
+//           sorted by value and index, and the cut lies among them.  With top-p and no top-k the 256 largest are tried: their weight tells whether
+//           the cut lies among them.
+//   region  Otherwise the cut lies in a stretch of values known from the pass that summed the weights (three stretches, between bounds from the threads'
+//           maxima).  A histogram of that stretch in 512 linear bins says near which bin the cut is; the logits of that bin and its neighbours are
 //           collected and sorted, the weight of all larger ones is summed exactly, and the sums tell whether the cut is there.
-//   neither Where the collection would not fit 1024 entries (many equal logits) one CTA does the row by radix passes (dw_row_plain).
+//   neither Where a collection would not fit 512 entries (many equal logits) one CTA does the row by radix passes (dw_row_plain).
 // Without top-k and top-p no cut is needed: min-p's is a value that follows from the maximum.
 //
-// The draw: sums of the kept weights per warp, whose logits follow each other in the vocabulary, then the one warp's stretch again, split over the CTA.
+// The draw: sums of the kept weights per warp, whose logits follow each other in the vocabulary, then the one warp's stretch again, split over a CTA.
+//
+// What the CTAs tell each other is written into the receiver's shared memory before a cluster barrier, so that nobody has to stay for others to read: one
+// CTA finishes a row while the others' places go to the next rows.
 #pragma once
 #include "draw.cuh"
 #include "tc_ptx.cuh"
 
 namespace rsv {
 
-constexpr int kDcList = 1024;     // entries of a collection: two per thread
-constexpr int kDcBins = 2048;     // four per thread
-constexpr int kDcFastK = 384;     // most thread maxima asked for, of 512
-constexpr int kDcTryK = 256;      // entries tried for top-p alone
+constexpr int kDcList = 512;  // entries of a collection
+constexpr int kDcPer = kDcList / kDwThreads;
+constexpr int kDcBins = 512;
+constexpr int kDcBinsPer = kDcBins / kDwThreads;
+static_assert(kDcBinsPer == 2, "bins are read in pairs");
+constexpr int kDcFastK = 300;                   // most entries of top-k that are collected whole
+constexpr int kDcMostPart = kDwThreads * 7 / 8;  // most of a CTA's thread maxima that are asked for
+constexpr int kDcTryK = 256;                     // entries tried for top-p alone,
+constexpr int kDcTryPart = kDwThreads * 3 / 8;   // and of one CTA's thread maxima
 constexpr int kDcMaxCtas = 8;
-constexpr int kDcSliceBytes = 64 * 1024;
+constexpr int kDcPlaces = 256;  // noted places of a warp's stretch
+constexpr int kDcSliceBytes = 32 * 1024;  // a CTA's part of a row, as long as eight CTAs suffice
+constexpr int kDcMostSliceBytes = 192 * 1024;
 
+struct DcSums {
+    u64 total, mass, n, from_b, from_c;  // weight of the slice, of its collection, entries collected, weights from the two bounds on
+};
 struct DcShared {
+    // written by the other CTAs
+    float4 top[kDcMaxCtas];  // largest logit (NaN: there is one), smallest of the threads' maxima, two lower bounds
+    DcSums sums[kDcMaxCtas];
+    u64 segs[kDcMaxCtas * kDwWarps];  // weights of the warps' stretches
+    int above[kDcMaxCtas];            // logits above a region
+    u64 left, cut_p;                  // what top-k leaves; 0: the row is done
+    int n_list[3];                    // entries of the collections below (one after the other)
+    alignas(16) u64 list[kDcList];    // key << 32 | ~index
     // read by the other CTAs
-    alignas(16) u64 list[kDcList];  // key << 32 | ~index
-    union {
-        uint32_t hist[kDcBins];
-        u64 keys[kDcList];  // the collections of all CTAs, sorted (this CTA's own copy)
-    };
-    u64 seg[kDwWarps];  // kept weight of every warp's stretch
-    u64 total, mass;    // weight of the slice, and of its collection
-    float mx, thr_all, thr_part;
-    int nan, n_list, n_above;
+    alignas(16) uint32_t hist[kDcBins];
     // this CTA's own
-    double tab[16];
-    u64 wsum[kDwWarps], segs[kDcMaxCtas * kDwWarps];
-    float red[kDwWarps], redmin[kDwWarps];
-    uint32_t wcnt[kDwWarps], tmhist[256], first, key_all, key_part;
-    int cross_all, cross_part, bin, found;
+    alignas(16) u64 mine[kDcList];
+    double tab[16], rate, least;
+    u64 wsum[kDwWarps], seg_a[kDwWarps], seg_b[kDwWarps], seg_c[kDwWarps], before;
+    float red[kDwWarps], redmin[kDwWarps], thr_all, thr_part;
+    uint32_t tmhist[256], first;
+    int n_mine, n_places[kDwWarps], n_above[kDwWarps], bin, found;
+    unsigned short places[kDwWarps][kDcPlaces];  // of the logits in the stretch of values that holds the cut
 };
 
 __device__ __forceinline__ uint32_t dc_rank() {
@@ -57,38 +73,53 @@ __device__ __forceinline__ void dc_sync(int S) {
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 }
+// The two halves of a barrier: a CTA's shared memory may be written to once it has begun.
+__device__ __forceinline__ void dc_arrive(int S) {
+    if (S > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void dc_wait(int S) {
+    if (S > 1) {
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+}
 __device__ __forceinline__ uint32_t dc_map(const void* p, int rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
 }
-__device__ __forceinline__ uint32_t dc_u32(const void* p, int rank) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(dc_map(p, rank)) : "memory");
+__device__ __forceinline__ uint2 dc_u32x2(const void* p, int rank) {
+    uint2 v;
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(dc_map(p, rank)) : "memory");
     return v;
 }
-__device__ __forceinline__ u64 dc_u64(const void* p, int rank) {
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(dc_map(p, rank)) : "memory");
-    return v;
+__device__ __forceinline__ void dc_put(int rank, int* p, int v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dc_map(p, rank)), "r"(v) : "memory"); }
+__device__ __forceinline__ void dc_put(int rank, u64* p, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dc_map(p, rank)), "l"(v) : "memory"); }
+__device__ __forceinline__ void dc_put(int rank, float4* p, const float4& v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dc_map(p, rank)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
-__device__ __forceinline__ uint4 dc_u32x4(const void* p, int rank) {
-    uint4 v;
-    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(dc_map(p, rank)) : "memory");
-    return v;
+__device__ __forceinline__ int dc_add(int rank, int* p, int v) {
+    int before;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(before) : "r"(dc_map(p, rank)), "r"(v) : "memory");
+    return before;
 }
-__device__ __forceinline__ float dc_f32(const void* p, int rank) { return __uint_as_float(dc_u32(p, rank)); }
-
-// A value of every CTA, one per lane, put together (lane c and those eight apart read CTA c's).
-template <typename V, class Read, class Op>
-__device__ __forceinline__ V dc_over(int S, V none, Read&& read, Op&& op) {
-    const int c = threadIdx.x & (kDcMaxCtas - 1);
-    V v = none;
-    if (c < S) v = read(c);
+// A value of every CTA, one per lane (lane c and those eight apart have CTA c's), put together.
+template <typename V, class Op>
+__device__ __forceinline__ V dc_all(V v, Op&& op) {
 #pragma unroll
     for (int o = kDcMaxCtas / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+struct DcMax {
+    __device__ __forceinline__ float operator()(float x, float y) const { return fmaxf(x, y); }
+};
+struct DcMin {
+    __device__ __forceinline__ float operator()(float x, float y) const { return fminf(x, y); }
+};
+struct DcAdd {
+    __device__ __forceinline__ u64 operator()(u64 x, u64 y) const { return x + y; }
+    __device__ __forceinline__ int operator()(int x, int y) const { return x + y; }
+};
 
 template <typename T>
 struct DcVec {
@@ -114,25 +145,13 @@ __device__ __forceinline__ uint32_t dc_lowest(const float*) { return 0xFF800000u
 __device__ __forceinline__ uint32_t dc_lowest(const __half*) { return 0xFC00FC00u; }
 __device__ __forceinline__ uint32_t dc_lowest(const __nv_bfloat16*) { return 0xFF80FF80u; }
 
-// f(logit, place) for the logits of this warp's stretch of the slice
-template <typename T, class F>
-__device__ __forceinline__ void dc_scan(const T* slice, int seg, int warp, int lane, F&& f) {
-    constexpr int N = DcVec<T>::n;
-#pragma unroll 2
-    for (int o = lane * N; o < seg; o += 32 * N) {
-        float v[N];
-        dc_unpack(*reinterpret_cast<const uint4*>(slice + warp * seg + o), v, (const T*)nullptr);
-#pragma unroll
-        for (int e = 0; e < N; ++e) f(v[e], warp * seg + o + e);
-    }
-}
 __device__ __forceinline__ u64 dc_warp_sum(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// Sum over the CTA of the values before this thread's, and over all.
-__device__ __forceinline__ u64 dc_before(u64 v, u64* wsum, u64& all) {
+// Sum over the CTA of the values before this thread's, and over all.  (A function of its own, as the sort: the code of a row is run once, and has to be fetched.)
+__device__ __noinline__ ulonglong2 dc_before2(u64 v, u64* wsum) {
     u64 incl = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -142,57 +161,75 @@ __device__ __forceinline__ u64 dc_before(u64 v, u64* wsum, u64& all) {
     __syncthreads();
     if ((threadIdx.x & 31) == 31) wsum[threadIdx.x >> 5] = incl;
     __syncthreads();
-    u64 base = 0;
-    all = 0;
+    u64 base = 0, sum = 0;
 #pragma unroll
     for (int i = 0; i < kDwWarps; ++i) {
         const u64 t = wsum[i];
         if (i < (int)(threadIdx.x >> 5)) base += t;
-        all += t;
+        sum += t;
     }
-    return base + incl - v;
+    return make_ulonglong2(base + incl - v, sum);
 }
-// keys[0 .. n) in falling order; n a power of two from 32 to 1024
-__device__ __forceinline__ void dc_sort(u64* keys, int n) {
+__device__ __forceinline__ u64 dc_before(u64 v, u64* wsum, u64& all) {
+    const ulonglong2 t = dc_before2(v, wsum);
+    all = t.y;
+    return t.x;
+}
+// keys[0 .. n) in falling order, all different; up to a thread's number by counting the larger ones, more by a bitonic network (space for a power of two).
+__device__ __noinline__ void dc_sort(u64* keys, int n) {
     const int tid = threadIdx.x;
+    if (n <= kDwThreads) {
+        u64 mine = tid < n ? keys[tid] : 0ull;
+        if (tid == 0 && n < kDwThreads) keys[n] = 0;  // (pairs are read)
+        __syncthreads();
+        int place = 0;
+        if (tid < n)
+#pragma unroll 4
+            for (int j = 0; j < n; j += 2) {
+                const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&keys[j]);
+                place += (k.x > mine) + (k.y > mine);
+            }
+        __syncthreads();
+        if (tid < n) keys[place] = mine;
+        __syncthreads();
+        return;
+    }
+    int np = kDwThreads;
+    while (np < n) np <<= 1;
+    for (int i = n + tid; i < np; i += kDwThreads) keys[i] = 0;
+    __syncthreads();
 #pragma unroll 1
-    for (int k = 2; k <= n; k <<= 1)
+    for (int k = 2; k <= np; k <<= 1)
 #pragma unroll 1
         for (int j = k >> 1; j > 0; j >>= 1) {
-            if (tid < n / 2) {
-                const int a = 2 * tid - (tid & (j - 1)), b = a + j;
+#pragma unroll 1
+            for (int i = tid; i < np / 2; i += kDwThreads) {
+                const int a = 2 * i - (i & (j - 1)), b = a + j;
                 const u64 va = keys[a], vb = keys[b];
                 if ((a & k) == 0 ? va < vb : va > vb) {
                     keys[a] = vb;
                     keys[b] = va;
                 }
             }
-            if (j > 32 || (j == 1 && k >= 64))  // (pairs up to 32 apart stay within a warp's 64 entries)
+            if (j > 32 || (j == 1 && k >= 64))  // (pairs up to 32 apart stay within 64 entries, which are always the same warp's)
                 __syncthreads();
             else
                 __syncwarp();
         }
     __syncthreads();
 }
-__device__ __forceinline__ float dc_next(float v, bool up) {
-    const uint32_t b = __float_as_uint(v);
-    if (v == 0.f) return __uint_as_float(up ? 1u : 0x80000001u);
-    return __uint_as_float((v > 0.f) == up ? b + 1 : b - 1);
-}
-// The least logit with y >= ymin.
+// The least logit l (lowest finite .. max) with (l - max) c >= ymin, by a half warp: the quotient, and sixteen floats around it.
 __device__ __forceinline__ float dc_threshold(const DwRow& r, double ymin) {
     const float lowest = -3.402823466e38f;
-    float t = (float)(r.mxd + ymin / r.c);
-    t = t >= lowest ? fminf(t, r.mx) : lowest;  // (the quotient is not a number where T is infinite)
-#pragma unroll 1
-    for (int i = 0; i < 4 && !(dw_y(r, t) >= ymin) && t < r.mx; ++i) t = dc_next(t, true);
-#pragma unroll 1
-    for (int i = 0; i < 4 && t > lowest; ++i) {
-        const float d = dc_next(t, false);
-        if (!(dw_y(r, d) >= ymin)) break;
-        t = d;
-    }
-    return t;
+    float t = (float)(r.mxd + ymin * (double)r.T * 0.69314718055994531);
+    t = t >= lowest ? fminf(t, r.mx) : lowest;
+    const uint32_t b = __float_as_uint(t);
+    int at = b & 0x80000000u ? (int)(0x80000000u - b) : (int)b;  // floats in order, +0 and -0 the same
+    at += (int)(threadIdx.x & 15) - 8;
+    const float v = at < 0 ? __uint_as_float(0x80000000u - (uint32_t)at) : __uint_as_float((uint32_t)at);
+    const bool ok = v <= r.mx && v >= lowest && dw_y(r, v) >= ymin;
+    const uint32_t half = (__ballot_sync(0xffffffffu, ok) >> (threadIdx.x & 16)) & 0xFFFFu;
+    return half ? __shfl_sync(0xffffffffu, v, (threadIdx.x & 16) + __ffs(half) - 1) : t;
 }
 
 template <typename T>
@@ -203,257 +240,319 @@ struct DcRow {
     DwRow r;
     int row, S, rank, n_slice, seg, off, warp, lane, tid;
     float floor_l, min_l;  // least logits with a weight, and that min-p keeps
+    static constexpr int N = DcVec<T>::n;
 
-    __device__ __forceinline__ uint32_t index_of(int c, int place) const { return (uint32_t)(c * n_slice + place - off); }
-    __device__ __forceinline__ u64 weight(float l) const { return l >= floor_l ? dw_fixed(dw_y(r, l), r.F, sh.tab) : 0ull; }
+    __device__ __forceinline__ uint32_t index_of(int place) const { return (uint32_t)(rank * n_slice + place - off); }
+    __device__ __forceinline__ u64 weight(float l) const { return l >= floor_l ? dw_fixed(r, l, sh.tab) : 0ull; }
+    __device__ __forceinline__ u64 weight_of(u64 key) const { return weight(dw_value((uint32_t)(key >> 32))); }
 
-    // Row to shared memory; this thread's largest logit.
-    __device__ __forceinline__ float load(bool& nan) {
-        constexpr int N = DcVec<T>::n;
+    // f(vector, place of its first logit) for this warp's stretch of the slice, whose vectors are as many for all lanes
+    template <class F>
+    __device__ __forceinline__ void scan(F&& f) const {
+#pragma unroll 1
+        for (int o = lane * N; o < seg; o += 32 * N) {
+            float v[N];
+            dc_unpack(*reinterpret_cast<const uint4*>(slice + warp * seg + o), v, (const T*)nullptr);
+            f(v, warp * seg + o);
+        }
+    }
+    // g(logit, weight) for the logits from `least` on; where a warp has one of four, for all of these (weights of logits under floor_l are any number).
+    // Four chains at a time: branches around single ones would put them in a row.  The weights are whole numbers in fp64, and so are a thread's sums of them.
+    template <class G>
+    __device__ __forceinline__ void weights(const float (&v)[N], float least, G&& g) const {
+#pragma unroll 1
+        for (int q = 0; q < N; q += 4) {
+            float l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) l[e] = N == 4 ? v[e] : q ? v[(e + 4) % N] : v[e];
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least)) {
+                double w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = dw_whole(r, l[e], sh.tab);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) g(l[e], w[e]);
+            }
+        }
+    }
+
+    // Logits at `place` of the slice, -inf where the row has none.
+    __device__ __forceinline__ uint4 fetch(const T* lg, int place) const {
+        const int i = rank * n_slice + place - off;
+        if (i >= 0 && i + N <= A.V) return __ldcs(reinterpret_cast<const uint4*>(lg + i));
+        const uint32_t none = dc_lowest((const T*)nullptr);
+        uint4 v = make_uint4(none, none, none, none);
+        if (i + N > 0 && i < A.V) {
+            T* part = slice + place;  // (put together where the vector goes)
+            *reinterpret_cast<uint4*>(part) = v;
+#pragma unroll 1
+            for (int e = 0; e < N; ++e)
+                if (i + e >= 0 && i + e < A.V) part[e] = lg[i + e];
+            v = *reinterpret_cast<uint4*>(part);
+        }
+        return v;
+    }
+    // Row to shared memory; this thread's largest logit.  `meanwhile` runs while the first loads are on their way.
+    template <class F>
+    __device__ __forceinline__ float load(bool& nan, F&& meanwhile) {
+        constexpr int B = 8;
         const T* lg = reinterpret_cast<const T*>(A.logits) + (size_t)row * A.ld;
         off = (int)((reinterpret_cast<uintptr_t>(lg) & 15) / sizeof(T));  // places count from the 16 bytes that the row starts in
         float tm = -INFINITY;
-#pragma unroll 4
-        for (int o = lane * N; o < seg; o += 32 * N) {
-            const int place = warp * seg + o, i = rank * n_slice + place - off;
-            uint4 v;
-            if (i >= 0 && i + N <= A.V) {
-                v = __ldcs(reinterpret_cast<const uint4*>(lg + i));
-            } else {
-                const uint32_t none = dc_lowest((const T*)nullptr);
-                v = make_uint4(none, none, none, none);
-                if (i + N > 0 && i < A.V) {
-                    alignas(16) T part[N];
-                    *reinterpret_cast<uint4*>(part) = v;
+#pragma unroll 1
+        for (int o = lane * N; o < seg; o += 32 * N * B) {
+            uint4 v[B];
 #pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (i + e >= 0 && i + e < A.V) part[e] = lg[i + e];
-                    v = *reinterpret_cast<uint4*>(part);
+            for (int b = 0; b < B; ++b)
+                if (o + 32 * N * b < seg) v[b] = fetch(lg, warp * seg + o + 32 * N * b);
+            if (o < 32 * N) meanwhile();
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                if (o + 32 * N * b < seg) {
+                    float f[N];
+                    dc_unpack(v[b], f, (const T*)nullptr);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        nan |= f[e] != f[e];
+                        tm = fmaxf(tm, f[e]);
+                    }
+                    *reinterpret_cast<uint4*>(slice + warp * seg + o + 32 * N * b) = v[b];
                 }
-            }
-            float f[N];
-            dc_unpack(v, f, (const T*)nullptr);
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                nan |= f[e] != f[e];
-                tm = fmaxf(tm, f[e]);
-            }
-            *reinterpret_cast<uint4*>(slice + place) = v;
         }
         return tm;
     }
 
-    // Lower bounds of the row's k-th largest logit from the threads' maxima: sh.thr_all, sh.thr_part (-inf: none).
+    // Lower bounds of the row's k-th largest logit from the threads' maxima (-inf: none): the k-th of this CTA's, and its (k / CTAs)-th, found to within the
+    // bins of a histogram; a hundredth of a bin is left for rounding (where that is not enough, too few are collected, which is seen).
     __device__ __forceinline__ void bounds(float tm, float mx, float mn, int k) {
         const int part = (k + S - 1) / S;
         const float s = mx > mn ? 255.0f / (mx - mn) : 0.f;
-        int bin = 255;
-        if (tm > -INFINITY) {
-            bin = max(0, min(255, (int)((mx - tm) * s)));
-            atomicAdd(&sh.tmhist[bin], 1u);
-        }
+        if (tm > -INFINITY) atomicAdd(&sh.tmhist[max(0, min(255, (int)((mx - tm) * s)))], 1u);
         __syncthreads();
         if (warp == 0) {
             uint32_t c[8], sum = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum += c[i] = sh.tmhist[lane * 8 + i];
-            uint32_t incl = sum;
+            uint32_t at = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += t;
+                const uint32_t t = __shfl_up_sync(0xffffffffu, at, o);
+                if (lane >= o) at += t;
             }
-            uint32_t at = incl - sum;
+            at -= sum;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (at < (uint32_t)k && at + c[i] >= (uint32_t)k) sh.cross_all = lane * 8 + i;
-                if (at < (uint32_t)part && at + c[i] >= (uint32_t)part) sh.cross_part = lane * 8 + i;
+                const float edge = s > 0.f ? mx - ((float)(lane * 8 + i) + 1.01f) / s : mx;
+                if (at < (uint32_t)k && at + c[i] >= (uint32_t)k) sh.thr_all = edge;
+                if (at < (uint32_t)part && at + c[i] >= (uint32_t)part) sh.thr_part = edge;
                 at += c[i];
             }
         }
         __syncthreads();
-        if (tm > -INFINITY) {
-            const uint32_t key = dw_key(tm);
-            if (bin <= sh.cross_all) atomicMin(&sh.key_all, key);
-            if (bin <= sh.cross_part) atomicMin(&sh.key_part, key);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            sh.thr_all = sh.key_all != ~0u ? dw_value(sh.key_all) : -INFINITY;
-            sh.thr_part = sh.key_part != ~0u ? dw_value(sh.key_part) : -INFINITY;
-        }
     }
 
-    __device__ __forceinline__ void collect(float l, int place) {
-        const int at = atomicAdd(&sh.n_list, 1);
-        if (at < kDcList) sh.list[at] = (u64)dw_key(l) << 32 | (uint32_t)~index_of(rank, place);
-    }
-    // Entries in all CTAs' collections, more than kDcList where one of them ran over.
-    __device__ __forceinline__ int collected() const {
-        return dc_over(S, 0, [&](int c) { return min((int)dc_u32(&sh.n_list, c), kDcList + 1); }, [](int x, int y) { return x + y; });
-    }
-    __device__ __forceinline__ u64 over_ctas(const u64* p) const {
-        return dc_over(S, (u64)0, [&](int c) { return dc_u64(p, c); }, [](u64 x, u64 y) { return x + y; });
-    }
-    // All collections, sorted, to sh.keys.  (Every thread holds entries 2 tid and 2 tid + 1 from here on.)
-    __device__ __forceinline__ void merge(int n, u64 (&key)[2]) {
-        int np = 32, at = 0;
-        while (np < n) np <<= 1;
-#pragma unroll 1
-        for (int c = 0; c < S; ++c) {
-            const int nc = (int)dc_u32(&sh.n_list, c);
-            for (int i = tid; i < nc; i += kDwThreads) sh.keys[at + i] = dc_u64(&sh.list[i], c);
-            at += nc;
-        }
-        for (int i = n + tid; i < np; i += kDwThreads) sh.keys[i] = 0;
-        __syncthreads();
-        dc_sort(sh.keys, np);
+    // The logits that `which` names go into this CTA's collection.
+    template <int E, class F>
+    __device__ __forceinline__ void collect(const float (&v)[E], F&& which, const int (&place)[E]) {
+        uint32_t m = 0;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) key[e] = 2 * tid + e < n ? sh.keys[2 * tid + e] : 0ull;
+        for (int e = 0; e < E; ++e) m |= which(v[e]) ? 1u << e : 0u;
+        if (m) {
+            int at = atomicAdd(&sh.n_mine, __popc(m));
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (m >> e & 1u) {
+                    if (at < kDcList) sh.mine[at] = (u64)dw_key(v[e]) << 32 | (uint32_t)~index_of(place[e]);
+                    ++at;
+                }
+        }
+    }
+    // This CTA's collection to the end of the first CTA's list number c, and its number back to none.  (Too many entries: the number says so.)
+    __device__ __forceinline__ void hand_in(int c) {
+        __syncthreads();
+        const int n = sh.n_mine;
+        if (tid == 0) sh.found = dc_add(0, &sh.n_list[c], n);
+        __syncthreads();
+        const int at = sh.found;
+        if (tid == 0) sh.n_mine = 0;
+#pragma unroll 1
+        for (int i = tid; i < min(n, kDcList); i += kDwThreads)
+            if (at + i < kDcList) dc_put(0, &sh.list[at + i], sh.mine[i]);
+    }
+    // Entries of a sorted list that a thread has: kDcPer consecutive ones, or one where they are no more than threads.
+    __device__ __forceinline__ int entry(int n, int e) const { return n <= kDwThreads ? (e ? kDcList : tid) : kDcPer * tid + e; }
+    __device__ __forceinline__ void sorted(int n, u64 (&key)[kDcPer]) {
+        dc_sort(sh.list, n);
+#pragma unroll
+        for (int e = 0; e < kDcPer; ++e) key[e] = entry(n, e) < n ? sh.list[entry(n, e)] : 0ull;
     }
     // Of the sorted entries those that come before number `most` and before which, with `above` before the first, the weight is under `share` of all that
     // `most` leaves (share <= 0: no such limit; total 0: the sum up to here): how many, their weights, and the sum up to the last of `most`.
-    __device__ __forceinline__ int cut_of(const u64 (&key)[2], int n, int most, u64 above, float share, u64 total, u64 (&w)[2], u64& P, u64& sum) {
-        u64 all, before;
+    __device__ __forceinline__ int cut_of(const u64 (&key)[kDcPer], int n, int most, u64 above, float share, u64 total, u64 (&w)[kDcPer], u64& P, u64& sum) {
+        u64 all, before, own = 0;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) w[e] = 2 * tid + e < min(n, most) ? weight(dw_value((uint32_t)(key[e] >> 32))) : 0ull;
-        before = above + dc_before(w[0] + w[1], sh.wsum, all);
+        for (int e = 0; e < kDcPer; ++e) own += w[e] = entry(n, e) < min(n, most) ? weight_of(key[e]) : 0ull;
+        before = above + dc_before(own, sh.wsum, all);
         sum = above + all;
         P = share > 0.f ? dw_share(share, total ? total : sum) : ~0ull;
-        const int k0 = w[0] && before < P, k1 = w[1] && before + w[0] < P;
-        if (!k0) w[0] = 0;
-        if (!k1) w[1] = 0;
-        return __syncthreads_count(k0) + __syncthreads_count(k1);
+        int kept = 0;
+#pragma unroll
+        for (int e = 0; e < kDcPer; ++e) {
+            const u64 x = w[e];
+            const bool k = x && before < P;
+            if (!k) w[e] = 0;
+            kept += __syncthreads_count(k);
+            before += x;
+        }
+        return kept;
     }
 
-    // The draw among collected entries alone (one CTA): entry e of the thread is kept where its weight is not 0.
-    __device__ __forceinline__ void draw_list(const u64 (&key)[2], u64 (&w)[2], int kept) {
+    // The draw among listed entries alone: an entry is kept where its weight is not 0.
+    __device__ __forceinline__ void draw_list(const u64 (&key)[kDcPer], u64 (&w)[kDcPer], int n, int kept) {
+        u64 own = 0, total;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < kDcPer; ++e) {
             if (w[e] && !(dw_value((uint32_t)(key[e] >> 32)) >= min_l)) w[e] = 0;
-        u64 total, unused = dc_before(w[0] + w[1], sh.wsum, total);
-        (void)unused;
+            own += w[e];
+        }
+        (void)dc_before(own, sh.wsum, total);
         const u64 U = dw_target(A.u[row], total);
-        u64* ws = sh.list;  // (all collections have been read)
+        u64* ws = sh.mine;
         if (kept <= 128) {
             // running sums in vocabulary order by comparing indices
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (2 * tid + e < kept) ws[2 * tid + e] = w[e];
+            for (int e = 0; e < kDcPer; ++e)
+                if (entry(n, e) < kept) ws[entry(n, e)] = w[e];
             __syncthreads();
             if (tid < kept) {
-                const u64 mine = sh.keys[tid];
-                const uint32_t inv = (uint32_t)mine;
+                const u64 k = sh.list[tid];
+                const uint32_t inv = (uint32_t)k;
                 u64 before = 0;
-                for (int j = 0; j < kept; ++j)
-                    if ((uint32_t)sh.keys[j] > inv) before += ws[j];
-                if (ws[tid] && before <= U && before + ws[tid] > U) dw_result(A, row, ~inv, dw_logprob(r, dw_value((uint32_t)(mine >> 32)), total));
+#pragma unroll 4
+                for (int j = 0; j < kept; ++j) before += (uint32_t)sh.list[j] > inv ? ws[j] : 0ull;
+                if (ws[tid] && before <= U && before + ws[tid] > U) dw_result(A, row, ~inv, dw_logprob(r, dw_value((uint32_t)(k >> 32)), total));
             }
             return;
         }
-        // sorted by their index (as ~index << 32 | place, rising index = falling word), then a prefix sum
+        // sorted by their index (~index << 32 | place: a rising index is a falling word), then prefix sums
         __syncthreads();
-        int np = 32;
-        while (np < kept) np <<= 1;
-        for (int i = tid; i < np; i += kDwThreads) ws[i] = i < kept ? (u64)(uint32_t)sh.keys[i] << 32 | (uint32_t)i : 0ull;
+        for (int i = tid; i < kept; i += kDwThreads) ws[i] = (u64)(uint32_t)sh.list[i] << 32 | (uint32_t)i;
         __syncthreads();
-        dc_sort(ws, np);
-        u64 v[2], k2[2];
+        dc_sort(ws, kept);
+        u64 v[kDcPer], sum = 0, all;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int i = 2 * tid + e;
-            k2[e] = i < kept ? sh.keys[(uint32_t)ws[i]] : 0ull;
-            const float l = dw_value((uint32_t)(k2[e] >> 32));
-            v[e] = i < kept && l >= min_l ? weight(l) : 0ull;
+        for (int e = 0; e < kDcPer; ++e) {
+            const int i = entry(kept, e);
+            const float l = i < kept ? dw_value((uint32_t)(sh.list[(uint32_t)ws[i]] >> 32)) : -INFINITY;
+            sum += v[e] = l >= min_l ? weight(l) : 0ull;
         }
-        u64 all, before = dc_before(v[0] + v[1], sh.wsum, all);
+        u64 before = dc_before(sum, sh.wsum, all);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            if (v[e] && before <= U && before + v[e] > U) dw_result(A, row, ~(uint32_t)k2[e], dw_logprob(r, dw_value((uint32_t)(k2[e] >> 32)), total));
+        for (int e = 0; e < kDcPer; ++e) {
+            if (v[e] && before <= U && before + v[e] > U) {
+                const u64 k = sh.list[(uint32_t)ws[entry(kept, e)]];
+                dw_result(A, row, ~(uint32_t)k, dw_logprob(r, dw_value((uint32_t)(k >> 32)), total));
+            }
             before += v[e];
         }
     }
 
-    // The draw among all logits down to `cut` (key << 32 | ~index) and min_l, from the warps' sums in sh.seg of all CTAs and the `kept` entries of a region.
-    __device__ __forceinline__ void draw_segments(u64 cut, int kept) {
+    // The draw among all logits down to `cut` (key << 32 | ~index) and min_l, from the weights of the warps' stretches in sh.segs, to which those of the first
+    // `kept` listed entries are added.  `alone`: one CTA for the row, with that stretch from global memory; otherwise the CTA that has it.  Sums over `limit`:
+    // left to radix passes.
+    __device__ __forceinline__ void draw_segments(u64 cut, int kept, bool alone, u64 limit) {
         const int n = S * kDwWarps;
-        __syncthreads();
-        if (tid < n) sh.segs[tid] = dc_u64(&sh.seg[tid % kDwWarps], tid / kDwWarps);
-        __syncthreads();
+#pragma unroll 1
         for (int i = tid; i < kept; i += kDwThreads) {
-            const u64 k = sh.keys[i];
-            const float l = dw_value((uint32_t)(k >> 32));
+            const u64 k = sh.list[i];
             const int place = (int)~(uint32_t)k + off;
-            if (l >= min_l) atomicAdd(&sh.segs[place / n_slice * kDwWarps + place % n_slice / seg], weight(l));
+            if (dw_value((uint32_t)(k >> 32)) >= min_l) atomicAdd(&sh.segs[place / n_slice * kDwWarps + place % n_slice / seg], weight_of(k));
         }
         __syncthreads();
         u64 total, w = tid < n ? sh.segs[tid] : 0ull;
         const u64 before = dc_before(w, sh.wsum, total);
+        if (total > limit) {
+            if (rank == 0) dw_row_plain<T>(A, row, *reinterpret_cast<DwPlainShared*>(slice));
+            return;
+        }
         const u64 U = dw_target(A.u[row], total);
         if (w && before <= U && before + w > U) {
             sh.found = tid;
-            sh.segs[0] = before;
+            sh.before = before;
         }
         __syncthreads();
-        const int f = sh.found;
-        if (f / kDwWarps != rank) return;
+        const int f = sh.found, c = f / kDwWarps;
+        if (c != rank && !alone) return;
         // that stretch again: consecutive logits per thread
-        const u64 base = sh.segs[0];
-        const int from = part_of(f, tid), to = part_of(f, tid + 1);
-        u64 sum = 0;
-        for (int i = from; i < to; ++i) sum += kept_weight(i, cut);
-        u64 all, b = base + dc_before(sum, sh.wsum, all);
-        if (sum && b <= U && b + sum > U)
-            for (int i = from; i < to; ++i) {
-                b += kept_weight(i, cut);
-                if (b > U) {
-                    dw_result(A, row, index_of(rank, i), dw_logprob(r, dw_f32(slice[i]), total));
-                    break;
+        const T* lg = reinterpret_cast<const T*>(A.logits) + (size_t)row * A.ld;
+        const int lo = f % kDwWarps * seg + (int)((unsigned)seg * (unsigned)tid / (unsigned)kDwThreads),
+                  hi = f % kDwWarps * seg + (int)((unsigned)seg * (unsigned)(tid + 1) / (unsigned)kDwThreads);
+        u64 b = 0;
+#pragma unroll 1
+        for (int turn = 0; turn < 2; ++turn) {
+            u64 sum = 0;
+#pragma unroll 1
+            for (int i = lo; i < hi; ++i) {
+                const int at = c * n_slice + i - off;
+                const float l = c == rank ? dw_f32(slice[i]) : at >= 0 && at < A.V ? dw_f32(lg[at]) : -INFINITY;
+                if (!(l >= min_l && ((u64)dw_key(l) << 32 | (uint32_t)~(uint32_t)at) >= cut)) continue;
+                const u64 x = weight(l);
+                sum += x;
+                if (turn) {
+                    b += x;
+                    if (b > U) {
+                        dw_result(A, row, (uint32_t)at, dw_logprob(r, l, total));
+                        break;
+                    }
                 }
             }
-    }
-    __device__ __forceinline__ int part_of(int f, int t) const { return f % kDwWarps * seg + (int)((unsigned)seg * (unsigned)t / (unsigned)kDwThreads); }
-    __device__ __forceinline__ u64 kept_weight(int place, u64 cut) const {
-        const float l = dw_f32(slice[place]);
-        if (!(l >= min_l)) return 0;
-        return ((u64)dw_key(l) << 32 | (uint32_t)~index_of(rank, place)) >= cut ? weight(l) : 0ull;
+            if (turn) return;
+            u64 all;
+            b = sh.before + dc_before(sum, sh.wsum, all);
+            if (!(sum && b <= U && b + sum > U)) return;
+        }
     }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kDwThreads, 2) draw_cluster_kernel(DrawArgs A, int S, int n_slice) {
+__global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A, int S, int n_slice) {
     extern __shared__ __align__(16) unsigned char dc_smem[];
     DcShared& sh = *reinterpret_cast<DcShared*>(dc_smem);
     DcRow<T> R = {A, sh, reinterpret_cast<T*>(dc_smem + sizeof(DcShared))};
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int N = DcVec<T>::n;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = S > 1 ? (int)dc_rank() : 0;
     R.tid = tid, R.lane = lane, R.warp = warp;
     R.S = S;
-    R.rank = S > 1 ? (int)dc_rank() : 0;
+    R.rank = rank;
     R.row = (int)blockIdx.x / S;
     R.n_slice = n_slice;
     R.seg = n_slice / kDwWarps;
-    R.r = dw_row(A, R.row);
+    dc_arrive(S);
+    R.r = dw_asked(A, R.row);
     DwRow& r = R.r;
-    dw_fill_table(sh.tab);
-    const bool small = A.V <= kDcList;
-    const bool list_k = !r.greedy && !small && r.top_k && r.top_k <= (uint32_t)kDcFastK, list_p = !r.greedy && !small && !r.top_k && r.top_p > 0.f;
-    const bool list = !r.greedy && (small || list_k || list_p);
-    bool binned = !r.greedy && !list && r.top_k;
 
     // ---- the row, its largest logit, bounds of what is kept
-    for (int i = tid; i < kDcBins; i += kDwThreads) sh.hist[i] = 0u;
-    if (tid < 256) sh.tmhist[tid] = 0u;
-    if (tid == 0) {
-        sh.n_list = 0;
-        sh.n_above = 0;
-        sh.key_all = sh.key_part = ~0u;
-        sh.cross_all = sh.cross_part = -1;
-        sh.thr_all = sh.thr_part = -INFINITY;
-        sh.first = kDwNone;
-        sh.total = sh.mass = 0;
-    }
     bool nan = false;
-    const float tm = R.load(nan);
+    const float tm = R.load(nan, [&] {
+        uint4* h = reinterpret_cast<uint4*>(sh.hist);
+        for (int i = tid; i < kDcBins / 4; i += kDwThreads) h[i] = make_uint4(0, 0, 0, 0);
+        sh.tmhist[tid] = 0u;
+        if (tid < kDwWarps) sh.seg_a[tid] = 0, sh.n_places[tid] = 0;
+        dw_fill_table(sh.tab, r.F);
+        if (tid == 0) {
+            sh.n_list[0] = sh.n_list[1] = sh.n_list[2] = sh.n_mine = 0;
+            sh.first = ~0u;
+            sh.thr_all = sh.thr_part = -INFINITY;
+        }
+        if (warp == kDwWarps - 1 && !r.greedy) {
+            const double c = dw_rate(r.T), y = dw_least(r.min_p);
+            if (lane == 0) sh.rate = c, sh.least = y;
+        }
+    });
+    const bool small = A.V <= kDcList;
+    const bool list_k = !r.greedy && !small && r.top_k && r.top_k <= (uint32_t)min(kDcFastK, S * kDcMostPart);
+    const bool list_p = !r.greedy && !small && !r.top_k && r.top_p > 0.f;
+    const bool list = !r.greedy && (small || list_k || list_p);
+    const bool binned_k = !r.greedy && !list && r.top_k;
     float mx = tm, mn = tm > -INFINITY ? tm : INFINITY;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -464,200 +563,315 @@ __global__ void __launch_bounds__(kDwThreads, 2) draw_cluster_kernel(DrawArgs A,
     nan = __syncthreads_or(nan);
 #pragma unroll
     for (int i = 0; i < kDwWarps; ++i) mx = fmaxf(mx, sh.red[i]), mn = fminf(mn, sh.redmin[i]);
-    if (tid == 0) sh.mx = mx, sh.nan = nan;
-    if (list_k || list_p) R.bounds(tm, mx, mn, list_k ? (int)r.top_k : kDcTryK);
+    if (list_k || list_p || binned_k) R.bounds(tm, mx, mn, list_p ? min(kDcTryK, S * kDcTryPart) : (int)r.top_k);
+    dc_wait(S);
+    if (tid < S) dc_put(tid, &sh.top[rank], make_float4(nan ? NAN : mx, mn, sh.thr_all, sh.thr_part));
     dc_sync(S);
-    const float mine = mx;
-    const auto larger = [](float x, float y) { return fmaxf(x, y); };
-    mx = dc_over(S, -INFINITY, [&](int c) { return dc_f32(&sh.mx, c); }, larger);
-    nan = dc_over(S, 0u, [&](int c) { return dc_u32(&sh.nan, c); }, [](uint32_t x, uint32_t y) { return x | y; }) != 0u;
-    const int owner = dc_over(S, S, [&](int c) { return dc_f32(&sh.mx, c) == mx ? c : S; }, [](int x, int y) { return min(x, y); });  // the first CTA with the largest logit
-    const float thr_all = dc_over(S, -INFINITY, [&](int c) { return dc_f32(&sh.thr_all, c); }, larger);
-    const float thr_part = dc_over(S, INFINITY, [&](int c) { return dc_f32(&sh.thr_part, c); }, [](float x, float y) { return fminf(x, y); });
-    if (nan || mx == -INFINITY || r.greedy) {
-        if (nan || mx == -INFINITY) {
-            if (R.rank == 0 && tid == 0) dw_result(A, R.row, kDwNone, nan ? NAN : -INFINITY);
-        } else if (R.rank == owner && mine == mx) {
-            uint32_t best = kDwNone;
-            dc_scan<T>(R.slice, R.seg, warp, lane, [&](float l, int place) {
-                if (l == mx) best = min(best, (uint32_t)place);
-            });
-            best = __reduce_min_sync(0xffffffffu, best);
-            if (lane == 0) atomicMin(&sh.first, best);
-            __syncthreads();
-            if (tid == 0) dw_result(A, R.row, R.index_of(R.rank, (int)sh.first), 0.f);
-        }
-        dc_sync(S);
+    float thr;
+    int owner;  // the first CTA with the largest logit
+    {
+        const float4 t = (lane & 7) < S ? sh.top[lane & 7] : make_float4(-INFINITY, INFINITY, -INFINITY, INFINITY);
+        nan = __any_sync(0xffffffffu, t.x != t.x);
+        mx = dc_all(t.x, DcMax());
+        mn = dc_all(t.y, DcMin());
+        thr = fmaxf(fmaxf(dc_all(t.z, DcMax()), dc_all(t.w, DcMin())), -3.402823466e38f);  // (-inf is never drawn)
+        owner = __ffs(__ballot_sync(0xffffffffu, t.x == mx)) - 1;
+    }
+    if (nan || mx == -INFINITY) {
+        if (rank == 0 && tid == 0) dw_result(A, R.row, kDwNone, nan ? NAN : -INFINITY);
         return;
     }
+    if (r.greedy) {
+        if (rank != owner) return;
+        uint32_t best = kDwNone;
+        R.scan([&](const float (&v)[N], int place) {
+#pragma unroll
+            for (int e = N - 1; e >= 0; --e)
+                if (v[e] == mx) best = min(best, (uint32_t)(place + e));
+        });
+        best = __reduce_min_sync(0xffffffffu, best);
+        if (lane == 0) atomicMin(&sh.first, best);
+        __syncthreads();
+        if (tid == 0) dw_result(A, R.row, R.index_of((int)sh.first), 0.f);
+        return;
+    }
+    const auto left_to_passes = [&] {
+        if (rank == 0) dw_row_plain<T>(A, R.row, *reinterpret_cast<DwPlainShared*>(R.slice));
+    };
+    if (mx == INFINITY) return left_to_passes();
     r.mx = mx;
     r.mxd = (double)mx;
+    r.c = sh.rate;
+    r.ymin = sh.least;
     R.floor_l = dc_threshold(r, -40.0);
     R.min_l = r.ymin > -40.0 ? dc_threshold(r, r.ymin) : R.floor_l;
 
-    bool plain = false;  // left to radix passes
-    u64 total = 0;       // weight of the whole row, where top-p needs it
+    u64 limit = ~0ull;  // (more weight than this in min-p's hands: top-p's cut is further up after all)
+    // ---- list
+    bool binned_p = false;
+    u64 total = 0;                        // weight of all that top-k leaves
+    float from_l = thr, to_l = INFINITY;  // the cut lies from here on, under this
+    const u64* base = nullptr;            // weights of the warps' stretches from to_l on (null: none),
+    u64 base_all = 0;                     // and of all
     if (list) {
-        const float thr = fmaxf(fmaxf(thr_all, thr_part), -3.402823466e38f);  // (-inf is never drawn)
-        u64 sum = 0, mass = 0;
-        dc_scan<T>(R.slice, R.seg, warp, lane, [&](float l, int place) {
-            if (l >= thr) R.collect(l, place);
-            if (list_p && l >= R.floor_l) {
-                const u64 w = dw_fixed(dw_y(r, l), r.F, sh.tab);
-                sum += w;
-                if (l >= thr) mass += w;
-            }
+        // bounds of the other stretches of values: the smallest of the threads' maxima (a fifth of normally distributed logits is larger), and half way to it
+        const float l_c = fmaxf(fminf(mn, thr), R.floor_l), l_b = fmaxf(thr + 0.5f * (fminf(mn, thr) - thr), R.floor_l);
+        double own = 0, own_b = 0, own_c = 0;
+        R.scan([&](const float (&v)[N], int place) {
+            int at[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) at[e] = place + e;
+            R.collect(v, [&](float l) { return l >= thr; }, at);
+            if (list_p)
+                R.weights(v, R.floor_l, [&](float l, double w) {
+                    if (l >= R.floor_l) own += w;
+                    if (l >= l_b) own_b += w;
+                    if (l >= l_c) own_c += w;
+                });
         });
+        u64 sum = (u64)own, sum_b = (u64)own_b, sum_c = (u64)own_c, mass = 0;
         if (list_p) {
             sum = dc_warp_sum(sum);
-            mass = dc_warp_sum(mass);
-            if (lane == 0) atomicAdd(&sh.total, sum), atomicAdd(&sh.mass, mass);
-        }
-        dc_sync(S);
-        const int n = R.collected();
-        bool here = n <= kDcList;
-        if (list_p) {
-            total = R.over_ctas(&sh.total);
-            here = here && R.over_ctas(&sh.mass) >= dw_share(r.top_p, total);
-            binned = !here;
-        } else {
-            plain = !here;
-        }
-        if (here) {
-            if (R.rank == 0) {
-                u64 key[2], w[2], P, sum;
-                R.merge(n, key);
-                const int kept = R.cut_of(key, n, r.top_k ? (int)r.top_k : n, 0, r.top_p, total, w, P, sum);
-                R.draw_list(key, w, kept);
+            sum_b = dc_warp_sum(sum_b);
+            sum_c = dc_warp_sum(sum_c);
+            if (lane == 0) sh.wsum[warp] = sum, sh.seg_b[warp] = sum_b, sh.seg_c[warp] = sum_c;
+            __syncthreads();
+            const int n = min(sh.n_mine, kDcList);
+#pragma unroll
+            for (int e = 0; e < kDcPer; ++e)
+                if (tid + e * kDwThreads < n) {
+                    const u64 k = sh.mine[tid + e * kDwThreads], w = R.weight_of(k);
+                    mass += w;
+                    atomicAdd(&sh.seg_a[((int)~(uint32_t)k + R.off - rank * n_slice) / R.seg], w);
+                }
+            if (warp == 0) {  // (lanes 0-7, 8-15 and 16-23 add up the warps of one sum each)
+                u64 t = lane < 8 ? sh.wsum[lane] : lane < 16 ? sh.seg_b[lane - 8] : lane < 24 ? sh.seg_c[lane - 16] : 0ull;
+                t = dc_all(t, DcAdd());
+                sum = __shfl_sync(0xffffffffu, t, 0);
+                sum_b = __shfl_sync(0xffffffffu, t, 8);
+                sum_c = __shfl_sync(0xffffffffu, t, 16);
             }
-            dc_sync(S);
+            u64 all;
+            (void)dc_before(mass, sh.wsum, all);
+            if (tid < S) {
+                dc_put(tid, &sh.sums[rank].total, sum);
+                dc_put(tid, &sh.sums[rank].mass, all);
+                dc_put(tid, &sh.sums[rank].n, (u64)sh.n_mine);
+                dc_put(tid, &sh.sums[rank].from_b, sum_b);
+                dc_put(tid, &sh.sums[rank].from_c, sum_c);
+            }
+        }
+        R.hand_in(0);
+        dc_sync(S);
+        if (list_p) {
+            const bool one = (lane & 7) < S;
+            const DcSums& o = sh.sums[lane & 7];
+            total = dc_all(one ? o.total : 0ull, DcAdd());
+            mass = dc_all(one ? o.mass : 0ull, DcAdd());
+            sum_b = dc_all(one ? o.from_b : 0ull, DcAdd());
+            sum_c = dc_all(one ? o.from_c : 0ull, DcAdd());
+            const u64 P = dw_share(r.top_p, total);
+            const bool over = dc_all(one ? o.n : 0ull, DcAdd()) > (u64)kDcList;
+            binned_p = over || mass < P;
+            from_l = l_b;
+            if (!over) to_l = thr, base = sh.seg_a, base_all = mass;
+            if (P > sum_b) from_l = l_c, to_l = l_b, base = sh.seg_b, base_all = sum_b;
+            if (P > sum_c) from_l = R.floor_l, to_l = l_c, base = sh.seg_c, base_all = sum_c;
+        }
+        if (!binned_p) {
+            if (rank != 0) return;
+            const int n = sh.n_list[0];
+            if (n > kDcList || n < (int)(list_k ? r.top_k : 0u)) {
+                // (fewer than top-k asks for: there are no more, or the bound was rounded up)
+                if (n > kDcList || thr > -3.402823466e38f) return left_to_passes();
+            }
+            u64 key[kDcPer], w[kDcPer], P, sum;
+            R.sorted(n, key);
+            const int kept = R.cut_of(key, n, r.top_k ? (int)r.top_k : n, 0, r.top_p, total, w, P, sum);
+            R.draw_list(key, w, n, kept);
             return;
         }
     }
-    u64 cut = 0;
-    int kept = 0;
-    bool summed = false;  // sh.seg holds the sums of what lies above the region of the cut
-    if (binned) {
-        // ---- histogram of the distance to the maximum
-        const float s = fminf(((float)kDcBins - 0.5f) / fminf((float)(40.0 / r.c), 3e38f), 1e30f);  // (what has a weight is in a bin)
-        const auto where = [&](float l) { return fmaxf(mx - l, 0.f) * s; };                           // (0 for inf - inf)
-        dc_scan<T>(R.slice, R.seg, warp, lane, [&](float l, int) {
-            const float q = where(l);
-            if (q < (float)kDcBins) atomicAdd(&sh.hist[(int)q], 1u);
+    from_l = fmaxf(from_l, R.floor_l);
+
+    // ---- region
+    if (binned_p || binned_k) {
+        const float top_l = fminf(to_l, mx), span = fminf(top_l - from_l, 2.5f * (mx - mn));  // (in the last bin: all that is further down)
+        const float s = span > 0.f ? fminf(((float)kDcBins - 1.0f) / span, 1e30f) : 1e30f;
+        const auto where = [&](float l) { return fminf((top_l - l) * s, (float)kDcBins - 0.5f); };
+        const auto inside = [&](float l) { return l >= from_l && l < to_l; };
+        R.scan([&](const float (&v)[N], int place) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) m |= inside(v[e]) ? 1u << e : 0u;
+            if (m) {
+                int at = atomicAdd(&sh.n_places[warp], __popc(m));
+#pragma unroll 1
+                do {
+                    const int i = place + __ffs(m) - 1;
+                    m &= m - 1;
+                    if (at < kDcPlaces) sh.places[warp][at] = (unsigned short)(i - warp * R.seg);
+                    ++at;
+                    atomicAdd(&sh.hist[(int)where(dw_f32(R.slice[i]))], 1u);
+                } while (m);
+            }
         });
         dc_sync(S);
-        uint32_t cnt[4] = {0, 0, 0, 0};
+        const int noted = sh.n_places[warp];
+        uint32_t cnt[kDcBinsPer] = {};
 #pragma unroll
         for (int c = 0; c < kDcMaxCtas; ++c)
             if (c < S) {
-                const uint4 h = dc_u32x4(&sh.hist[4 * tid], c);
-                cnt[0] += h.x, cnt[1] += h.y, cnt[2] += h.z, cnt[3] += h.w;
+                const uint2 h = dc_u32x2(&sh.hist[kDcBinsPer * tid], c);
+                cnt[0] += h.x, cnt[1] += h.y;
             }
-        // counts and (nearly) weights before this thread's bins
-        u64 all_cnt;
-        const u64 cnt_before = dc_before(cnt[0] + cnt[1] + cnt[2] + cnt[3], sh.wsum, all_cnt);
-        const float step = -40.0f / ((float)kDcBins - 0.5f);
-        u64 near[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) near[i] = (u64)((float)cnt[i] * exp2f(((float)(4 * tid + i) + 0.5f) * step) * 16777216.0f);
-        u64 near_all;
-        const u64 near_before = dc_before(near[0] + near[1] + near[2] + near[3], sh.wsum, near_all);
-        // One collection: logits of bins b1 .. b2, the weight and number of those before them.
-        auto region = [&](int b1, int b2, u64& above, int& n_above) {
+        // The logits of bins b1 .. b2 to list number c, and the weights of the warps' stretches before them to segs, all in the first CTA.
+        const auto region = [&](int c, int b1, int b2) {
             const float q1 = (float)b1, q2 = (float)(b2 + 1);
-            u64 sum = 0;
-            int na = 0;
-            dc_scan<T>(R.slice, R.seg, warp, lane, [&](float l, int place) {
-                const float q = where(l);
-                if (q < q1) {
-                    ++na;
-                    sum += R.weight(l);
-                } else if (q < q2) {
-                    R.collect(l, place);
+            const bool all = noted > kDcPlaces;
+            const int n = all ? R.seg : noted;
+            double own = 0;
+            int above = 0;
+#pragma unroll 1
+            for (int i = 0; i < n; i += 128) {
+                float l[4];
+                int at[4];
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = i + 32 * e + lane;
+                    at[e] = warp * R.seg + (j < n ? all ? j : (int)sh.places[warp][j] : 0);
+                    l[e] = j < n ? dw_f32(R.slice[at[e]]) : -INFINITY;
+                    any |= inside(l[e]) && where(l[e]) < q1;
                 }
-            });
-            sum = dc_warp_sum(sum);
-            na = __reduce_add_sync(0xffffffffu, na);
+                if (__any_sync(0xffffffffu, any)) {
+                    double w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = dw_whole(r, l[e], sh.tab);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (inside(l[e]) && where(l[e]) < q1) own += w[e], ++above;
+                }
+                R.collect(l, [&](float v) { return inside(v) && where(v) >= q1 && where(v) < q2; }, at);
+            }
+            const u64 sum = dc_warp_sum((u64)own) + (base ? base[warp] : 0ull);
+            above = __reduce_add_sync(0xffffffffu, above);
             if (lane == 0) {
-                sh.seg[warp] = sum;
-                atomicAdd(&sh.n_above, na);
+                dc_put(0, &sh.segs[rank * kDwWarps + warp], sum);
+                sh.n_above[warp] = above;
+            }
+            R.hand_in(c);
+            if (tid == 0) {
+                int t = 0;
+#pragma unroll
+                for (int i = 0; i < kDwWarps; ++i) t += sh.n_above[i];
+                dc_put(0, &sh.above[rank], t);
             }
             dc_sync(S);
-            n_above = dc_over(S, 0, [&](int c) { return (int)dc_u32(&sh.n_above, c); }, [](int x, int y) { return x + y; });
-            (void)dc_before(tid < S * kDwWarps ? dc_u64(&sh.seg[tid % kDwWarps], tid / kDwWarps) : 0ull, sh.wsum, above);
         };
-        auto find_bin = [&](u64 before, const auto (&v)[4], u64 want) {  // the bin where the running sum reaches `want`
-            __syncthreads();
+        const auto find_bin = [&](u64 before, const auto (&v)[kDcBinsPer], u64 want) {  // the bin where the running sum reaches `want`
             if (tid == 0) sh.bin = kDcBins - 1;
             __syncthreads();
             u64 at = before;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (at < want && at + v[i] >= want) sh.bin = 4 * tid + i;
-                at += v[i];
+            for (int i = 0; i < kDcBinsPer; ++i) {
+                if (at < want && at + (u64)v[i] >= want) sh.bin = kDcBinsPer * tid + i;
+                at += (u64)v[i];
             }
             __syncthreads();
             return sh.bin;
         };
-        u64 above = 0, key[2] = {0, 0}, w[2], P = ~0ull, sum;
-        int n_above = 0, n = 0, b1 = 0;
-        bool p_left = r.top_p > 0.f;
-        if (r.top_k && all_cnt > r.top_k) {
-            b1 = find_bin(cnt_before, cnt, r.top_k);
-            region(b1, b1, above, n_above);
-            n = R.collected();
-            plain = n > kDcList;
-            if (!plain) {
-                R.merge(n, key);
-                kept = R.cut_of(key, n, (int)r.top_k - n_above, above, r.top_p, 0, w, P, total);
-                p_left = p_left && above >= P;  // top-p's cut lies further up
+        u64 P = 0;
+        if (binned_k) {
+            u64 sum = 0, all;
+#pragma unroll
+            for (int i = 0; i < kDcBinsPer; ++i) sum += cnt[i];
+            const u64 before = dc_before(sum, sh.wsum, all);
+            // Where fewer logits have a weight (or the bound was rounded up) there is no cut of top-k among them.
+            const bool cut_k = all >= (u64)r.top_k;
+            if (!cut_k && thr >= R.floor_l) {
+                dc_sync(S);  // (the histograms are being read)
+                return left_to_passes();
             }
-        } else if (r.top_k && p_left) {  // top-k keeps all that have a weight
-            region(kDcBins, kDcBins, total, n_above);
-        }
-        if (p_left && !plain) {
+            const int b = cut_k ? find_bin(before, cnt, r.top_k) : kDcBins;
+            if (!(r.top_p > 0.f) && where(R.min_l) < (float)b) goto by_min_p;  // min-p's cut is the stricter one
+            region(1, b, b);
+            u64 key[kDcPer], w[kDcPer];
+            int n = 0, kept = 0;
+            if (rank == 0) {
+                n = sh.n_list[1];
+                u64 above = 0;
+                (void)dc_before(tid < S * kDwWarps ? sh.segs[tid] : 0ull, sh.wsum, above);
+                const int n_above = dc_all((lane & 7) < S ? sh.above[lane & 7] : 0, DcAdd());
+                const bool fits = n <= kDcList;
+                if (fits) {
+                    R.sorted(n, key);
+                    kept = R.cut_of(key, n, cut_k ? (int)r.top_k - n_above : 0, above, r.top_p, 0, w, P, total);
+                }
+                // Where top-p's cut lies further up the others are told what it is a share of.
+                const bool done = !fits || r.top_p <= 0.f || above < P;
+                const bool by_min = fits && r.top_p > 0.f && above < P && where(R.min_l) < (float)b;  // top-p's cut is here, min-p's further up
+                if (r.top_p > 0.f) {  // (without top-p they have left)
+                    if (tid < S) {
+                        dc_put(tid, &sh.left, total);
+                        dc_put(tid, &sh.cut_p, by_min ? ~0ull : done ? 0ull : P);
+                    }
+                    dc_sync(S);
+                }
+                if (!fits) return left_to_passes();
+                if (done && !by_min) return R.draw_segments(kept ? sh.list[kept - 1] : 0ull, kept, true, ~0ull);
+            } else {
+                if (r.top_p <= 0.f) return;
+                dc_sync(S);
+            }
+            P = sh.cut_p;
+            total = sh.left;
+            if (P == 0) return;
+            if (P == ~0ull) goto by_min_p;
+        } else {
             P = dw_share(r.top_p, total);
-            const u64 want = (u64)((double)P * exp2(24.0 - (double)r.F));  // in the units of `near`
-            const int b = find_bin(near_before, near, want > 0 ? want : 1);
-            if (r.top_k) dc_sync(S);  // (the collection before this one may still be read)
-            if (tid == 0) sh.n_list = sh.n_above = 0;
-            __syncthreads();
-            b1 = max(b - 1, 0);
-            region(b1, b + 1, above, n_above);
-            n = R.collected();
-            plain = n > kDcList || above >= P;
-            if (!plain) {
-                R.merge(n, key);
-                kept = R.cut_of(key, n, n, above, r.top_p, total, w, P, sum);
-                plain = sum < P;  // the cut lies further down
+        }
+        {
+            // top-p's cut: the bin that the middles of the bins say, and one more on each side
+            const double unit = exp2(24.0 - (double)r.F);
+            const float step = -(float)r.c / s, first = -(float)((r.mxd - (double)top_l) * r.c);
+            float near[kDcBinsPer];
+            u64 sum = 0, all;
+#pragma unroll
+            for (int i = 0; i < kDcBinsPer; ++i) {
+                near[i] = rintf((float)cnt[i] * exp2f(first + ((float)(kDcBinsPer * tid + i) + 0.5f) * step) * 16777216.0f);
+                sum += (u64)near[i];
             }
-        }
-        if (!plain && kept > 0) {
-            cut = sh.keys[kept - 1];
-            summed = !(where(R.min_l) < (float)b1);  // min-p keeps all that lies above the region
-            if (!summed) kept = 0;
+            const u64 before = dc_before(sum, sh.wsum, all), want = (u64)((double)(P - base_all) * unit);
+            const int b = find_bin(before, near, want > 0 ? want : 1), b1 = max(b - 1, 0);
+            limit = P;
+            if (where(R.min_l) < (float)b1 || R.min_l >= to_l) goto by_min_p;
+            region(2, b1, b + 1);
+            if (rank != 0) return;
+            const int n = sh.n_list[2];
+            u64 above = 0;
+            (void)dc_before(tid < S * kDwWarps ? sh.segs[tid] : 0ull, sh.wsum, above);
+            if (n > kDcList || above >= P) return left_to_passes();
+            u64 key[kDcPer], w[kDcPer], P2, upto;
+            R.sorted(n, key);
+            const int kept = R.cut_of(key, n, n, above, r.top_p, total, w, P2, upto);
+            if (upto < P) return left_to_passes();  // the cut lies further down
+            return R.draw_segments(sh.list[kept - 1], kept, true, ~0ull);
         }
     }
-    if (plain) {
-        if (R.rank == 0) dw_row_plain<T>(A, R.row, *reinterpret_cast<DwPlainShared*>(R.slice));
-        dc_sync(S);
-        return;
-    }
-    if (!summed) {
-        // min-p's cut is the stricter one, or there is no other
-        u64 sum = 0;
-        dc_scan<T>(R.slice, R.seg, warp, lane, [&](float l, int) {
-            if (l >= R.min_l) sum += dw_fixed(dw_y(r, l), r.F, sh.tab);
+by_min_p: {
+    // ---- min-p's cut, or none
+    double own = 0;
+    R.scan([&](const float (&v)[N], int) {
+        R.weights(v, R.min_l, [&](float l, double w) {
+            if (l >= R.min_l) own += w;
         });
-        sum = dc_warp_sum(sum);
-        if (binned) dc_sync(S);  // (the sums of a region may still be read)
-        if (lane == 0) sh.seg[warp] = sum;
-        dc_sync(S);
-        cut = 0;
-        kept = 0;
-    }
-    R.draw_segments(cut, kept);
-    dc_sync(S);  // no CTA leaves while its shared memory may be read
+    });
+    const u64 sum = dc_warp_sum((u64)own);
+    if (lane < S) dc_put(lane, &sh.segs[rank * kDwWarps + warp], sum);
+    dc_sync(S);
+    R.draw_segments(0, 0, false, limit);
+}
 }
 
 }  // namespace rsv
