@@ -33,6 +33,7 @@ constexpr int kDcTryK = 256;                     // entries tried for top-p alon
 constexpr int kDcTryPart = kDwThreads * 3 / 8;   // and of one CTA's thread maxima
 constexpr int kDcMaxCtas = 8;
 constexpr int kDcPlaces = 256;  // noted places of a warp's stretch
+static_assert(kDcMaxCtas * kDwWarps == 64 && kDwWarps == 8, "two stretches a lane; warps add up among eight lanes");
 constexpr int kDcSliceBytes = 32 * 1024;  // a CTA's part of a row, as long as eight CTAs suffice
 constexpr int kDcMostSliceBytes = 192 * 1024;
 
@@ -53,8 +54,8 @@ struct DcShared {
     // this CTA's own
     alignas(16) u64 mine[kDcList];
     double tab[16], rate, least;
-    u64 wsum[kDwWarps], seg_a[kDwWarps], seg_b[kDwWarps], seg_c[kDwWarps], before;
-    float red[kDwWarps], redmin[kDwWarps], thr_all, thr_part;
+    u64 wsum[kDwWarps], seg_a[kDwWarps], seg_b[kDwWarps], seg_c[kDwWarps], before, target, sum;
+    float red[kDwWarps], redmin[kDwWarps], thr_all, thr_part, floor_l, min_l;
     uint32_t tmhist[256], first;
     int n_mine, n_places[kDwWarps], n_above[kDwWarps], bin, found;
     unsigned short places[kDwWarps][kDcPlaces];  // of the logits in the stretch of values that holds the cut
@@ -103,6 +104,22 @@ __device__ __forceinline__ int dc_add(int rank, int* p, int v) {
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(before) : "r"(dc_map(p, rank)), "r"(v) : "memory");
     return before;
 }
+// Largest of three (NaN where one is), and largest and smallest of a warp's.
+__device__ __forceinline__ float dc_max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float dc_warp_max(float v) {
+    float d;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+    return d;
+}
+__device__ __forceinline__ float dc_warp_min(float v) {
+    float d;
+    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+    return d;
+}
 // A value of every CTA, one per lane (lane c and those eight apart have CTA c's), put together.
 template <typename V, class Op>
 __device__ __forceinline__ V dc_all(V v, Op&& op) {
@@ -110,16 +127,18 @@ __device__ __forceinline__ V dc_all(V v, Op&& op) {
     for (int o = kDcMaxCtas / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-struct DcMax {
-    __device__ __forceinline__ float operator()(float x, float y) const { return fmaxf(x, y); }
-};
-struct DcMin {
-    __device__ __forceinline__ float operator()(float x, float y) const { return fminf(x, y); }
-};
 struct DcAdd {
     __device__ __forceinline__ u64 operator()(u64 x, u64 y) const { return x + y; }
     __device__ __forceinline__ int operator()(int x, int y) const { return x + y; }
 };
+
+template <int N>
+__device__ __forceinline__ float dc_largest(const float (&v)[N]) {
+    float m = dc_max3(v[0], v[1], v[2]);
+#pragma unroll
+    for (int e = 3; e + 1 < N; e += 2) m = dc_max3(m, v[e], v[e + 1]);
+    return fmaxf(m, v[N - 1]);
+}
 
 template <typename T>
 struct DcVec {
@@ -246,32 +265,31 @@ struct DcRow {
     __device__ __forceinline__ u64 weight(float l) const { return l >= floor_l ? dw_fixed(r, l, sh.tab) : 0ull; }
     __device__ __forceinline__ u64 weight_of(u64 key) const { return weight(dw_value((uint32_t)(key >> 32))); }
 
-    // f(vector, place of its first logit) for this warp's stretch of the slice, whose vectors are as many for all lanes
+    // f(vector, its largest logit, place of its first) for this warp's stretch of the slice, whose vectors are as many for all lanes
     template <class F>
     __device__ __forceinline__ void scan(F&& f) const {
 #pragma unroll 1
         for (int o = lane * N; o < seg; o += 32 * N) {
             float v[N];
             dc_unpack(*reinterpret_cast<const uint4*>(slice + warp * seg + o), v, (const T*)nullptr);
-            f(v, warp * seg + o);
+            f(v, dc_largest(v), warp * seg + o);
         }
     }
-    // g(logit, weight) for the logits from `least` on; where a warp has one of four, for all of these (weights of logits under floor_l are any number).
-    // Four chains at a time: branches around single ones would put them in a row.  The weights are whole numbers in fp64, and so are a thread's sums of them.
+    // g(logit, weight) for all logits of the vectors where a lane's largest is from `least` on (weights of logits under floor_l are any number).  Four chains at
+    // a time: branches around single ones would put them in a row.  The weights are whole numbers in fp64, and so are a thread's sums of them.
     template <class G>
-    __device__ __forceinline__ void weights(const float (&v)[N], float least, G&& g) const {
+    __device__ __forceinline__ void weights(const float (&v)[N], float largest, float least, G&& g) const {
+        if (!__any_sync(0xffffffffu, largest >= least)) return;
 #pragma unroll 1
         for (int q = 0; q < N; q += 4) {
             float l[4];
+            double w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) l[e] = N == 4 ? v[e] : q ? v[(e + 4) % N] : v[e];
-            if (__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= least)) {
-                double w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = dw_whole(r, l[e], sh.tab);
+            for (int e = 0; e < 4; ++e) w[e] = dw_whole(r, l[e], sh.tab);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) g(l[e], w[e]);
-            }
+            for (int e = 0; e < 4; ++e) g(l[e], w[e]);
         }
     }
 
@@ -291,19 +309,27 @@ struct DcRow {
         }
         return v;
     }
-    // Row to shared memory; this thread's largest logit.  `meanwhile` runs while the first loads are on their way.
+    // Row to shared memory; this thread's largest logit (NaN where there is one).  `meanwhile` runs while the first loads are on their way.
     template <class F>
-    __device__ __forceinline__ float load(bool& nan, F&& meanwhile) {
+    __device__ __forceinline__ float load(F&& meanwhile) {
         constexpr int B = 8;
         const T* lg = reinterpret_cast<const T*>(A.logits) + (size_t)row * A.ld;
         off = (int)((reinterpret_cast<uintptr_t>(lg) & 15) / sizeof(T));  // places count from the 16 bytes that the row starts in
+        const bool whole = rank * n_slice >= off && (rank + 1) * n_slice - off <= A.V;
+        const uint4* src = reinterpret_cast<const uint4*>(lg - off + (ptrdiff_t)rank * n_slice + warp * seg);  // (read where the slice is whole)
         float tm = -INFINITY;
 #pragma unroll 1
         for (int o = lane * N; o < seg; o += 32 * N * B) {
             uint4 v[B];
+            if (whole) {
 #pragma unroll
-            for (int b = 0; b < B; ++b)
-                if (o + 32 * N * b < seg) v[b] = fetch(lg, warp * seg + o + 32 * N * b);
+                for (int b = 0; b < B; ++b)
+                    if (o + 32 * N * b < seg) v[b] = __ldcs(src + o / N + 32 * b);
+            } else {
+#pragma unroll
+                for (int b = 0; b < B; ++b)
+                    if (o + 32 * N * b < seg) v[b] = fetch(lg, warp * seg + o + 32 * N * b);
+            }
             if (o < 32 * N) meanwhile();
 #pragma unroll
             for (int b = 0; b < B; ++b)
@@ -311,10 +337,7 @@ struct DcRow {
                     float f[N];
                     dc_unpack(v[b], f, (const T*)nullptr);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        nan |= f[e] != f[e];
-                        tm = fmaxf(tm, f[e]);
-                    }
+                    for (int e = 0; e < N; e += 2) tm = dc_max3(tm, f[e], f[e + 1]);
                     *reinterpret_cast<uint4*>(slice + warp * seg + o + 32 * N * b) = v[b];
                 }
         }
@@ -468,18 +491,33 @@ struct DcRow {
             if (dw_value((uint32_t)(k >> 32)) >= min_l) atomicAdd(&sh.segs[place / n_slice * kDwWarps + place % n_slice / seg], weight_of(k));
         }
         __syncthreads();
-        u64 total, w = tid < n ? sh.segs[tid] : 0ull;
-        const u64 before = dc_before(w, sh.wsum, total);
+        if (warp == 0) {  // (up to two stretches a lane)
+            const u64 w0 = 2 * lane < n ? sh.segs[2 * lane] : 0ull, w1 = 2 * lane + 1 < n ? sh.segs[2 * lane + 1] : 0ull;
+            u64 upto = w0 + w1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 t = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += t;
+            }
+            const u64 all = __shfl_sync(0xffffffffu, upto, 31), from = upto - w0 - w1;
+            if (all <= limit) {
+                const u64 U = dw_target(A.u[row], all);
+                if (from <= U && upto > U) {
+                    const bool second = from + w0 <= U;
+                    sh.found = 2 * lane + second;
+                    sh.before = second ? from + w0 : from;
+                    sh.target = U;
+                }
+            }
+            if (lane == 0) sh.sum = all;
+        }
+        __syncthreads();
+        const u64 total = sh.sum;
         if (total > limit) {
             if (rank == 0) dw_row_plain<T>(A, row, *reinterpret_cast<DwPlainShared*>(slice));
             return;
         }
-        const u64 U = dw_target(A.u[row], total);
-        if (w && before <= U && before + w > U) {
-            sh.found = tid;
-            sh.before = before;
-        }
-        __syncthreads();
+        const u64 U = sh.target;
         const int f = sh.found, c = f / kDwWarps;
         if (c != rank && !alone) return;
         // that stretch again: consecutive logits per thread
@@ -531,8 +569,7 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
     DwRow& r = R.r;
 
     // ---- the row, its largest logit, bounds of what is kept
-    bool nan = false;
-    const float tm = R.load(nan, [&] {
+    const float tm = R.load([&] {
         uint4* h = reinterpret_cast<uint4*>(sh.hist);
         for (int i = tid; i < kDcBins / 4; i += kDwThreads) h[i] = make_uint4(0, 0, 0, 0);
         sh.tmhist[tid] = 0u;
@@ -553,38 +590,32 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
     const bool list_p = !r.greedy && !small && !r.top_k && r.top_p > 0.f;
     const bool list = !r.greedy && (small || list_k || list_p);
     const bool binned_k = !r.greedy && !list && r.top_k;
-    float mx = tm, mn = tm > -INFINITY ? tm : INFINITY;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-    }
+    float mx = dc_warp_max(tm), mn = dc_warp_min(tm > -INFINITY ? tm : INFINITY);
     if (lane == 0) sh.red[warp] = mx, sh.redmin[warp] = mn;
-    nan = __syncthreads_or(nan);
-#pragma unroll
-    for (int i = 0; i < kDwWarps; ++i) mx = fmaxf(mx, sh.red[i]), mn = fminf(mn, sh.redmin[i]);
+    __syncthreads();
+    mx = dc_warp_max(sh.red[lane & (kDwWarps - 1)]);
+    mn = dc_warp_min(sh.redmin[lane & (kDwWarps - 1)]);
     if (list_k || list_p || binned_k) R.bounds(tm, mx, mn, list_p ? min(kDcTryK, S * kDcTryPart) : (int)r.top_k);
     dc_wait(S);
-    if (tid < S) dc_put(tid, &sh.top[rank], make_float4(nan ? NAN : mx, mn, sh.thr_all, sh.thr_part));
+    if (tid < S) dc_put(tid, &sh.top[rank], make_float4(mx, mn, sh.thr_all, sh.thr_part));
     dc_sync(S);
     float thr;
     int owner;  // the first CTA with the largest logit
     {
         const float4 t = (lane & 7) < S ? sh.top[lane & 7] : make_float4(-INFINITY, INFINITY, -INFINITY, INFINITY);
-        nan = __any_sync(0xffffffffu, t.x != t.x);
-        mx = dc_all(t.x, DcMax());
-        mn = dc_all(t.y, DcMin());
-        thr = fmaxf(fmaxf(dc_all(t.z, DcMax()), dc_all(t.w, DcMin())), -3.402823466e38f);  // (-inf is never drawn)
+        mx = dc_warp_max(t.x);
+        mn = dc_warp_min(t.y);
+        thr = fmaxf(fmaxf(dc_warp_max(t.z), dc_warp_min(t.w)), -3.402823466e38f);  // (-inf is never drawn)
         owner = __ffs(__ballot_sync(0xffffffffu, t.x == mx)) - 1;
     }
-    if (nan || mx == -INFINITY) {
-        if (rank == 0 && tid == 0) dw_result(A, R.row, kDwNone, nan ? NAN : -INFINITY);
+    if (!(mx > -INFINITY)) {  // (a NaN, or nothing to draw)
+        if (rank == 0 && tid == 0) dw_result(A, R.row, kDwNone, mx);
         return;
     }
     if (r.greedy) {
         if (rank != owner) return;
         uint32_t best = kDwNone;
-        R.scan([&](const float (&v)[N], int place) {
+        R.scan([&](const float (&v)[N], float, int place) {
 #pragma unroll
             for (int e = N - 1; e >= 0; --e)
                 if (v[e] == mx) best = min(best, (uint32_t)(place + e));
@@ -603,8 +634,13 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
     r.mxd = (double)mx;
     r.c = sh.rate;
     r.ymin = sh.least;
-    R.floor_l = dc_threshold(r, -40.0);
-    R.min_l = r.ymin > -40.0 ? dc_threshold(r, r.ymin) : R.floor_l;
+    if (warp == 0) {
+        const float a = dc_threshold(r, -40.0), b = r.ymin > -40.0 ? dc_threshold(r, r.ymin) : a;
+        if (lane == 0) sh.floor_l = a, sh.min_l = b;
+    }
+    __syncthreads();
+    R.floor_l = sh.floor_l;
+    R.min_l = sh.min_l;
 
     u64 limit = ~0ull;  // (more weight than this in min-p's hands: top-p's cut is further up after all)
     // ---- list
@@ -617,13 +653,15 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
         // bounds of the other stretches of values: the smallest of the threads' maxima (a fifth of normally distributed logits is larger), and half way to it
         const float l_c = fmaxf(fminf(mn, thr), R.floor_l), l_b = fmaxf(thr + 0.5f * (fminf(mn, thr) - thr), R.floor_l);
         double own = 0, own_b = 0, own_c = 0;
-        R.scan([&](const float (&v)[N], int place) {
-            int at[N];
+        R.scan([&](const float (&v)[N], float largest, int place) {
+            if (largest >= thr) {
+                int at[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) at[e] = place + e;
-            R.collect(v, [&](float l) { return l >= thr; }, at);
+                for (int e = 0; e < N; ++e) at[e] = place + e;
+                R.collect(v, [&](float l) { return l >= thr; }, at);
+            }
             if (list_p)
-                R.weights(v, R.floor_l, [&](float l, double w) {
+                R.weights(v, largest, R.floor_l, [&](float l, double w) {
                     if (l >= R.floor_l) own += w;
                     if (l >= l_b) own_b += w;
                     if (l >= l_c) own_c += w;
@@ -700,10 +738,11 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
         const float s = span > 0.f ? fminf(((float)kDcBins - 1.0f) / span, 1e30f) : 1e30f;
         const auto where = [&](float l) { return fminf((top_l - l) * s, (float)kDcBins - 0.5f); };
         const auto inside = [&](float l) { return l >= from_l && l < to_l; };
-        R.scan([&](const float (&v)[N], int place) {
+        R.scan([&](const float (&v)[N], float largest, int place) {
             uint32_t m = 0;
+            if (largest >= from_l)
 #pragma unroll
-            for (int e = 0; e < N; ++e) m |= inside(v[e]) ? 1u << e : 0u;
+                for (int e = 0; e < N; ++e) m |= inside(v[e]) ? 1u << e : 0u;
             if (m) {
                 int at = atomicAdd(&sh.n_places[warp], __popc(m));
 #pragma unroll 1
@@ -862,8 +901,8 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
 by_min_p: {
     // ---- min-p's cut, or none
     double own = 0;
-    R.scan([&](const float (&v)[N], int) {
-        R.weights(v, R.min_l, [&](float l, double w) {
+    R.scan([&](const float (&v)[N], float largest, int) {
+        R.weights(v, largest, R.min_l, [&](float l, double w) {
             if (l >= R.min_l) own += w;
         });
     });
