@@ -38,7 +38,7 @@ constexpr int kDcSliceBytes = 32 * 1024;  // a CTA's part of a row, as long as e
 constexpr int kDcMostSliceBytes = 192 * 1024;
 
 struct DcSums {
-    u64 total, mass, n, from_b, from_c;  // weight of the slice, of its collection, entries collected, weights from the two bounds on
+    u64 total, n, from_a, from_b, from_c;  // weight of the slice, entries collected, weights from the three bounds on
 };
 struct DcShared {
     // written by the other CTAs
@@ -56,8 +56,9 @@ struct DcShared {
     double tab[16], rate, least;
     u64 wsum[kDwWarps], seg_a[kDwWarps], seg_b[kDwWarps], seg_c[kDwWarps], before, target, sum;
     float red[kDwWarps], redmin[kDwWarps], thr_all, thr_part, floor_l, min_l;
-    uint32_t tmhist[256], first;
-    int n_mine, n_places[kDwWarps], n_above[kDwWarps], bin, found;
+    alignas(16) uint32_t tmhist[256];
+    uint32_t first;
+    int n_mine, n_above[kDwWarps], bin, found;
     unsigned short places[kDwWarps][kDcPlaces];  // of the logits in the stretch of values that holds the cut
 };
 
@@ -164,10 +165,9 @@ __device__ __forceinline__ uint32_t dc_lowest(const float*) { return 0xFF800000u
 __device__ __forceinline__ uint32_t dc_lowest(const __half*) { return 0xFC00FC00u; }
 __device__ __forceinline__ uint32_t dc_lowest(const __nv_bfloat16*) { return 0xFF80FF80u; }
 
+// Sum over the warp of values under 2^52, in two halves.
 __device__ __forceinline__ u64 dc_warp_sum(u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    return ((u64)__reduce_add_sync(0xffffffffu, (uint32_t)(v >> 26)) << 26) + __reduce_add_sync(0xffffffffu, (uint32_t)v & 0x3FFFFFFu);
 }
 // Sum over the CTA of the values before this thread's, and over all.  (A function of its own, as the sort: the code of a row is run once, and has to be fetched.)
 __device__ __noinline__ ulonglong2 dc_before2(u64 v, u64* wsum) {
@@ -352,9 +352,11 @@ struct DcRow {
         if (tm > -INFINITY) atomicAdd(&sh.tmhist[max(0, min(255, (int)((mx - tm) * s)))], 1u);
         __syncthreads();
         if (warp == 0) {
-            uint32_t c[8], sum = 0;
+            const uint4 h0 = reinterpret_cast<const uint4*>(sh.tmhist)[2 * lane], h1 = reinterpret_cast<const uint4*>(sh.tmhist)[2 * lane + 1];
+            const uint32_t c[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
+            uint32_t sum = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += c[i] = sh.tmhist[lane * 8 + i];
+            for (int i = 0; i < 8; ++i) sum += c[i];
             uint32_t at = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -362,9 +364,10 @@ struct DcRow {
                 if (lane >= o) at += t;
             }
             at -= sum;
+            const float width = (mx - mn) / 255.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float edge = s > 0.f ? mx - ((float)(lane * 8 + i) + 1.01f) / s : mx;
+                const float edge = mx > mn ? mx - ((float)(lane * 8 + i) + 1.01f) * width : mx;
                 if (at < (uint32_t)k && at + c[i] >= (uint32_t)k) sh.thr_all = edge;
                 if (at < (uint32_t)part && at + c[i] >= (uint32_t)part) sh.thr_part = edge;
                 at += c[i];
@@ -573,7 +576,6 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
         uint4* h = reinterpret_cast<uint4*>(sh.hist);
         for (int i = tid; i < kDcBins / 4; i += kDwThreads) h[i] = make_uint4(0, 0, 0, 0);
         sh.tmhist[tid] = 0u;
-        if (tid < kDwWarps) sh.seg_a[tid] = 0, sh.n_places[tid] = 0;
         dw_fill_table(sh.tab, r.F);
         if (tid == 0) {
             sh.n_list[0] = sh.n_list[1] = sh.n_list[2] = sh.n_mine = 0;
@@ -651,8 +653,8 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
     u64 base_all = 0;                     // and of all
     if (list) {
         // bounds of the other stretches of values: the smallest of the threads' maxima (a fifth of normally distributed logits is larger), and half way to it
-        const float l_c = fmaxf(fminf(mn, thr), R.floor_l), l_b = fmaxf(thr + 0.5f * (fminf(mn, thr) - thr), R.floor_l);
-        double own = 0, own_b = 0, own_c = 0;
+        const float l_a = fmaxf(thr, R.floor_l), l_c = fmaxf(fminf(mn, thr), R.floor_l), l_b = fmaxf(thr + 0.5f * (fminf(mn, thr) - thr), R.floor_l);
+        double own = 0, own_a = 0, own_b = 0, own_c = 0;
         R.scan([&](const float (&v)[N], float largest, int place) {
             if (largest >= thr) {
                 int at[N];
@@ -663,40 +665,21 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
             if (list_p)
                 R.weights(v, largest, R.floor_l, [&](float l, double w) {
                     if (l >= R.floor_l) own += w;
+                    if (l >= l_a) own_a += w;
                     if (l >= l_b) own_b += w;
                     if (l >= l_c) own_c += w;
                 });
         });
-        u64 sum = (u64)own, sum_b = (u64)own_b, sum_c = (u64)own_c, mass = 0;
         if (list_p) {
-            sum = dc_warp_sum(sum);
-            sum_b = dc_warp_sum(sum_b);
-            sum_c = dc_warp_sum(sum_c);
-            if (lane == 0) sh.wsum[warp] = sum, sh.seg_b[warp] = sum_b, sh.seg_c[warp] = sum_c;
+            const u64 sum = dc_warp_sum((u64)own), sum_a = dc_warp_sum((u64)own_a), sum_b = dc_warp_sum((u64)own_b), sum_c = dc_warp_sum((u64)own_c);
+            if (lane == 0) sh.wsum[warp] = sum, sh.seg_a[warp] = sum_a, sh.seg_b[warp] = sum_b, sh.seg_c[warp] = sum_c;
             __syncthreads();
-            const int n = min(sh.n_mine, kDcList);
-#pragma unroll
-            for (int e = 0; e < kDcPer; ++e)
-                if (tid + e * kDwThreads < n) {
-                    const u64 k = sh.mine[tid + e * kDwThreads], w = R.weight_of(k);
-                    mass += w;
-                    atomicAdd(&sh.seg_a[((int)~(uint32_t)k + R.off - rank * n_slice) / R.seg], w);
-                }
-            if (warp == 0) {  // (lanes 0-7, 8-15 and 16-23 add up the warps of one sum each)
-                u64 t = lane < 8 ? sh.wsum[lane] : lane < 16 ? sh.seg_b[lane - 8] : lane < 24 ? sh.seg_c[lane - 16] : 0ull;
-                t = dc_all(t, DcAdd());
-                sum = __shfl_sync(0xffffffffu, t, 0);
-                sum_b = __shfl_sync(0xffffffffu, t, 8);
-                sum_c = __shfl_sync(0xffffffffu, t, 16);
-            }
-            u64 all;
-            (void)dc_before(mass, sh.wsum, all);
-            if (tid < S) {
-                dc_put(tid, &sh.sums[rank].total, sum);
-                dc_put(tid, &sh.sums[rank].mass, all);
-                dc_put(tid, &sh.sums[rank].n, (u64)sh.n_mine);
-                dc_put(tid, &sh.sums[rank].from_b, sum_b);
-                dc_put(tid, &sh.sums[rank].from_c, sum_c);
+            if (warp == 0) {  // (eight lanes add up the warps of one sum each)
+                const u64* p = lane < 8 ? sh.wsum : lane < 16 ? sh.seg_a : lane < 24 ? sh.seg_b : sh.seg_c;
+                const u64 t = dc_all(p[lane & 7], DcAdd());
+                u64* to = lane < 8 ? &sh.sums[rank].total : lane < 16 ? &sh.sums[rank].from_a : lane < 24 ? &sh.sums[rank].from_b : &sh.sums[rank].from_c;
+                if ((lane & 7) < S) dc_put(lane & 7, to, t);
+                if (lane < S) dc_put(lane, &sh.sums[rank].n, (u64)sh.n_mine);
             }
         }
         R.hand_in(0);
@@ -705,14 +688,12 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
             const bool one = (lane & 7) < S;
             const DcSums& o = sh.sums[lane & 7];
             total = dc_all(one ? o.total : 0ull, DcAdd());
-            mass = dc_all(one ? o.mass : 0ull, DcAdd());
-            sum_b = dc_all(one ? o.from_b : 0ull, DcAdd());
-            sum_c = dc_all(one ? o.from_c : 0ull, DcAdd());
+            const u64 sum_a = dc_all(one ? o.from_a : 0ull, DcAdd()), sum_b = dc_all(one ? o.from_b : 0ull, DcAdd()), sum_c = dc_all(one ? o.from_c : 0ull, DcAdd());
             const u64 P = dw_share(r.top_p, total);
             const bool over = dc_all(one ? o.n : 0ull, DcAdd()) > (u64)kDcList;
-            binned_p = over || mass < P;
+            binned_p = over || sum_a < P;
             from_l = l_b;
-            if (!over) to_l = thr, base = sh.seg_a, base_all = mass;
+            if (P > sum_a) to_l = thr, base = sh.seg_a, base_all = sum_a;
             if (P > sum_b) from_l = l_c, to_l = l_b, base = sh.seg_b, base_all = sum_b;
             if (P > sum_c) from_l = R.floor_l, to_l = l_c, base = sh.seg_c, base_all = sum_c;
         }
@@ -738,25 +719,20 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
         const float s = span > 0.f ? fminf(((float)kDcBins - 1.0f) / span, 1e30f) : 1e30f;
         const auto where = [&](float l) { return fminf((top_l - l) * s, (float)kDcBins - 0.5f); };
         const auto inside = [&](float l) { return l >= from_l && l < to_l; };
+        int noted = 0;  // (the same for the whole warp; an atomic counter takes a warp's lanes one by one)
         R.scan([&](const float (&v)[N], float largest, int place) {
-            uint32_t m = 0;
-            if (largest >= from_l)
+            if (!__any_sync(0xffffffffu, largest >= from_l)) return;
 #pragma unroll
-                for (int e = 0; e < N; ++e) m |= inside(v[e]) ? 1u << e : 0u;
-            if (m) {
-                int at = atomicAdd(&sh.n_places[warp], __popc(m));
-#pragma unroll 1
-                do {
-                    const int i = place + __ffs(m) - 1;
-                    m &= m - 1;
-                    if (at < kDcPlaces) sh.places[warp][at] = (unsigned short)(i - warp * R.seg);
-                    ++at;
-                    atomicAdd(&sh.hist[(int)where(dw_f32(R.slice[i]))], 1u);
-                } while (m);
+            for (int e = 0; e < N; ++e) {
+                const bool in = inside(v[e]);
+                const uint32_t m = __ballot_sync(0xffffffffu, in);
+                const int at = noted + __popc(m & ((1u << lane) - 1u));
+                if (in) atomicAdd(&sh.hist[(int)where(v[e])], 1u);
+                if (in && at < kDcPlaces) sh.places[warp][at] = (unsigned short)(place + e - warp * R.seg);
+                noted += __popc(m);
             }
         });
         dc_sync(S);
-        const int noted = sh.n_places[warp];
         uint32_t cnt[kDcBinsPer] = {};
 #pragma unroll
         for (int c = 0; c < kDcMaxCtas; ++c)
