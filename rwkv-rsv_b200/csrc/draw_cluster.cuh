@@ -6,7 +6,7 @@
 //           logit, and so is the smallest over the CTAs of the (k / CTAs)-th; the logits from the larger of the two on are collected (k and a few more) and
 //           sorted by value and index, and the cut lies among them.  With top-p and no top-k the 256 largest are tried: their weight tells whether
 //           the cut lies among them.
-//   region  Otherwise the cut lies in a stretch of values known from the pass that summed the weights (three stretches, between bounds from the threads'
+//   region  Otherwise the cut lies in a stretch of values known from the pass that summed the weights (three stretches, divided by bounds from the threads'
 //           maxima).  A histogram of that stretch in 512 linear bins says near which bin the cut is; the logits of that bin and its neighbours are
 //           collected and sorted, the weight of all larger ones is summed exactly, and the sums tell whether the cut is there.
 //   neither Where a collection would not fit 512 entries (many equal logits) one CTA does the row by radix passes (dw_row_plain).
@@ -32,13 +32,13 @@ constexpr int kDcMostPart = kDwThreads * 7 / 8;  // most of a CTA's thread maxim
 constexpr int kDcTryK = 256;                     // entries tried for top-p alone,
 constexpr int kDcTryPart = kDwThreads * 3 / 8;   // and of one CTA's thread maxima
 constexpr int kDcMaxCtas = 8;
-constexpr int kDcPlaces = 256;  // noted places of a warp's stretch
+constexpr int kDcMarked = 8;  // vectors a thread can mark the logits of
 static_assert(kDcMaxCtas * kDwWarps == 64 && kDwWarps == 8, "two stretches a lane; warps add up among eight lanes");
 constexpr int kDcSliceBytes = 32 * 1024;  // a CTA's part of a row, as long as eight CTAs suffice
 constexpr int kDcMostSliceBytes = 192 * 1024;
 
 struct DcSums {
-    u64 total, n, from_a, from_b, from_c;  // weight of the slice, entries collected, weights from the three bounds on
+    u64 total, n, from_a, from_c;  // weight of the slice, entries collected, weights from the two bounds on
 };
 struct DcShared {
     // written by the other CTAs
@@ -54,12 +54,11 @@ struct DcShared {
     // this CTA's own
     alignas(16) u64 mine[kDcList];
     double tab[16], rate, least;
-    u64 wsum[kDwWarps], seg_a[kDwWarps], seg_b[kDwWarps], seg_c[kDwWarps], before, target, sum;
+    u64 wsum[kDwWarps], seg_a[kDwWarps], seg_c[kDwWarps], before, target, sum;
     float red[kDwWarps], redmin[kDwWarps], thr_all, thr_part, floor_l, min_l;
     alignas(16) uint32_t tmhist[256];
     uint32_t first;
-    int n_mine, n_above[kDwWarps], bin, found;
-    unsigned short places[kDwWarps][kDcPlaces];  // of the logits in the stretch of values that holds the cut
+    int n_mine, n_above[kDwWarps], bin, bins, found;
 };
 
 __device__ __forceinline__ uint32_t dc_rank() {
@@ -265,14 +264,38 @@ struct DcRow {
     __device__ __forceinline__ u64 weight(float l) const { return l >= floor_l ? dw_fixed(r, l, sh.tab) : 0ull; }
     __device__ __forceinline__ u64 weight_of(u64 key) const { return weight(dw_value((uint32_t)(key >> 32))); }
 
-    // f(vector, its largest logit, place of its first) for this warp's stretch of the slice, whose vectors are as many for all lanes
+    // f(vector, its largest logit, place of its first, its number) for this warp's stretch of the slice, whose vectors are as many for all lanes
     template <class F>
     __device__ __forceinline__ void scan(F&& f) const {
+        int i = 0;
 #pragma unroll 1
         for (int o = lane * N; o < seg; o += 32 * N) {
             float v[N];
             dc_unpack(*reinterpret_cast<const uint4*>(slice + warp * seg + o), v, (const T*)nullptr);
-            f(v, dc_largest(v), warp * seg + o);
+            f(v, dc_largest(v), warp * seg + o, i++);
+        }
+    }
+    // The marks of a vector's logits that `which` names (bit 4 i + e: logit e of a group of four of vector i).
+    template <class F>
+    __device__ __forceinline__ void mark(uint32_t (&marks)[N / 4], const float (&v)[N], int i, F&& which) const {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (which(v[e])) marks[e / 4] |= 1u << (e & 3) << 4 * i;
+    }
+    // f(logit, place) for the marked ones, or, where a stretch is too long for marks, for all.
+    template <class F>
+    __device__ __forceinline__ void each(const uint32_t (&marks)[N / 4], F&& f) const {
+        if (seg <= 32 * N * kDcMarked) {
+#pragma unroll
+            for (int g = 0; g < N / 4; ++g)
+#pragma unroll 1
+                for (uint32_t m = marks[g]; m; m &= m - 1) {
+                    const int b = __ffs(m) - 1, place = warp * seg + (b >> 2) * 32 * N + lane * N + 4 * g + (b & 3);
+                    f(dw_f32(slice[place]), place);
+                }
+        } else {
+#pragma unroll 1
+            for (int o = lane; o < seg; o += 32) f(dw_f32(slice[warp * seg + o]), warp * seg + o);
         }
     }
     // g(logit, weight) for all logits of the vectors where a lane's largest is from `least` on (weights of logits under floor_l are any number).  Four chains at
@@ -376,21 +399,9 @@ struct DcRow {
         __syncthreads();
     }
 
-    // The logits that `which` names go into this CTA's collection.
-    template <int E, class F>
-    __device__ __forceinline__ void collect(const float (&v)[E], F&& which, const int (&place)[E]) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) m |= which(v[e]) ? 1u << e : 0u;
-        if (m) {
-            int at = atomicAdd(&sh.n_mine, __popc(m));
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (m >> e & 1u) {
-                    if (at < kDcList) sh.mine[at] = (u64)dw_key(v[e]) << 32 | (uint32_t)~index_of(place[e]);
-                    ++at;
-                }
-        }
+    __device__ __forceinline__ void collect(float l, int place) {
+        const int at = atomicAdd(&sh.n_mine, 1);
+        if (at < kDcList) sh.mine[at] = (u64)dw_key(l) << 32 | (uint32_t)~index_of(place);
     }
     // This CTA's collection to the end of the first CTA's list number c, and its number back to none.  (Too many entries: the number says so.)
     __device__ __forceinline__ void hand_in(int c) {
@@ -555,7 +566,7 @@ struct DcRow {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A, int S, int n_slice) {
+__global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A, int S, int n_slice) {
     extern __shared__ __align__(16) unsigned char dc_smem[];
     DcShared& sh = *reinterpret_cast<DcShared*>(dc_smem);
     DcRow<T> R = {A, sh, reinterpret_cast<T*>(dc_smem + sizeof(DcShared))};
@@ -617,7 +628,7 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
     if (r.greedy) {
         if (rank != owner) return;
         uint32_t best = kDwNone;
-        R.scan([&](const float (&v)[N], float, int place) {
+        R.scan([&](const float (&v)[N], float, int place, int) {
 #pragma unroll
             for (int e = N - 1; e >= 0; --e)
                 if (v[e] == mx) best = min(best, (uint32_t)(place + e));
@@ -646,40 +657,53 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
 
     u64 limit = ~0ull;  // (more weight than this in min-p's hands: top-p's cut is further up after all)
     // ---- list
-    bool binned_p = false;
+    bool binned_p = false, done_marks = false;
     u64 total = 0;                        // weight of all that top-k leaves
     float from_l = thr, to_l = INFINITY;  // the cut lies from here on, under this
     const u64* base = nullptr;            // weights of the warps' stretches from to_l on (null: none),
     u64 base_all = 0;                     // and of all
+    uint32_t marks[N / 4] = {};           // logits from from_l on
+    const bool marked = R.seg <= 32 * N * kDcMarked;
+    // The bin of a logit from from_l on and under to_l; in the last one: all that is further down.
+    float top_l = 0.f, per_bin = 0.f;
+    const auto set_bins = [&] {
+        top_l = fminf(to_l, mx);
+        const float span = fminf(top_l - from_l, 2.5f * (mx - mn));
+        per_bin = span > 0.f ? fminf(((float)kDcBins - 1.0f) / span, 1e30f) : 1e30f;
+    };
+    const auto where = [&](float l) { return fminf((top_l - l) * per_bin, (float)kDcBins - 0.5f); };
+    const auto count = [&] {
+        R.each(marks, [&](float l, int) {
+            if (l >= from_l && l < to_l) atomicAdd(&sh.hist[(int)where(l)], 1u);
+        });
+    };
     if (list) {
-        // bounds of the other stretches of values: the smallest of the threads' maxima (a fifth of normally distributed logits is larger), and half way to it
-        const float l_a = fmaxf(thr, R.floor_l), l_c = fmaxf(fminf(mn, thr), R.floor_l), l_b = fmaxf(thr + 0.5f * (fminf(mn, thr) - thr), R.floor_l);
-        double own = 0, own_a = 0, own_b = 0, own_c = 0;
-        R.scan([&](const float (&v)[N], float largest, int place) {
-            if (largest >= thr) {
-                int at[N];
+        // the smallest of the threads' maxima bounds the other stretches of values: a fifth of normally distributed logits is larger
+        const float l_a = fmaxf(thr, R.floor_l), l_c = fmaxf(fminf(mn, thr), R.floor_l);
+        double own = 0, own_a = 0, own_c = 0;
+        R.scan([&](const float (&v)[N], float largest, int place, int i) {
+            if (largest >= thr)
 #pragma unroll
-                for (int e = 0; e < N; ++e) at[e] = place + e;
-                R.collect(v, [&](float l) { return l >= thr; }, at);
-            }
-            if (list_p)
+                for (int e = 0; e < N; ++e)
+                    if (v[e] >= thr) R.collect(v[e], place + e);
+            if (list_p) {
                 R.weights(v, largest, R.floor_l, [&](float l, double w) {
                     if (l >= R.floor_l) own += w;
                     if (l >= l_a) own_a += w;
-                    if (l >= l_b) own_b += w;
                     if (l >= l_c) own_c += w;
                 });
+                if (marked) R.mark(marks, v, i, [&](float l) { return l >= l_c; });
+            }
         });
         if (list_p) {
-            const u64 sum = dc_warp_sum((u64)own), sum_a = dc_warp_sum((u64)own_a), sum_b = dc_warp_sum((u64)own_b), sum_c = dc_warp_sum((u64)own_c);
-            if (lane == 0) sh.wsum[warp] = sum, sh.seg_a[warp] = sum_a, sh.seg_b[warp] = sum_b, sh.seg_c[warp] = sum_c;
+            const u64 sum = dc_warp_sum((u64)own), sum_a = dc_warp_sum((u64)own_a), sum_c = dc_warp_sum((u64)own_c);
+            if (lane == 0) sh.wsum[warp] = sum, sh.seg_a[warp] = sum_a, sh.seg_c[warp] = sum_c;
             __syncthreads();
             if (warp == 0) {  // (eight lanes add up the warps of one sum each)
-                const u64* p = lane < 8 ? sh.wsum : lane < 16 ? sh.seg_a : lane < 24 ? sh.seg_b : sh.seg_c;
+                const u64* p = lane < 8 ? sh.wsum : lane < 16 ? sh.seg_a : sh.seg_c;
                 const u64 t = dc_all(p[lane & 7], DcAdd());
-                u64* to = lane < 8 ? &sh.sums[rank].total : lane < 16 ? &sh.sums[rank].from_a : lane < 24 ? &sh.sums[rank].from_b : &sh.sums[rank].from_c;
-                if ((lane & 7) < S) dc_put(lane & 7, to, t);
-                if (lane < S) dc_put(lane, &sh.sums[rank].n, (u64)sh.n_mine);
+                u64* to = lane < 8 ? &sh.sums[rank].total : lane < 16 ? &sh.sums[rank].from_a : lane < 24 ? &sh.sums[rank].from_c : &sh.sums[rank].n;
+                if ((lane & 7) < S) dc_put(lane & 7, to, lane < 24 ? t : (u64)sh.n_mine);
             }
         }
         R.hand_in(0);
@@ -688,13 +712,13 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
             const bool one = (lane & 7) < S;
             const DcSums& o = sh.sums[lane & 7];
             total = dc_all(one ? o.total : 0ull, DcAdd());
-            const u64 sum_a = dc_all(one ? o.from_a : 0ull, DcAdd()), sum_b = dc_all(one ? o.from_b : 0ull, DcAdd()), sum_c = dc_all(one ? o.from_c : 0ull, DcAdd());
+            const u64 sum_a = dc_all(one ? o.from_a : 0ull, DcAdd()), sum_c = dc_all(one ? o.from_c : 0ull, DcAdd());
             const u64 P = dw_share(r.top_p, total);
             const bool over = dc_all(one ? o.n : 0ull, DcAdd()) > (u64)kDcList;
-            binned_p = over || sum_a < P;
-            from_l = l_b;
-            if (P > sum_a) to_l = thr, base = sh.seg_a, base_all = sum_a;
-            if (P > sum_b) from_l = l_c, to_l = l_b, base = sh.seg_b, base_all = sum_b;
+            binned_p = over || P > sum_a;
+            done_marks = P <= sum_c;
+            from_l = l_c, to_l = l_a, base = sh.seg_a, base_all = sum_a;
+            if (P <= sum_a) to_l = INFINITY, base = nullptr, base_all = 0;
             if (P > sum_c) from_l = R.floor_l, to_l = l_c, base = sh.seg_c, base_all = sum_c;
         }
         if (!binned_p) {
@@ -715,23 +739,15 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
 
     // ---- region
     if (binned_p || binned_k) {
-        const float top_l = fminf(to_l, mx), span = fminf(top_l - from_l, 2.5f * (mx - mn));  // (in the last bin: all that is further down)
-        const float s = span > 0.f ? fminf(((float)kDcBins - 1.0f) / span, 1e30f) : 1e30f;
-        const auto where = [&](float l) { return fminf((top_l - l) * s, (float)kDcBins - 0.5f); };
-        const auto inside = [&](float l) { return l >= from_l && l < to_l; };
-        int noted = 0;  // (the same for the whole warp; an atomic counter takes a warp's lanes one by one)
-        R.scan([&](const float (&v)[N], float largest, int place) {
-            if (!__any_sync(0xffffffffu, largest >= from_l)) return;
+        set_bins();
+        if (marked && !done_marks) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const bool in = inside(v[e]);
-                const uint32_t m = __ballot_sync(0xffffffffu, in);
-                const int at = noted + __popc(m & ((1u << lane) - 1u));
-                if (in) atomicAdd(&sh.hist[(int)where(v[e])], 1u);
-                if (in && at < kDcPlaces) sh.places[warp][at] = (unsigned short)(place + e - warp * R.seg);
-                noted += __popc(m);
-            }
-        });
+            for (int g = 0; g < N / 4; ++g) marks[g] = 0;
+            R.scan([&](const float (&v)[N], float largest, int, int i) {
+                if (largest >= from_l) R.mark(marks, v, i, [&](float l) { return l >= from_l; });
+            });
+        }
+        count();
         dc_sync(S);
         uint32_t cnt[kDcBinsPer] = {};
 #pragma unroll
@@ -743,32 +759,17 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
         // The logits of bins b1 .. b2 to list number c, and the weights of the warps' stretches before them to segs, all in the first CTA.
         const auto region = [&](int c, int b1, int b2) {
             const float q1 = (float)b1, q2 = (float)(b2 + 1);
-            const bool all = noted > kDcPlaces;
-            const int n = all ? R.seg : noted;
             double own = 0;
             int above = 0;
-#pragma unroll 1
-            for (int i = 0; i < n; i += 128) {
-                float l[4];
-                int at[4];
-                bool any = false;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = i + 32 * e + lane;
-                    at[e] = warp * R.seg + (j < n ? all ? j : (int)sh.places[warp][j] : 0);
-                    l[e] = j < n ? dw_f32(R.slice[at[e]]) : -INFINITY;
-                    any |= inside(l[e]) && where(l[e]) < q1;
+            R.each(marks, [&](float l, int place) {
+                const float q = where(l);
+                if (l >= from_l && l < to_l && q < q2) {
+                    if (q < q1)
+                        own += dw_whole(r, l, sh.tab), ++above;
+                    else
+                        R.collect(l, place);
                 }
-                if (__any_sync(0xffffffffu, any)) {
-                    double w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = dw_whole(r, l[e], sh.tab);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (inside(l[e]) && where(l[e]) < q1) own += w[e], ++above;
-                }
-                R.collect(l, [&](float v) { return inside(v) && where(v) >= q1 && where(v) < q2; }, at);
-            }
+            });
             const u64 sum = dc_warp_sum((u64)own) + (base ? base[warp] : 0ull);
             above = __reduce_add_sync(0xffffffffu, above);
             if (lane == 0) {
@@ -785,12 +786,16 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
             dc_sync(S);
         };
         const auto find_bin = [&](u64 before, const auto (&v)[kDcBinsPer], u64 want) {  // the bin where the running sum reaches `want`
-            if (tid == 0) sh.bin = kDcBins - 1;
+            if (tid == 0) sh.bin = kDcBins - 1, sh.bins = 1;
             __syncthreads();
             u64 at = before;
+            const int near_by = (int)__reduce_add_sync(0xffffffffu, cnt[0] + cnt[1]);  // logits of the warp's 64 bins
 #pragma unroll
             for (int i = 0; i < kDcBinsPer; ++i) {
-                if (at < want && at + (u64)v[i] >= want) sh.bin = kDcBinsPer * tid + i;
+                if (at < want && at + (u64)v[i] >= want) {
+                    sh.bin = kDcBinsPer * tid + i;
+                    sh.bins = max(1, min(64, 90 * 64 / (near_by + 64)));  // neighbours that make about two hundred logits
+                }
                 at += (u64)v[i];
             }
             __syncthreads();
@@ -847,9 +852,9 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
             P = dw_share(r.top_p, total);
         }
         {
-            // top-p's cut: the bin that the middles of the bins say, and one more on each side
+            // top-p's cut: the bin that the middles of the bins say, and some on each side
             const double unit = exp2(24.0 - (double)r.F);
-            const float step = -(float)r.c / s, first = -(float)((r.mxd - (double)top_l) * r.c);
+            const float step = -(float)r.c / per_bin, first = -(float)((r.mxd - (double)top_l) * r.c);
             float near[kDcBinsPer];
             u64 sum = 0, all;
 #pragma unroll
@@ -858,10 +863,10 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
                 sum += (u64)near[i];
             }
             const u64 before = dc_before(sum, sh.wsum, all), want = (u64)((double)(P - base_all) * unit);
-            const int b = find_bin(before, near, want > 0 ? want : 1), b1 = max(b - 1, 0);
+            const int b = find_bin(before, near, want > 0 ? want : 1), wide = sh.bins, b1 = max(b - wide, 0);
             limit = P;
             if (where(R.min_l) < (float)b1 || R.min_l >= to_l) goto by_min_p;
-            region(2, b1, b + 1);
+            region(2, b1, b + wide);
             if (rank != 0) return;
             const int n = sh.n_list[2];
             u64 above = 0;
@@ -877,7 +882,7 @@ __global__ void __launch_bounds__(kDwThreads, 4) draw_cluster_kernel(DrawArgs A,
 by_min_p: {
     // ---- min-p's cut, or none
     double own = 0;
-    R.scan([&](const float (&v)[N], float largest, int) {
+    R.scan([&](const float (&v)[N], float largest, int, int) {
         R.weights(v, largest, R.min_l, [&](float l, double w) {
             if (l >= R.min_l) own += w;
         });
