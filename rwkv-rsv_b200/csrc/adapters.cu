@@ -1,26 +1,75 @@
 // The entry point of the low-rank adapters (adapters.cuh); see include/rsv_b200.h for the contract.
 #include "adapters.cuh"
 
+#include <algorithm>
+#include <initializer_list>
+
 #include "entry.hpp"
 #include "rsv_b200.h"
 
 namespace rsv {
 
-template <typename X, typename W>
-static void launch_adapters(cudaStream_t stream, const AdapterArgs& P) {
-    adapters_row_kernel<X, W><<<(unsigned)P.rows, kAdThreads, 0, stream>>>(P);
-    RSV_CUDA(cudaGetLastError());
+template <typename X, typename W, int MT>
+static void launch_tiles(cudaStream_t stream, int device, AdapterArgs P) {
+    constexpr int T = 16 * MT, pieces = AdTypes<X, W>::pieces;
+    static_assert(T * kAdMaxRank <= kAdMostCells || MT == 4, "only the largest tile depends on the rank");
+    P.block_rows = std::min(P.rows, kAdBlockRows);
+    const int blocks = (P.rows + P.block_rows - 1) / P.block_rows;
+    P.tiles = std::min(P.block_rows, P.block_rows / T + std::min(P.slots + P.copies, P.block_rows));
+    P.S = kAdMaxCtas;
+    while (P.S > 1 && (int64_t)blocks * P.tiles * P.S > 148 * 4) P.S /= 2;
+    const size_t smem = ad_smem(T, P.rank_cap, pieces);
+    static bool configured[64] = {false};
+    if (device >= 64 || !configured[device]) {
+        RSV_CUDA(cudaFuncSetAttribute(adapters_kernel<X, W, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ad_smem(T, std::min(kAdMaxRank, kAdMostCells / T), pieces)));
+        if (device < 64) configured[device] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((int64_t)blocks * P.tiles * P.S));
+    cfg.blockDim = dim3(kAdThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)P.S;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    RSV_CUDA(cudaLaunchKernelEx(&cfg, adapters_kernel<X, W, MT>, P));
 }
 
-void engine_adapters(cudaStream_t stream, int xtype, int wtype, const AdapterArgs& P) {
-    if (xtype == RSV_F16)
-        launch_adapters<__half, __half>(stream, P);
-    else if (xtype == RSV_BF16)
-        launch_adapters<__nv_bfloat16, __nv_bfloat16>(stream, P);
-    else if (wtype == RSV_F16)
-        launch_adapters<float, __half>(stream, P);
+template <typename X, typename W>
+static void launch_adapters(cudaStream_t stream, int device, AdapterArgs P) {
+    const int each = std::min(P.rows, kAdBlockRows) / std::min(P.slots, std::min(P.rows, kAdBlockRows));  // rows of an adapter, if they are shared evenly
+    if (each >= 48 && 64 * P.rank_cap <= kAdMostCells)
+        launch_tiles<X, W, 4>(stream, device, P);
+    else if (each >= 24)
+        launch_tiles<X, W, 2>(stream, device, P);
     else
-        launch_adapters<float, __nv_bfloat16>(stream, P);
+        launch_tiles<X, W, 1>(stream, device, P);
+}
+
+void engine_adapters(cudaStream_t stream, int device, int xtype, int wtype, AdapterArgs P) {
+    const int xs = xtype == RSV_F32 ? 4 : 2;
+    const auto wide = [](const void* p, int64_t size, std::initializer_list<int64_t> strides) {
+        bool ok = (uintptr_t)p % (4 * size) == 0;
+        for (int64_t s : strides) ok = ok && s % 4 == 0;
+        return ok ? 1 : 0;
+    };
+    P.wide_x = wide(P.x, xs, {P.ldx});
+    P.wide_a = wide(P.a, 2, {P.a_slot, P.a_row});
+    P.wide_b = wide(P.b, 2, {P.b_slot, P.b_row});
+    P.wide_out = wide(P.out, xs, {P.ldout}) && (!P.base || wide(P.base, xs, {P.ldbase}));
+    P.copies = P.base != P.out;
+    P.rank_cap = (P.max_rank + 15) / 16 * 16;
+    if (xtype == RSV_F16)
+        launch_adapters<__half, __half>(stream, device, P);
+    else if (xtype == RSV_BF16)
+        launch_adapters<__nv_bfloat16, __nv_bfloat16>(stream, device, P);
+    else if (wtype == RSV_F16)
+        launch_adapters<float, __half>(stream, device, P);
+    else
+        launch_adapters<float, __nv_bfloat16>(stream, device, P);
 }
 
 // First and one past the last byte of `rows` rows of `cols` elements.
@@ -39,8 +88,8 @@ extern "C" int rsv_adapters_apply(int device, void* stream, const rsv_adapters* 
         if (ad->dtype != RSV_F16 && ad->dtype != RSV_BF16) throw std::runtime_error("adapters: the adapters' dtype must be RSV_F16 or RSV_BF16");
         if (xtype != RSV_F32 && xtype != ad->dtype) throw std::runtime_error("adapters: activations must be RSV_F32 or of the adapters' dtype");
         const int64_t lim = 0x7fffffffLL;
-        if (ad->K < 1 || ad->M < 1 || ad->slots < 1 || ad->K > lim / 8 || ad->M > lim / 8 || ad->slots > 65536)
-            throw std::runtime_error("adapters: K and M must be between 1 and 2^28 - 1, slots between 1 and 65536");
+        if (ad->K < 1 || ad->M < 1 || ad->slots < 1 || ad->K > lim / 8 || ad->M > lim / 8 || ad->slots > kAdMaxSlots)
+            throw std::runtime_error("adapters: K and M must be between 1 and 2^28 - 1, slots between 1 and 4096");
         if (ad->max_rank < 1 || ad->max_rank > kAdMaxRank) throw std::runtime_error("adapters: max_rank must be between 1 and 256");
         if (ad->a_row < 0 || ad->a_slot < 0 || ad->b_row < 0 || ad->b_slot < 0 || x_stride < 0 || base_stride < 0) throw std::runtime_error("adapters: negative stride");
         if (rows < 0 || rows > lim / 64) throw std::runtime_error("adapters: rows must be between 0 and 2^25");
@@ -62,6 +111,6 @@ extern "C" int rsv_adapters_apply(int device, void* stream, const rsv_adapters* 
         DeviceScope on(device);
         AdapterArgs P = {x_dev, index_dev, ad->a, ad->b, ad->ranks, ad->scales, base_dev, out_dev, x_stride, base_stride, out_stride, ad->a_slot, ad->a_row, ad->b_slot, ad->b_row,
                          (int)rows, (int)ad->K, (int)ad->M, (int)ad->slots, (int)ad->max_rank};
-        engine_adapters((cudaStream_t)stream, xtype, ad->dtype, P);
+        engine_adapters((cudaStream_t)stream, device, xtype, ad->dtype, P);
     });
 }

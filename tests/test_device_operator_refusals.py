@@ -32,7 +32,7 @@ def adapters(dtype=1, slots=2, max_rank=8, K=64, M=32, a=P, b=P, xtype=0, x=1 <<
 
 @pytest.mark.parametrize("kw,says", [
     (dict(dtype=0), "adapters' dtype"), (dict(dtype=3), "adapters' dtype"), (dict(xtype=2), "activations"), (dict(dtype=2, xtype=1), "activations"), (dict(K=0), "K and M"),
-    (dict(M=0), "K and M"), (dict(slots=0), "K and M"), (dict(slots=65537), "K and M"), (dict(max_rank=0), "max_rank"), (dict(max_rank=257), "max_rank"),
+    (dict(M=0), "K and M"), (dict(slots=0), "K and M"), (dict(slots=4097), "K and M"), (dict(max_rank=0), "max_rank"), (dict(max_rank=257), "max_rank"),
     (dict(rows=-1), "rows"), (dict(rows=(1 << 25) + 1), "rows"), (dict(ldx=-1), "negative stride"), (dict(a_row=-1), "negative stride"), (dict(b_slot=-1), "negative stride"),
     (dict(ldo=31), "overlap"), (dict(a=None), "null"), (dict(b=None), "null"), (dict(x=None), "null"), (dict(index=None), "null"), (dict(out=None), "null"),
     (dict(x=(1 << 30) + 2), "aligned"), (dict(a=P + 1), "aligned"), (dict(index=P + 2), "aligned"), (dict(scales=P + 2), "aligned"), (dict(out=1 << 30), "out and x overlap"),
