@@ -11,17 +11,18 @@ namespace rsv {
 
 template <typename X, typename W, int MT>
 static void launch_tiles(cudaStream_t stream, int device, AdapterArgs P) {
-    constexpr int T = 16 * MT, pieces = AdTypes<X, W>::pieces;
+    typedef AdShape<X, W, MT> Z;
+    constexpr int T = Z::T;
     static_assert(T * kAdMaxRank <= kAdMostCells || MT == 4, "only the largest tile depends on the rank");
     P.block_rows = std::min(P.rows, kAdBlockRows);
     const int blocks = (P.rows + P.block_rows - 1) / P.block_rows;
     P.tiles = std::min(P.block_rows, P.block_rows / T + std::min(P.slots + P.copies, P.block_rows));
     P.S = kAdMaxCtas;
     while (P.S > 1 && (int64_t)blocks * P.tiles * P.S > 148 * 4) P.S /= 2;
-    const size_t smem = ad_smem(T, P.rank_cap, pieces);
+    const size_t smem = Z::smem(P.rank_cap);
     static bool configured[64] = {false};
     if (device >= 64 || !configured[device]) {
-        RSV_CUDA(cudaFuncSetAttribute(adapters_kernel<X, W, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ad_smem(T, std::min(kAdMaxRank, kAdMostCells / T), pieces)));
+        RSV_CUDA(cudaFuncSetAttribute(adapters_kernel<X, W, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Z::smem(std::min(kAdMaxRank, kAdMostCells / T))));
         if (device < 64) configured[device] = true;
     }
     cudaLaunchConfig_t cfg = {};
@@ -51,15 +52,16 @@ static void launch_adapters(cudaStream_t stream, int device, AdapterArgs P) {
 
 void engine_adapters(cudaStream_t stream, int device, int xtype, int wtype, AdapterArgs P) {
     const int xs = xtype == RSV_F32 ? 4 : 2;
-    const auto wide = [](const void* p, int64_t size, std::initializer_list<int64_t> strides) {
-        bool ok = (uintptr_t)p % (4 * size) == 0;
-        for (int64_t s : strides) ok = ok && s % 4 == 0;
+    const auto at = [](int bytes, const void* p, int64_t size, std::initializer_list<int64_t> strides) {  // rows start at multiples of `bytes`
+        bool ok = (uintptr_t)p % bytes == 0;
+        for (int64_t s : strides) ok = ok && s * size % bytes == 0;
         return ok ? 1 : 0;
     };
-    P.wide_x = wide(P.x, xs, {P.ldx});
-    P.wide_a = wide(P.a, 2, {P.a_slot, P.a_row});
-    P.wide_b = wide(P.b, 2, {P.b_slot, P.b_row});
-    P.wide_out = wide(P.out, xs, {P.ldout}) && (!P.base || wide(P.base, xs, {P.ldbase}));
+    P.wide_x = at(16, P.x, xs, {P.ldx});
+    P.wide_a = at(16, P.a, 2, {P.a_slot, P.a_row});
+    P.wide_b = at(16, P.b, 2, {P.b_slot, P.b_row});
+    P.wide_base = at(16, P.base, xs, {P.ldbase});
+    P.wide_out = at(4 * xs, P.out, xs, {P.ldout});
     P.copies = P.base != P.out;
     P.rank_cap = (P.max_rank + 15) / 16 * 16;
     if (xtype == RSV_F16)

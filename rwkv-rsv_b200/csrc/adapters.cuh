@@ -32,7 +32,8 @@ struct AdapterArgs {
     int rows, K, M, slots, max_rank;
     // launch
     int S, tiles, block_rows, rank_cap;  // CTAs of a cluster; tiles and rows of a block of rows; max_rank rounded up to 16
-    int wide_x, wide_a, wide_b, wide_out;  // four values at a time may be loaded (stored)
+    int wide_x, wide_a, wide_b, wide_base;  // rows start at 16 bytes
+    int wide_out;                           // four values at a time may be stored
     int copies;                            // rows without adapter are written
 };
 
@@ -44,11 +45,10 @@ constexpr int kAdBlockRows = 4096;
 constexpr int kAdMaxCtas = 8;
 constexpr int kAdChunk = 64;  // ranks whose sums a warp holds at a time
 
-template <typename X, typename W>
-struct AdTypes {
-    static constexpr bool wide = sizeof(X) == 4;                                                    // fp32 activations
-    static constexpr int pieces = sizeof(X) == 4 && std::is_same<W, __nv_bfloat16>::value ? 3 : 2;  // 16-bit numbers for a value of t
-};
+constexpr size_t kAdSumBytes = (size_t)kAdWarps * 16 * (kAdChunk + 8) * 4;
+constexpr int kAdMostCells = 8192;  // rows x rank_cap of a tile: t lies where the sums were
+static_assert((kAdMaxSlots + 2) * 2 <= kAdSumBytes && kAdMostCells * 4 <= kAdSumBytes, "the counters lie where the sums go later, and t after them");
+
 __device__ __forceinline__ float ad_f32(float v) { return v; }
 __device__ __forceinline__ float ad_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float ad_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -131,19 +131,34 @@ __device__ __forceinline__ void ad_mma16(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Shared memory: rows | t, this CTA's part [16 MT][rank_cap] fp32 | t's pieces [pieces][16 MT][rank_cap + 8] | sums of the warps (before: counters of the adapters).
-__host__ __device__ constexpr size_t ad_part_bytes(int T, int cap) { return (size_t)T * cap * 4; }
-__host__ __device__ constexpr size_t ad_piece_bytes(int T, int cap, int pieces) { return (size_t)pieces * T * (cap + 8) * 2; }
+// How a tile of 16 MT rows is worked on: the warps are MT groups of rows times KS parts of K or M.
+template <typename X, typename W, int MT>
+struct AdShape {
+    static constexpr bool wide = sizeof(X) == 4;                                                    // fp32 activations
+    static constexpr int pieces = sizeof(X) == 4 && std::is_same<W, __nv_bfloat16>::value ? 3 : 2;  // 16-bit numbers for a value of t
+    static constexpr int T = 16 * MT, KS = kAdWarps / MT;
+    static constexpr int KC = MT == 1 ? 128 : 64;       // k of a stage
+    static constexpr int FW = MT == 4 ? 32 : 16;        // outputs of a warp in a stage
+    static constexpr int FB = FW * KS;                  // ... and of a stage
+    static constexpr int stages = wide && MT == 4 ? 2 : 3;  // (two CTAs fit on an SM)
+    // Bytes from row to row.  A lane reads four values of the row that is its number over four: the rows of a quarter (16-byte reads) or half (8-byte reads)
+    // of a warp lie in different banks when they are 16 or 8 words apart, modulo 32.
+    static constexpr int xld = (KC + 16) * (int)sizeof(X), ald = (KC + 16) * 2, bld = (FB + 16) * (int)sizeof(X);
+    static constexpr int stage1 = T * xld + kAdChunk * ald;
+    __host__ __device__ static constexpr int wld(int ranks16) { return (ranks16 % 32 ? ranks16 : ranks16 + 16) * 2; }
+    __host__ __device__ static constexpr int stage2(int ranks16) { return FB * wld(ranks16) + T * bld; }
+    __host__ __device__ static constexpr size_t part_bytes(int cap) { return (size_t)T * cap * 4; }
+    __host__ __device__ static constexpr size_t piece_bytes(int cap) { return (size_t)pieces * T * wld(cap); }
+    __host__ __device__ static constexpr size_t smem(int cap) {
+        const int s2 = stage2(cap < kAdChunk ? cap : kAdChunk), st = stages * (stage1 > s2 ? stage1 : s2);
+        return 1024 + part_bytes(cap) + piece_bytes(cap) + (st > (int)kAdSumBytes ? st : kAdSumBytes);
+    }
+};
 constexpr int kAdSumLd = kAdChunk + 8;  // (rows eight banks apart)
-constexpr size_t kAdSumBytes = (size_t)kAdWarps * 16 * kAdSumLd * 4;
-constexpr int kAdMostCells = 8192;  // rows x rank_cap of a tile: t lies where the sums were
-static_assert((kAdMaxSlots + 2) * 2 <= kAdSumBytes && kAdMostCells * 4 <= kAdSumBytes, "the counters lie where the sums go later, and t after them");
-__host__ __device__ constexpr size_t ad_smem(int T, int cap, int pieces) { return 1024 + ad_part_bytes(T, cap) + ad_piece_bytes(T, cap, pieces) + kAdSumBytes; }
-
 struct AdTile {
     int rows[64];
     float scale[64];  // 2^e of the row's t, times the adapter's scale
-    int slot, n, wsum[kAdWarps];
+    int slot, n, skip, wsum[kAdWarps];
 };
 static_assert(sizeof(AdTile) <= 1024, "the tile's part of shared memory");
 
@@ -176,19 +191,48 @@ __device__ __forceinline__ int ad_before(int v, int* wsum, int& all) {
 // The rows of tile `tile` of the block of rows; false: there are fewer tiles.
 template <int T>
 __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, int rows, int tile, AdTile& sh, unsigned short* cnt) {
-    const int tid = threadIdx.x, groups = P.slots + 1;  // the last one: rows without adapter
+    const int tid = threadIdx.x, lane = tid & 31, groups = P.slots + 1;  // the last one: rows without adapter
+    const int32_t* ix = P.index + first;
+    if (rows <= 32) {
+        // every warp by itself: a lane has a row, a group is known by its first lane
+        const int a = lane < rows ? ix[lane] : -1;
+        const int mine = lane >= rows ? P.slots + 1 : a >= 0 && a < P.slots ? a : P.slots;
+        const uint32_t same = __match_any_sync(0xffffffffu, mine);
+        const bool leads = __ffs(same) - 1 == lane && lane < rows && (mine < P.slots || P.copies);
+        const int tiles = leads ? (__popc(same) + T - 1) / T : 0;
+        int upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        const uint32_t here = __ballot_sync(0xffffffffu, tile >= upto - tiles && tile < upto);
+        if (!here) return false;
+        const int lead = __ffs(here) - 1, skip = (tile - __shfl_sync(0xffffffffu, upto - tiles, lead)) * T;
+        const uint32_t members = __shfl_sync(0xffffffffu, same, lead);
+        const int place = __popc(members & ((1u << lane) - 1u)) - skip;
+        if (tid < 32) {
+            if (members >> lane & 1u && place >= 0 && place < T) sh.rows[place] = first + lane;
+            if (lane == lead) sh.slot = mine;
+            if (lane == 0) sh.n = min(T, __popc(members) - skip);
+        }
+        __syncthreads();
+        return true;
+    }
+    constexpr int per_thread = kAdBlockRows / kAdThreads;
+    const int each = (rows + kAdThreads - 1) / kAdThreads, i0 = tid * each;
+    int group[per_thread];  // of consecutive rows
+#pragma unroll
+    for (int i = 0; i < per_thread; ++i) {
+        const int a = i < each && i0 + i < rows ? ix[i0 + i] : -2;
+        group[i] = i < each && i0 + i < rows ? (a >= 0 && a < P.slots ? a : P.slots) : -1;
+    }
     for (int i = tid; i < (groups + 1) / 2; i += kAdThreads) reinterpret_cast<uint32_t*>(cnt)[i] = 0;
     if (tid == 0) sh.slot = -1;
     __syncthreads();
-    const int32_t* ix = P.index + first;
-    const auto group = [&](int i) {
-        const int a = ix[i];
-        return a >= 0 && a < P.slots ? a : P.slots;
-    };
-    for (int i = tid; i < rows; i += kAdThreads) {
-        const int g = group(i);
-        atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (g >> 1), g & 1 ? 65536u : 1u);  // (no counter passes 4096)
-    }
+#pragma unroll
+    for (int i = 0; i < per_thread; ++i)
+        if (group[i] >= 0) atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (group[i] >> 1), group[i] & 1 ? 65536u : 1u);  // (no counter passes 4096)
     __syncthreads();
     const int per = (groups + kAdThreads - 1) / kAdThreads, g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     const auto tiles_of = [&](int g) { return g == P.slots && !P.copies ? 0 : ((int)cnt[g] + T - 1) / T; };
@@ -201,98 +245,156 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
             const int t = tiles_of(g);
             if (tile < at + t) {
                 sh.slot = g;
-                sh.n = tile - at;
+                sh.skip = (tile - at) * T;
+                sh.n = min(T, (int)cnt[g] - (tile - at) * T);
                 break;
             }
             at += t;
         }
     __syncthreads();
-    const int mine = sh.slot, skip = sh.n * T;
-    __syncthreads();
-    if (tid == 0) sh.n = min(T, (int)cnt[mine] - skip);
-    const int each = (rows + kAdThreads - 1) / kAdThreads, i0 = min(tid * each, rows), i1 = min(i0 + each, rows);
+    const int mine = sh.slot;
     int n = 0;
-    for (int i = i0; i < i1; ++i) n += group(i) == mine;
-    int place = ad_before(n, sh.wsum, all) - skip;
+#pragma unroll
+    for (int i = 0; i < per_thread; ++i) n += group[i] == mine;
+    int place = ad_before(n, sh.wsum, all) - sh.skip;
     if (n && place < T && place + n > 0)
-        for (int i = i0; i < i1; ++i)
-            if (group(i) == mine) {
-                if (place >= 0 && place < T) sh.rows[place] = first + i;
+#pragma unroll
+        for (int i = 0; i < per_thread; ++i)
+            if (group[i] == mine) {
+                if (place >= 0 && place < T) sh.rows[place] = first + i0 + i;
                 ++place;
             }
     __syncthreads();
     return true;
 }
 
+// 16 bytes to shared memory, of which the first `bytes` exist (the others are 0).
+__device__ __forceinline__ void ad_copy16(void* dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+// `n` values (none for n <= 0) of a row from src on to 16 bytes of shared memory, zeros behind them; `wide`: src is at 16 bytes.
+template <typename E>
+__device__ __forceinline__ void ad_fill16(void* dst, const E* src, int n, bool wide, const E* any) {
+    constexpr int N = 16 / (int)sizeof(E);
+    n = max(0, min(n, N));
+    if (wide) {
+        ad_copy16(dst, n ? src : any, n * (int)sizeof(E));
+        return;
+    }
+    alignas(16) E v[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = e < n ? src[e] : E(0.f);
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+}
+__device__ __forceinline__ void ad_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void ad_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// `count` stages: fill(i) begins to load stage i, use(i) works on it.
+template <int STAGES, class Fill, class Use>
+__device__ __forceinline__ void ad_pipeline(int count, Fill&& fill, Use&& use) {
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+        if (i < count) fill(i);
+        ad_commit();
+    }
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+        ad_wait<STAGES - 2>();
+        __syncthreads();  // stage i is there for all, and the one before it has been used
+        if (i + STAGES - 1 < count) fill(i + STAGES - 1);
+        ad_commit();
+        use(i);
+    }
+    ad_wait<0>();
+    __syncthreads();
+}
+
 template <typename X, typename W, int MT>
 __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) {
-    constexpr int T = 16 * MT, KS = kAdWarps / MT, pieces = AdTypes<X, W>::pieces;
-    constexpr bool wide = AdTypes<X, W>::wide;
-    extern __shared__ __align__(16) unsigned char ad_smem_bytes[];
-    AdTile& sh = *reinterpret_cast<AdTile*>(ad_smem_bytes);
-    const int cap = P.rank_cap, ld16 = cap + 8;
-    float* part = reinterpret_cast<float*>(ad_smem_bytes + 1024);
-    W* t16 = reinterpret_cast<W*>(ad_smem_bytes + 1024 + ad_part_bytes(T, cap));
-    float* sums = reinterpret_cast<float*>(ad_smem_bytes + 1024 + ad_part_bytes(T, cap) + ad_piece_bytes(T, cap, pieces));
+    typedef AdShape<X, W, MT> Z;
+    constexpr int T = Z::T, KS = Z::KS, KC = Z::KC, FW = Z::FW, FB = Z::FB, J = FW / 8, pieces = Z::pieces;
+    extern __shared__ __align__(16) unsigned char ad_smem[];
+    AdTile& sh = *reinterpret_cast<AdTile*>(ad_smem);
+    const int cap = P.rank_cap, pld = Z::wld(cap);
+    float* part = reinterpret_cast<float*>(ad_smem + 1024);
+    unsigned char* t16 = ad_smem + 1024 + Z::part_bytes(cap);
+    unsigned char* stage = t16 + Z::piece_bytes(cap);
+    float* sums = reinterpret_cast<float*>(stage);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3, mt = warp % MT, ks = warp / MT;
     const int S = P.S, rank = S > 1 ? (int)ad_rank() : 0;
     const int job = (int)blockIdx.x / S, block = job / P.tiles, first = block * P.block_rows;
     if (!ad_find_tile<T>(P, first, min(P.block_rows, P.rows - first), job % P.tiles, sh, reinterpret_cast<unsigned short*>(sums))) return;  // (all CTAs of the cluster)
     const int n_rows = sh.n, a = sh.slot;
     const bool has = a < P.slots;
-    const int r_all = !has ? 0 : P.ranks ? max(0, min(__ldg(P.ranks + a), P.max_rank)) : P.max_rank;
-    const float scale = has && P.scales ? __ldg(P.scales + a) : 1.f;
+    const int r_all = !has ? 0 : P.ranks ? max(0, min(__ldg(P.ranks + a), P.max_rank)) : P.max_rank, r16 = (r_all + 15) / 16 * 16;
     const X* xp = reinterpret_cast<const X*>(P.x);
     const X* bp = reinterpret_cast<const X*>(P.base);
     X* op = reinterpret_cast<X*>(P.out);
-    // rows of this lane in the tile's products (rows past the last one repeat it and are not stored)
-    const int64_t row0 = sh.rows[min(16 * mt + g, n_rows - 1)], row1 = sh.rows[min(16 * mt + g + 8, n_rows - 1)];
 
     if (r_all > 0) {
-        // ---- t = A x: this CTA's part of K
-        const int units = (P.K + 15) / 16, u0 = (int)((long long)units * rank / S), u1 = (int)((long long)units * (rank + 1) / S);
-        const int v0 = u0 + (u1 - u0) * ks / KS, v1 = u0 + (u1 - u0) * (ks + 1) / KS;
-        const X *x0 = xp + row0 * P.ldx, *x1 = xp + row1 * P.ldx;
+        // ---- t = A x: this CTA's part of K, 64 k and more at a time through shared memory
+        const int units = (P.K + 63) / 64, k_from = 64 * (int)((long long)units * rank / S), k_to = min(P.K, 64 * (int)((long long)units * (rank + 1) / S));
+        const int count = (max(k_to - k_from, 0) + KC - 1) / KC;
         const W* wa = reinterpret_cast<const W*>(P.a) + a * P.a_slot;
 #pragma unroll 1
         for (int c0 = 0; c0 < r_all; c0 += kAdChunk) {
-            const int nt = (min(kAdChunk, r_all - c0) + 7) / 8;
+            const int ranks = min(kAdChunk, r_all - c0), nt = (ranks + 7) / 8;
             float acc[kAdChunk / 8][4];
 #pragma unroll
             for (int j = 0; j < kAdChunk / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-            const W* wr = wa + (int64_t)min(c0 + g, r_all - 1) * P.a_row;
-#pragma unroll 1
-            for (int v = v0; v < v1; ++v) {
-                // A lane has four consecutive k of every row; the products do not mind in which order the tensor core takes them, as long as both operands agree.
-                const int k = 16 * v + 4 * q, left = P.K - k;
-                uint2 w[kAdChunk / 8];
+            __syncthreads();  // (the counters, or the sums before these, have been read)
+            const auto fill = [&](int i) {
+                unsigned char* xs = stage + i % Z::stages * Z::stage1;
+                unsigned char* ws = xs + T * Z::xld;
+                const int k0 = k_from + i * KC;
+                constexpr int XN = 16 / (int)sizeof(X), XU = KC / XN, WU = KC / 8;  // values of 16 bytes, and those of a row
 #pragma unroll
-                for (int j = 0; j < kAdChunk / 8; ++j)
-                    if (j < nt) w[j] = c0 + 8 * j + g < r_all ? ad_load4(wr + (int64_t)8 * j * P.a_row + k, left, P.wide_a) : make_uint2(0u, 0u);
-                const auto y0 = ad_load4(x0 + k, left, P.wide_x), y1 = ad_load4(x1 + k, left, P.wide_x);
-                if constexpr (wide) {
-                    const float f[2][4] = {{y0.x, y0.y, y0.z, y0.w}, {y1.x, y1.y, y1.z, y1.w}};
-                    uint32_t hi[2][4], lo[2][4];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) ad_split(f[i >> 2][i & 3], hi[i >> 2][i & 3], lo[i >> 2][i & 3]);
-#pragma unroll
-                    for (int j = 0; j < kAdChunk / 8; ++j)
-                        if (j < nt) {
-                            const float4 b = ad_floats(w[j], (const W*)nullptr);
-                            const uint32_t b0 = __float_as_uint(b.x), b1 = __float_as_uint(b.y), b2 = __float_as_uint(b.z), b3 = __float_as_uint(b.w);
-                            ad_mma_tf32(acc[j], lo[0][0], lo[1][0], lo[0][1], lo[1][1], b0, b1);
-                            ad_mma_tf32(acc[j], lo[0][2], lo[1][2], lo[0][3], lo[1][3], b2, b3);
-                            ad_mma_tf32(acc[j], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b0, b1);
-                            ad_mma_tf32(acc[j], hi[0][2], hi[1][2], hi[0][3], hi[1][3], b2, b3);
-                        }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < kAdChunk / 8; ++j)
-                        if (j < nt) ad_mma16(acc[j], y0.x, y1.x, y0.y, y1.y, w[j].x, w[j].y, (const W*)nullptr);
+                for (int v = tid; v < T * XU; v += kAdThreads) {
+                    const int row = v / XU, k = k0 + v % XU * XN;
+                    ad_fill16(xs + row * Z::xld + v % XU * 16, xp + (int64_t)sh.rows[min(row, n_rows - 1)] * P.ldx + k, row < n_rows ? k_to - k : 0, P.wide_x, xp);
                 }
-            }
+                for (int v = tid; v < 8 * nt * WU; v += kAdThreads) {
+                    const int row = v / WU, k = k0 + v % WU * 8;
+                    ad_fill16(ws + row * Z::ald + v % WU * 16, wa + (int64_t)min(c0 + row, r_all - 1) * P.a_row + k, row < ranks ? k_to - k : 0, P.wide_a, wa);
+                }
+            };
+            ad_pipeline<Z::stages>(count, fill, [&](int i) {
+                const unsigned char* xs = stage + i % Z::stages * Z::stage1 + (16 * mt + g) * Z::xld;
+                const unsigned char* ws = stage + i % Z::stages * Z::stage1 + T * Z::xld + g * Z::ald;
+                // A lane has four consecutive k of every row; the products do not mind in which order the tensor core takes them, as long as both operands agree.
+#pragma unroll
+                for (int s = 0; s < KC / 16 / KS; ++s) {
+                    const int k = 16 * (ks + KS * s) + 4 * q;
+                    if constexpr (Z::wide) {
+                        const float4 y0 = *reinterpret_cast<const float4*>(xs + k * 4), y1 = *reinterpret_cast<const float4*>(xs + 8 * Z::xld + k * 4);
+                        const float f[2][4] = {{y0.x, y0.y, y0.z, y0.w}, {y1.x, y1.y, y1.z, y1.w}};
+                        uint32_t hi[2][4], lo[2][4];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) ad_split(f[e >> 2][e & 3], hi[e >> 2][e & 3], lo[e >> 2][e & 3]);
+#pragma unroll
+                        for (int j = 0; j < kAdChunk / 8; ++j)
+                            if (j < nt) {
+                                const float4 b = ad_floats(*reinterpret_cast<const uint2*>(ws + 8 * j * Z::ald + k * 2), (const W*)nullptr);
+                                const uint32_t b0 = __float_as_uint(b.x), b1 = __float_as_uint(b.y), b2 = __float_as_uint(b.z), b3 = __float_as_uint(b.w);
+                                ad_mma_tf32(acc[j], lo[0][0], lo[1][0], lo[0][1], lo[1][1], b0, b1);
+                                ad_mma_tf32(acc[j], lo[0][2], lo[1][2], lo[0][3], lo[1][3], b2, b3);
+                                ad_mma_tf32(acc[j], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b0, b1);
+                                ad_mma_tf32(acc[j], hi[0][2], hi[1][2], hi[0][3], hi[1][3], b2, b3);
+                            }
+                    } else {
+                        const uint2 y0 = *reinterpret_cast<const uint2*>(xs + k * 2), y1 = *reinterpret_cast<const uint2*>(xs + 8 * Z::xld + k * 2);
+#pragma unroll
+                        for (int j = 0; j < kAdChunk / 8; ++j)
+                            if (j < nt) {
+                                const uint2 b = *reinterpret_cast<const uint2*>(ws + 8 * j * Z::ald + k * 2);
+                                ad_mma16(acc[j], y0.x, y1.x, y0.y, y1.y, b.x, b.y, (const W*)nullptr);
+                            }
+                    }
+                }
+            });
             // the warps' sums meet: sums[ks][row][rank]
-            __syncthreads();  // (the counters, or the chunk before this one, have been read)
 #pragma unroll
             for (int j = 0; j < kAdChunk / 8; ++j)
                 if (j < nt) {
@@ -301,7 +403,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                     *reinterpret_cast<float2*>(s0 + 8 * kAdSumLd) = make_float2(acc[j][2], acc[j][3]);
                 }
             __syncthreads();
-            const int cols = (min(kAdChunk, r_all - c0) + 15) / 16 * 16;  // (ranks behind the last one: zeros)
+            const int cols = (ranks + 15) / 16 * 16;  // (ranks behind the last one: zeros)
             for (int i = tid; i < T * cols / 4; i += kAdThreads) {
                 const int row = i / (cols / 4), c = i % (cols / 4) * 4;
                 float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -315,113 +417,143 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             }
         }
         // ---- the CTAs' parts meet, and become 16-bit operands
+        const float scale = P.scales ? __ldg(P.scales + a) : 1.f;
         if (S > 1) {
             __syncwarp();
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         } else {
             __syncthreads();
         }
-        const int r16 = (r_all + 15) / 16 * 16;
         constexpr int TPR = kAdThreads / T;  // threads of a row
-        {
-            const int row = tid / TPR, c = tid % TPR;
-            float most = 0.f;
-            for (int i = 4 * c; i < r16; i += 4 * TPR) {
-                float4 s = *reinterpret_cast<const float4*>(part + row * cap + i);
-                if (S > 1) {
-                    s = make_float4(0.f, 0.f, 0.f, 0.f);
-                    const uint32_t at = smem_u32(part + row * cap + i);
+        const int row = tid / TPR, c = tid % TPR;
+        float most = 0.f;
+        for (int i = 4 * c; i < r16; i += 4 * TPR) {
+            float4 s = *reinterpret_cast<const float4*>(part + row * cap + i);
+            if (S > 1) {
+                s = make_float4(0.f, 0.f, 0.f, 0.f);
+                const uint32_t at = smem_u32(part + row * cap + i);
+                float4 v[kAdMaxCtas];
 #pragma unroll
-                    for (int p = 0; p < kAdMaxCtas; ++p)
-                        if (p < S) {
-                            uint32_t from;
-                            float4 v;
-                            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(p));
-                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(from) : "memory");
-                            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-                        }
-                }
-                most = fmaxf(most, fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w))));
-                *reinterpret_cast<float4*>(sums + row * cap + i) = s;
-            }
-#pragma unroll
-            for (int o = TPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            // fp16: relative to a power of two from the row's largest on
-            float up = 1.f, down = 1.f;
-            if (std::is_same<W, __half>::value && most > 0.f && most < INFINITY) {
-                const int e = min(max((int)(__float_as_uint(most) >> 23) - 126, -120), 126);
-                up = __uint_as_float((uint32_t)(127 + e) << 23);
-                down = __uint_as_float((uint32_t)(127 - e) << 23);
-            }
-            if (c == 0) sh.scale[row] = up * scale;
-            __syncwarp();
-            for (int i = 4 * c; i < r16; i += 4 * TPR) {
-                const float4 s = *reinterpret_cast<const float4*>(sums + row * cap + i);
-                float f[4] = {s.x * down, s.y * down, s.z * down, s.w * down};
-#pragma unroll
-                for (int p = 0; p < pieces; ++p) {
-                    W h[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        h[e] = ad_round<W>(f[e]);
-                        const float b = ad_f32(h[e]);
-                        f[e] = fabsf(b) == INFINITY ? 0.f : f[e] - b;
+                for (int p = 0; p < kAdMaxCtas; ++p)
+                    if (p < S) {
+                        uint32_t from;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(p));
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[p].x), "=f"(v[p].y), "=f"(v[p].z), "=f"(v[p].w) : "r"(from) : "memory");
                     }
-                    *reinterpret_cast<uint2*>(t16 + (size_t)(p * T + row) * ld16 + i) = *reinterpret_cast<const uint2*>(h);
+#pragma unroll
+                for (int p = 0; p < kAdMaxCtas; ++p)
+                    if (p < S) s.x += v[p].x, s.y += v[p].y, s.z += v[p].z, s.w += v[p].w;
+            }
+            most = fmaxf(most, fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w))));
+            *reinterpret_cast<float4*>(sums + row * cap + i) = s;
+        }
+#pragma unroll
+        for (int o = TPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        // fp16: relative to a power of two from the row's largest on
+        float up = 1.f, down = 1.f;
+        if (std::is_same<W, __half>::value && most > 0.f && most < INFINITY) {
+            const int e = min(max((int)(__float_as_uint(most) >> 23) - 126, -120), 126);
+            up = __uint_as_float((uint32_t)(127 + e) << 23);
+            down = __uint_as_float((uint32_t)(127 - e) << 23);
+        }
+        if (c == 0) sh.scale[row] = up * scale;
+        for (int i = 4 * c; i < r16; i += 4 * TPR) {
+            const float4 s = *reinterpret_cast<const float4*>(sums + row * cap + i);
+            float f[4] = {s.x * down, s.y * down, s.z * down, s.w * down};
+#pragma unroll
+            for (int p = 0; p < pieces; ++p) {
+                W h[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h[e] = ad_round<W>(f[e]);
+                    const float b = ad_f32(h[e]);
+                    f[e] = fabsf(b) == INFINITY ? 0.f : f[e] - b;
                 }
+                *reinterpret_cast<uint2*>(t16 + (p * T + row) * pld + i * 2) = *reinterpret_cast<const uint2*>(h);
             }
         }
-        __syncthreads();
-        if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (nothing of the others is read from here on)
+        if (S > 1) {
+            __syncwarp();
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (nothing of the others is read from here on)
+        }
     }
+    __syncthreads();
 
-    // ---- out = base + B t: this CTA's part of M, 32 outputs at a time; an output's place in a product's columns is chosen so that a lane has four neighbours
-    const int units = (P.M + 31) / 32, u0 = (int)((long long)units * rank / S), u1 = (int)((long long)units * (rank + 1) / S), ksteps = (r_all + 15) / 16;
+    // ---- out = base + B t: this CTA's part of M, FB outputs and 64 ranks at a time through shared memory
+    const int units = (P.M + 31) / 32, m_from = 32 * (int)((long long)units * rank / S), m_to = min(P.M, 32 * (int)((long long)units * (rank + 1) / S));
+    const int chunks = max(1, (r16 + kAdChunk - 1) / kAdChunk), rc = min(r16, kAdChunk), wld = Z::wld(rc), s2 = Z::stage2(rc);
+    const int count = (max(m_to - m_from, 0) + FB - 1) / FB * chunks;
     const float s0 = r_all ? sh.scale[16 * mt + g] : 0.f, s1 = r_all ? sh.scale[16 * mt + g + 8] : 0.f;
     const bool have0 = 16 * mt + g < n_rows, have1 = 16 * mt + g + 8 < n_rows;
+    X* const o0 = op + (int64_t)sh.rows[min(16 * mt + g, n_rows - 1)] * P.ldout;
+    X* const o1 = op + (int64_t)sh.rows[min(16 * mt + g + 8, n_rows - 1)] * P.ldout;
     const W* wb = reinterpret_cast<const W*>(P.b) + (has ? a * P.b_slot : 0);
-#pragma unroll 1
-    for (int u = u0 + ks; u < u1; u += KS) {
-        const int m = 32 * u;
-        float acc[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        float4 b[2][2];  // [row][half]
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int f = m + 16 * h + 4 * q, left = P.M - f;
-            b[0][h] = bp && have0 && left > 0 ? ad_floats(ad_load4(bp + row0 * P.ldbase + f, left, P.wide_out), (const X*)nullptr) : make_float4(0.f, 0.f, 0.f, 0.f);
-            b[1][h] = bp && have1 && left > 0 ? ad_floats(ad_load4(bp + row1 * P.ldbase + f, left, P.wide_out), (const X*)nullptr) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll 2
-        for (int k = 0; k < ksteps; ++k) {
-            const int r = 16 * k + 4 * q, left = r_all - r;
-            uint2 w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int f = m + 16 * (j >> 1) + 4 * (g >> 1) + 2 * (j & 1) + (g & 1);
-                w[j] = f < P.M ? ad_load4(wb + (int64_t)f * P.b_row + r, left, P.wide_b) : make_uint2(0u, 0u);
+    const auto fill = [&](int i) {
+        unsigned char* ws = stage + i % Z::stages * s2;
+        unsigned char* bs = ws + FB * wld;
+        const int m0 = m_from + i / chunks * FB, ch = i % chunks, r0 = ch * kAdChunk, wu = min(kAdChunk, r16 - r0) / 8;
+        if (wu > 0)
+            for (int v = tid; v < FB * wu; v += kAdThreads) {
+                const int f = v / wu, r = r0 + v % wu * 8;
+                // (output 4 x + 2 y + z of sixteen is row 8 y + 2 x + z: column 2 x + z of product y)
+                const int at = (f & ~15) + (f >> 1 & 1) * 8 + (f >> 2 & 3) * 2 + (f & 1);
+                ad_fill16(ws + at * wld + v % wu * 16, wb + (int64_t)min(m0 + f, P.M - 1) * P.b_row + r, m0 + f < m_to ? r_all - r : 0, P.wide_b, wb);
             }
+        if (bp && ch == chunks - 1) {
+            constexpr int XN = 16 / (int)sizeof(X), BU = FB / XN;
 #pragma unroll
-            for (int p = pieces - 1; p >= 0; --p) {
-                const W* t0 = t16 + (size_t)(p * T + 16 * mt + g) * ld16 + r;
-                const uint2 a0 = *reinterpret_cast<const uint2*>(t0), a1 = *reinterpret_cast<const uint2*>(t0 + 8 * ld16);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) ad_mma16(acc[j], a0.x, a1.x, a0.y, a1.y, w[j].x, w[j].y, (const W*)nullptr);
+            for (int v = tid; v < T * BU; v += kAdThreads) {
+                const int row = v / BU, f = m0 + v % BU * XN;
+                ad_fill16(bs + row * Z::bld + v % BU * 16, bp + (int64_t)sh.rows[min(row, n_rows - 1)] * P.ldbase + f, row < n_rows ? m_to - f : 0, P.wide_base, bp);
             }
         }
+    };
+    float acc[J][4];
+    ad_pipeline<Z::stages>(count, fill, [&](int i) {
+        const unsigned char* ws = stage + i % Z::stages * s2 + (FW * ks + g) * wld + 8 * q;
+        const unsigned char* bs = stage + i % Z::stages * s2 + FB * wld;
+        const int ch = i % chunks, steps = min(kAdChunk, r16 - ch * kAdChunk) / 16;
+        if (ch == 0)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int f = m + 16 * h + 4 * q, left = P.M - f;
-            float4 v0 = b[0][h], v1 = b[1][h];
-            if (r_all) {
-                v0 = make_float4(fmaf(s0, acc[2 * h][0], v0.x), fmaf(s0, acc[2 * h][1], v0.y), fmaf(s0, acc[2 * h + 1][0], v0.z), fmaf(s0, acc[2 * h + 1][1], v0.w));
-                v1 = make_float4(fmaf(s1, acc[2 * h][2], v1.x), fmaf(s1, acc[2 * h][3], v1.y), fmaf(s1, acc[2 * h + 1][2], v1.z), fmaf(s1, acc[2 * h + 1][3], v1.w));
+            for (int j = 0; j < J; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+        const unsigned char* tp = t16 + (16 * mt + g) * pld + ch * kAdChunk * 2 + 8 * q;
+#pragma unroll
+        for (int k = 0; k < kAdChunk / 16; ++k)
+            if (k < steps) {
+                uint2 w[J];
+#pragma unroll
+                for (int j = 0; j < J; ++j) w[j] = *reinterpret_cast<const uint2*>(ws + 8 * j * wld + 32 * k);
+#pragma unroll
+                for (int p = pieces - 1; p >= 0; --p) {
+                    const uint2 a0 = *reinterpret_cast<const uint2*>(tp + p * T * pld + 32 * k), a1 = *reinterpret_cast<const uint2*>(tp + (p * T + 8) * pld + 32 * k);
+#pragma unroll
+                    for (int j = 0; j < J; ++j) ad_mma16(acc[j], a0.x, a1.x, a0.y, a1.y, w[j].x, w[j].y, (const W*)nullptr);
+                }
             }
-            if (have0 && left > 0) ad_store4(op + row0 * P.ldout + f, v0, left, P.wide_out);
-            if (have1 && left > 0) ad_store4(op + row1 * P.ldout + f, v1, left, P.wide_out);
+        if (ch == chunks - 1) {
+            const int m0 = m_from + i / chunks * FB;
+#pragma unroll
+            for (int h = 0; h < FW / 16; ++h) {
+                // a lane has four neighbouring outputs of two rows
+                const int f = FW * ks + 16 * h + 4 * q, left = m_to - m0 - f;
+                float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
+                if (bp) {
+                    const unsigned char* b0 = bs + (16 * mt + g) * Z::bld + f * (int)sizeof(X);
+                    if constexpr (Z::wide) {
+                        v0 = *reinterpret_cast<const float4*>(b0), v1 = *reinterpret_cast<const float4*>(b0 + 8 * Z::bld);
+                    } else {
+                        v0 = ad_floats(*reinterpret_cast<const uint2*>(b0), (const X*)nullptr), v1 = ad_floats(*reinterpret_cast<const uint2*>(b0 + 8 * Z::bld), (const X*)nullptr);
+                    }
+                }
+                if (r_all) {
+                    v0 = make_float4(fmaf(s0, acc[2 * h][0], v0.x), fmaf(s0, acc[2 * h][1], v0.y), fmaf(s0, acc[2 * h + 1][0], v0.z), fmaf(s0, acc[2 * h + 1][1], v0.w));
+                    v1 = make_float4(fmaf(s1, acc[2 * h][2], v1.x), fmaf(s1, acc[2 * h][3], v1.y), fmaf(s1, acc[2 * h + 1][2], v1.z), fmaf(s1, acc[2 * h + 1][3], v1.w));
+                }
+                if (have0 && left > 0) ad_store4(o0 + m0 + f, v0, left, P.wide_out);
+                if (have1 && left > 0) ad_store4(o1 + m0 + f, v1, left, P.wide_out);
+            }
         }
-    }
+    });
     if (r_all > 0 && S > 1) {
         __syncwarp();
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // no CTA leaves while its part may be read
