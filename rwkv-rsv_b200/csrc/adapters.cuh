@@ -232,7 +232,11 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < per_thread; ++i)
-        if (group[i] >= 0) atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (group[i] >> 1), group[i] & 1 ? 65536u : 1u);  // (no counter passes 4096)
+        if (i < each) {  // (a few adapters have most rows: one addition per warp and adapter)
+            const uint32_t same = __match_any_sync(0xffffffffu, group[i]);
+            if (group[i] >= 0 && __ffs(same) - 1 == lane)
+                atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (group[i] >> 1), (uint32_t)__popc(same) << (group[i] & 1 ? 16 : 0));  // (no counter passes 4096)
+        }
     __syncthreads();
     const int per = (groups + kAdThreads - 1) / kAdThreads, g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     const auto tiles_of = [&](int g) { return g == P.slots && !P.copies ? 0 : ((int)cnt[g] + T - 1) / T; };
@@ -281,10 +285,9 @@ __device__ __forceinline__ void ad_fill16(void* dst, const E* src, int n, bool w
         ad_copy16(dst, n ? src : any, n * (int)sizeof(E));
         return;
     }
-    alignas(16) E v[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = e < n ? src[e] : E(0.f);
-    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+    E* to = reinterpret_cast<E*>(dst);
+#pragma unroll 1
+    for (int e = 0; e < N; ++e) to[e] = e < n ? src[e] : E(0.f);
 }
 __device__ __forceinline__ void ad_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -345,20 +348,29 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
 #pragma unroll
             for (int j = 0; j < kAdChunk / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
             __syncthreads();  // (the counters, or the sums before these, have been read)
-            const auto fill = [&](int i) {
-                unsigned char* xs = stage + i % Z::stages * Z::stage1;
-                unsigned char* ws = xs + T * Z::xld;
-                const int k0 = k_from + i * KC;
-                constexpr int XN = 16 / (int)sizeof(X), XU = KC / XN, WU = KC / 8;  // values of 16 bytes, and those of a row
+            constexpr int XN = 16 / (int)sizeof(X), XU = KC / XN, XP = T * XU / kAdThreads;  // values of 16 bytes, those of a row, and those of a thread
+            constexpr int WU = KC / 8, WP = kAdChunk * WU / kAdThreads;
+            const int xu = tid % XU * XN, xrow = tid / XU, wu = tid % WU * 8, wrow = tid / WU;
+            const X* src[XP];
+            int have[XP];  // (rows past the last one are zeros)
 #pragma unroll
-                for (int v = tid; v < T * XU; v += kAdThreads) {
-                    const int row = v / XU, k = k0 + v % XU * XN;
-                    ad_fill16(xs + row * Z::xld + v % XU * 16, xp + (int64_t)sh.rows[min(row, n_rows - 1)] * P.ldx + k, row < n_rows ? k_to - k : 0, P.wide_x, xp);
-                }
-                for (int v = tid; v < 8 * nt * WU; v += kAdThreads) {
-                    const int row = v / WU, k = k0 + v % WU * 8;
-                    ad_fill16(ws + row * Z::ald + v % WU * 16, wa + (int64_t)min(c0 + row, r_all - 1) * P.a_row + k, row < ranks ? k_to - k : 0, P.wide_a, wa);
-                }
+            for (int p = 0; p < XP; ++p) {
+                const int row = xrow + p * (kAdThreads / XU);
+                src[p] = xp + (int64_t)sh.rows[min(row, n_rows - 1)] * P.ldx + xu + k_from;
+                have[p] = row < n_rows ? KC : 0;
+            }
+            const W* wsrc = wa + (int64_t)(c0 + wrow) * P.a_row + wu + k_from;
+            const int64_t wstep = (int64_t)(kAdThreads / WU) * P.a_row;
+            const auto fill = [&](int i) {
+                unsigned char* xs = stage + i % Z::stages * Z::stage1 + xrow * Z::xld + tid % XU * 16;
+                unsigned char* ws = stage + i % Z::stages * Z::stage1 + T * Z::xld + wrow * Z::ald + tid % WU * 16;
+                const int k = i * KC, left = k_to - k_from - k;
+#pragma unroll
+                for (int p = 0; p < XP; ++p) ad_fill16(xs + p * (kAdThreads / XU) * Z::xld, src[p] + k, min(have[p], left - xu), P.wide_x, xp);
+#pragma unroll
+                for (int p = 0; p < WP; ++p)
+                    if (wrow + p * (kAdThreads / WU) < 8 * nt)
+                        ad_fill16(ws + p * (kAdThreads / WU) * Z::ald, wsrc + p * wstep + k, wrow + p * (kAdThreads / WU) < ranks ? left - wu : 0, P.wide_a, wa);
             };
             ad_pipeline<Z::stages>(count, fill, [&](int i) {
                 const unsigned char* xs = stage + i % Z::stages * Z::stage1 + (16 * mt + g) * Z::xld;
@@ -488,31 +500,45 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
     X* const o0 = op + (int64_t)sh.rows[min(16 * mt + g, n_rows - 1)] * P.ldout;
     X* const o1 = op + (int64_t)sh.rows[min(16 * mt + g + 8, n_rows - 1)] * P.ldout;
     const W* wb = reinterpret_cast<const W*>(P.b) + (has ? a * P.b_slot : 0);
+    // units of 16 bytes of a row of B, as a power of two
+    const int lw = rc <= 8 ? 0 : rc <= 16 ? 1 : rc <= 32 ? 2 : 3, wu = tid & ((1 << lw) - 1), wrow = tid >> lw, wstep = kAdThreads >> lw;
+    // output 4 x + 2 y + z of sixteen is row 8 y + 2 x + z: column 2 x + z of product y
+    const int wat = (wrow & ~15) + (wrow >> 1 & 1) * 8 + (wrow >> 2 & 3) * 2 + (wrow & 1);
+    constexpr int XN = 16 / (int)sizeof(X), BU = FB / XN, BP = T * BU / kAdThreads;
+    const int bu = tid % BU * XN, brow = tid / BU;
+    const W* wsrc = wb + (int64_t)(m_from + wrow) * P.b_row + 8 * wu;
+    const X* bsrc[BP];
+    bool bhave[BP];
+#pragma unroll
+    for (int p = 0; p < BP; ++p) {
+        const int row = brow + p * (kAdThreads / BU);
+        bsrc[p] = bp + (bp ? (int64_t)sh.rows[min(row, n_rows - 1)] * P.ldbase + m_from + bu : 0);
+        bhave[p] = bp && row < n_rows;
+    }
     const auto fill = [&](int i) {
         unsigned char* ws = stage + i % Z::stages * s2;
-        unsigned char* bs = ws + FB * wld;
-        const int m0 = m_from + i / chunks * FB, ch = i % chunks, r0 = ch * kAdChunk, wu = min(kAdChunk, r16 - r0) / 8;
-        if (wu > 0)
-            for (int v = tid; v < FB * wu; v += kAdThreads) {
-                const int f = v / wu, r = r0 + v % wu * 8;
-                // (output 4 x + 2 y + z of sixteen is row 8 y + 2 x + z: column 2 x + z of product y)
-                const int at = (f & ~15) + (f >> 1 & 1) * 8 + (f >> 2 & 3) * 2 + (f & 1);
-                ad_fill16(ws + at * wld + v % wu * 16, wb + (int64_t)min(m0 + f, P.M - 1) * P.b_row + r, m0 + f < m_to ? r_all - r : 0, P.wide_b, wb);
-            }
-        if (bp && ch == chunks - 1) {
-            constexpr int XN = 16 / (int)sizeof(X), BU = FB / XN;
-#pragma unroll
-            for (int v = tid; v < T * BU; v += kAdThreads) {
-                const int row = v / BU, f = m0 + v % BU * XN;
-                ad_fill16(bs + row * Z::bld + v % BU * 16, bp + (int64_t)sh.rows[min(row, n_rows - 1)] * P.ldbase + f, row < n_rows ? m_to - f : 0, P.wide_base, bp);
+        unsigned char* bs = ws + FB * wld + brow * Z::bld + tid % BU * 16;
+        const int fb = chunks == 1 ? i : i / chunks, ch = chunks == 1 ? 0 : i % chunks, m = fb * FB, left = m_to - m_from - m, r = ch * kAdChunk + 8 * wu;
+        if (r < r16) {
+            const W* from = wsrc + (int64_t)m * P.b_row + ch * kAdChunk;
+            unsigned char* to = ws + wat * wld + wu * 16;
+#pragma unroll 1
+            for (int f = wrow; f < FB; f += wstep) {
+                ad_fill16(to, from, f < left ? r_all - r : 0, P.wide_b, wb);
+                from += (int64_t)wstep * P.b_row;
+                to += wstep * wld;
             }
         }
+        if (ch == chunks - 1)
+#pragma unroll
+            for (int p = 0; p < BP; ++p)
+                if (bhave[p]) ad_fill16(bs + p * (kAdThreads / BU) * Z::bld, bsrc[p] + m, left - bu, P.wide_base, bp);
     };
     float acc[J][4];
     ad_pipeline<Z::stages>(count, fill, [&](int i) {
         const unsigned char* ws = stage + i % Z::stages * s2 + (FW * ks + g) * wld + 8 * q;
         const unsigned char* bs = stage + i % Z::stages * s2 + FB * wld;
-        const int ch = i % chunks, steps = min(kAdChunk, r16 - ch * kAdChunk) / 16;
+        const int fb = chunks == 1 ? i : i / chunks, ch = chunks == 1 ? 0 : i % chunks, steps = min(kAdChunk, r16 - ch * kAdChunk) / 16;
         if (ch == 0)
 #pragma unroll
             for (int j = 0; j < J; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
@@ -531,7 +557,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                 }
             }
         if (ch == chunks - 1) {
-            const int m0 = m_from + i / chunks * FB;
+            const int m0 = m_from + fb * FB;
 #pragma unroll
             for (int h = 0; h < FW / 16; ++h) {
                 // a lane has four neighbouring outputs of two rows
