@@ -104,6 +104,10 @@ __device__ __forceinline__ void ad_store4(H* p, const float4& v, int n, bool wid
         if (i < n) p[i] = h[i];
 }
 
+// Four 8 x 8 matrices of 16-bit values, a row's address from every lane: an operand of 16 x 16, or two of 8 x 16.
+__device__ __forceinline__ void ad_ldm(uint32_t (&v)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+}
 __device__ __forceinline__ uint32_t ad_tf32(float v) {
     uint32_t t;
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(t) : "f"(v));
@@ -141,11 +145,12 @@ struct AdShape {
     static constexpr int FW = MT == 4 ? 32 : 16;        // outputs of a warp in a stage
     static constexpr int FB = FW * KS;                  // ... and of a stage
     static constexpr int stages = wide && MT == 4 ? 2 : 3;  // (two CTAs fit on an SM)
-    // Bytes from row to row.  A lane reads four values of the row that is its number over four: the rows of a quarter (16-byte reads) or half (8-byte reads)
-    // of a warp lie in different banks when they are 16 or 8 words apart, modulo 32.
-    static constexpr int xld = (KC + 16) * (int)sizeof(X), ald = (KC + 16) * 2, bld = (FB + 16) * (int)sizeof(X);
+    // Bytes from row to row.  16-bit operands are read as matrices of eight rows of 16 bytes: rows an odd multiple of 16 bytes apart lie in different banks.
+    // Of the others a lane reads four values of the row that is its number over four: the rows of a quarter (16-byte reads) or half (8-byte reads) of a warp
+    // lie in different banks when they are 16 or 8 words apart, modulo 32.
+    static constexpr int xld = wide ? (KC + 16) * 4 : (KC + 8) * 2, ald = wide ? (KC + 16) * 2 : (KC + 8) * 2, bld = (FB + 16) * (int)sizeof(X);
     static constexpr int stage1 = T * xld + kAdChunk * ald;
-    __host__ __device__ static constexpr int wld(int ranks16) { return (ranks16 % 32 ? ranks16 : ranks16 + 16) * 2; }
+    __host__ __device__ static constexpr int wld(int ranks16) { return (ranks16 + 8) * 2; }
     __host__ __device__ static constexpr int stage2(int ranks16) { return FB * wld(ranks16) + T * bld; }
     __host__ __device__ static constexpr size_t part_bytes(int cap) { return (size_t)T * cap * 4; }
     __host__ __device__ static constexpr size_t piece_bytes(int cap) { return (size_t)pieces * T * wld(cap); }
@@ -294,21 +299,24 @@ template <int N>
 __device__ __forceinline__ void ad_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// `count` stages: fill(i) begins to load stage i, use(i) works on it.
+// `count` stages: fill(i, slot) begins to load stage i, use(i, slot) works on it.
 template <int STAGES, class Fill, class Use>
 __device__ __forceinline__ void ad_pipeline(int count, Fill&& fill, Use&& use) {
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) {
-        if (i < count) fill(i);
+        if (i < count) fill(i, i);
         ad_commit();
     }
+    int slot = 0, next = STAGES - 1;
 #pragma unroll 1
     for (int i = 0; i < count; ++i) {
         ad_wait<STAGES - 2>();
         __syncthreads();  // stage i is there for all, and the one before it has been used
-        if (i + STAGES - 1 < count) fill(i + STAGES - 1);
+        if (i + STAGES - 1 < count) fill(i + STAGES - 1, next);
         ad_commit();
-        use(i);
+        use(i, slot);
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
+        next = next + 1 == STAGES ? 0 : next + 1;
     }
     ad_wait<0>();
     __syncthreads();
@@ -361,9 +369,9 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             }
             const W* wsrc = wa + (int64_t)(c0 + wrow) * P.a_row + wu + k_from;
             const int64_t wstep = (int64_t)(kAdThreads / WU) * P.a_row;
-            const auto fill = [&](int i) {
-                unsigned char* xs = stage + i % Z::stages * Z::stage1 + xrow * Z::xld + tid % XU * 16;
-                unsigned char* ws = stage + i % Z::stages * Z::stage1 + T * Z::xld + wrow * Z::ald + tid % WU * 16;
+            const auto fill = [&](int i, int slot) {
+                unsigned char* xs = stage + slot * Z::stage1 + xrow * Z::xld + tid % XU * 16;
+                unsigned char* ws = stage + slot * Z::stage1 + T * Z::xld + wrow * Z::ald + tid % WU * 16;
                 const int k = i * KC, left = k_to - k_from - k;
 #pragma unroll
                 for (int p = 0; p < XP; ++p) ad_fill16(xs + p * (kAdThreads / XU) * Z::xld, src[p] + k, min(have[p], left - xu), P.wide_x, xp);
@@ -372,10 +380,13 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                     if (wrow + p * (kAdThreads / WU) < 8 * nt)
                         ad_fill16(ws + p * (kAdThreads / WU) * Z::ald, wsrc + p * wstep + k, wrow + p * (kAdThreads / WU) < ranks ? left - wu : 0, P.wide_a, wa);
             };
-            ad_pipeline<Z::stages>(count, fill, [&](int i) {
-                const unsigned char* xs = stage + i % Z::stages * Z::stage1 + (16 * mt + g) * Z::xld;
-                const unsigned char* ws = stage + i % Z::stages * Z::stage1 + T * Z::xld + g * Z::ald;
-                // A lane has four consecutive k of every row; the products do not mind in which order the tensor core takes them, as long as both operands agree.
+            ad_pipeline<Z::stages>(count, fill, [&](int, int slot) {
+                const unsigned char* xs = stage + slot * Z::stage1 + (16 * mt + g) * Z::xld;
+                const unsigned char* ws = stage + slot * Z::stage1 + T * Z::xld + g * Z::ald;
+                // (16-bit operands: this lane's row, and which of its two halves)
+                const uint32_t xm = smem_u32(stage + slot * Z::stage1 + (16 * mt + (lane & 15)) * Z::xld + (lane >> 4) * 16);
+                const uint32_t wm = smem_u32(stage + slot * Z::stage1 + T * Z::xld + ((lane & 7) + (lane >> 4) * 8) * Z::ald + (lane >> 3 & 1) * 16);
+                // fp32: a lane has four consecutive k of every row; the products do not mind in which order the tensor core takes them, as long as both operands agree.
 #pragma unroll
                 for (int s = 0; s < KC / 16 / KS; ++s) {
                     const int k = 16 * (ks + KS * s) + 4 * q;
@@ -396,12 +407,15 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                                 ad_mma_tf32(acc[j], hi[0][2], hi[1][2], hi[0][3], hi[1][3], b2, b3);
                             }
                     } else {
-                        const uint2 y0 = *reinterpret_cast<const uint2*>(xs + k * 2), y1 = *reinterpret_cast<const uint2*>(xs + 8 * Z::xld + k * 2);
+                        uint32_t y[4];
+                        ad_ldm(y, xm + 32 * (ks + KS * s));
 #pragma unroll
-                        for (int j = 0; j < kAdChunk / 8; ++j)
-                            if (j < nt) {
-                                const uint2 b = *reinterpret_cast<const uint2*>(ws + 8 * j * Z::ald + k * 2);
-                                ad_mma16(acc[j], y0.x, y1.x, y0.y, y1.y, b.x, b.y, (const W*)nullptr);
+                        for (int j = 0; j < kAdChunk / 8; j += 2)
+                            if (j < nt) {  // (a second one past the last rank: zeros or numbers that nothing uses)
+                                uint32_t b[4];
+                                ad_ldm(b, wm + 8 * j * Z::ald + 32 * (ks + KS * s));
+                                ad_mma16(acc[j], y[0], y[1], y[2], y[3], b[0], b[1], (const W*)nullptr);
+                                ad_mma16(acc[j + 1], y[0], y[1], y[2], y[3], b[2], b[3], (const W*)nullptr);
                             }
                     }
                 }
@@ -515,8 +529,8 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
         bsrc[p] = bp + (bp ? (int64_t)sh.rows[min(row, n_rows - 1)] * P.ldbase + m_from + bu : 0);
         bhave[p] = bp && row < n_rows;
     }
-    const auto fill = [&](int i) {
-        unsigned char* ws = stage + i % Z::stages * s2;
+    const auto fill = [&](int i, int slot) {
+        unsigned char* ws = stage + slot * s2;
         unsigned char* bs = ws + FB * wld + brow * Z::bld + tid % BU * 16;
         const int fb = chunks == 1 ? i : i / chunks, ch = chunks == 1 ? 0 : i % chunks, m = fb * FB, left = m_to - m_from - m, r = ch * kAdChunk + 8 * wu;
         if (r < r16) {
@@ -535,25 +549,28 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                 if (bhave[p]) ad_fill16(bs + p * (kAdThreads / BU) * Z::bld, bsrc[p] + m, left - bu, P.wide_base, bp);
     };
     float acc[J][4];
-    ad_pipeline<Z::stages>(count, fill, [&](int i) {
-        const unsigned char* ws = stage + i % Z::stages * s2 + (FW * ks + g) * wld + 8 * q;
-        const unsigned char* bs = stage + i % Z::stages * s2 + FB * wld;
+    const uint32_t wm = smem_u32(stage) + (FW * ks + (lane & 7) + (lane >> 4) * 8) * wld + (lane >> 3 & 1) * 16;
+    const uint32_t tm = smem_u32(t16) + (16 * mt + (lane & 15)) * pld + (lane >> 4) * 16;
+    ad_pipeline<Z::stages>(count, fill, [&](int i, int slot) {
+        const uint32_t ws = wm + slot * s2;
+        const unsigned char* bs = stage + slot * s2 + FB * wld;
         const int fb = chunks == 1 ? i : i / chunks, ch = chunks == 1 ? 0 : i % chunks, steps = min(kAdChunk, r16 - ch * kAdChunk) / 16;
         if (ch == 0)
 #pragma unroll
             for (int j = 0; j < J; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        const unsigned char* tp = t16 + (16 * mt + g) * pld + ch * kAdChunk * 2 + 8 * q;
+        const uint32_t tp = tm + ch * kAdChunk * 2;
 #pragma unroll
         for (int k = 0; k < kAdChunk / 16; ++k)
             if (k < steps) {
-                uint2 w[J];
+                uint32_t w[J / 2][4];
 #pragma unroll
-                for (int j = 0; j < J; ++j) w[j] = *reinterpret_cast<const uint2*>(ws + 8 * j * wld + 32 * k);
+                for (int j = 0; j < J / 2; ++j) ad_ldm(w[j], ws + 16 * j * wld + 32 * k);
 #pragma unroll
                 for (int p = pieces - 1; p >= 0; --p) {
-                    const uint2 a0 = *reinterpret_cast<const uint2*>(tp + p * T * pld + 32 * k), a1 = *reinterpret_cast<const uint2*>(tp + (p * T + 8) * pld + 32 * k);
+                    uint32_t t[4];
+                    ad_ldm(t, tp + p * T * pld + 32 * k);
 #pragma unroll
-                    for (int j = 0; j < J; ++j) ad_mma16(acc[j], a0.x, a1.x, a0.y, a1.y, w[j].x, w[j].y, (const W*)nullptr);
+                    for (int j = 0; j < J; ++j) ad_mma16(acc[j], t[0], t[1], t[2], t[3], w[j / 2][j % 2 * 2], w[j / 2][j % 2 * 2 + 1], (const W*)nullptr);
                 }
             }
         if (ch == chunks - 1) {
