@@ -82,26 +82,33 @@ __device__ __forceinline__ float ad_hi(uint32_t v, const __nv_bfloat16*) { retur
 __device__ __forceinline__ float4 ad_floats(const float4& v, const float*) { return v; }
 template <typename H>
 __device__ __forceinline__ float4 ad_floats(const uint2& v, const H* h) { return make_float4(ad_lo(v.x, h), ad_hi(v.x, h), ad_lo(v.y, h), ad_hi(v.y, h)); }
-__device__ __forceinline__ void ad_store4(float* p, const float4& v, int n, bool wide) {
-    if (wide && n >= 4) {
-        *reinterpret_cast<float4*>(p) = v;
-        return;
-    }
-    if (n > 0) p[0] = v.x;
-    if (n > 1) p[1] = v.y;
-    if (n > 2) p[2] = v.z;
-    if (n > 3) p[3] = v.w;
+__device__ __forceinline__ uint32_t ad_pack(float a, float b, const __half*) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ uint32_t ad_pack(float a, float b, const __nv_bfloat16*) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Four values to p, of which the first n exist; `wide`: all at once, where all exist.
+__device__ __forceinline__ void ad_store4(float* p, const float4& v) { *reinterpret_cast<float4*>(p) = v; }
 template <typename H>
-__device__ __forceinline__ void ad_store4(H* p, const float4& v, int n, bool wide) {
-    const H h[4] = {ad_round<H>(v.x), ad_round<H>(v.y), ad_round<H>(v.z), ad_round<H>(v.w)};
-    if (wide && n >= 4) {
-        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < n) p[i] = h[i];
+__device__ __forceinline__ void ad_store4(H* p, const float4& v) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(ad_pack(v.x, v.y, p), ad_pack(v.z, v.w, p));
+}
+template <typename E>
+__device__ __noinline__ void ad_store_some(E* p, float4 v, int n) {
+    if (n > 0) p[0] = ad_round<E>(v.x);
+    if (n > 1) p[1] = ad_round<E>(v.y);
+    if (n > 2) p[2] = ad_round<E>(v.z);
+    if (n > 3) p[3] = ad_round<E>(v.w);
+}
+template <typename E>
+__device__ __forceinline__ void ad_store4(E* p, const float4& v, int n, bool wide) {
+    if (wide && n >= 4)
+        ad_store4(p, v);
+    else
+        ad_store_some(p, v, n);
 }
 
 // Four 8 x 8 matrices of 16-bit values, a row's address from every lane: an operand of 16 x 16, or two of 8 x 16.
@@ -225,23 +232,18 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
         return true;
     }
     constexpr int per_thread = kAdBlockRows / kAdThreads;
-    const int each = (rows + kAdThreads - 1) / kAdThreads, i0 = tid * each;
-    int group[per_thread];  // of consecutive rows
+    int group[per_thread];  // of rows tid, tid + 256, ...
 #pragma unroll
     for (int i = 0; i < per_thread; ++i) {
-        const int a = i < each && i0 + i < rows ? ix[i0 + i] : -2;
-        group[i] = i < each && i0 + i < rows ? (a >= 0 && a < P.slots ? a : P.slots) : -1;
+        const int row = i * kAdThreads + tid, a = row < rows ? ix[row] : -1;
+        group[i] = row < rows ? (a >= 0 && a < P.slots ? a : P.slots) : -1;
     }
     for (int i = tid; i < (groups + 1) / 2; i += kAdThreads) reinterpret_cast<uint32_t*>(cnt)[i] = 0;
     if (tid == 0) sh.slot = -1;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < per_thread; ++i)
-        if (i < each) {  // (a few adapters have most rows: one addition per warp and adapter)
-            const uint32_t same = __match_any_sync(0xffffffffu, group[i]);
-            if (group[i] >= 0 && __ffs(same) - 1 == lane)
-                atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (group[i] >> 1), (uint32_t)__popc(same) << (group[i] & 1 ? 16 : 0));  // (no counter passes 4096)
-        }
+        if (group[i] >= 0) atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (group[i] >> 1), group[i] & 1 ? 65536u : 1u);  // (no counter passes 4096)
     __syncthreads();
     const int per = (groups + kAdThreads - 1) / kAdThreads, g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     const auto tiles_of = [&](int g) { return g == P.slots && !P.copies ? 0 : ((int)cnt[g] + T - 1) / T; };
@@ -270,7 +272,7 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
 #pragma unroll
         for (int i = 0; i < per_thread; ++i)
             if (group[i] == mine) {
-                if (place >= 0 && place < T) sh.rows[place] = first + i0 + i;
+                if (place >= 0 && place < T) sh.rows[place] = first + i * kAdThreads + tid;
                 ++place;
             }
     __syncthreads();
@@ -281,9 +283,12 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
 __device__ __forceinline__ void ad_copy16(void* dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void ad_copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
 // `n` values (none for n <= 0) of a row from src on to 16 bytes of shared memory, zeros behind them; `wide`: src is at 16 bytes.
 template <typename E>
-__device__ __forceinline__ void ad_fill16(void* dst, const E* src, int n, bool wide, const E* any) {
+__device__ __noinline__ void ad_fill16(void* dst, const E* src, int n, bool wide, const E* any) {
     constexpr int N = 16 / (int)sizeof(E);
     n = max(0, min(n, N));
     if (wide) {
@@ -359,26 +364,30 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             constexpr int XN = 16 / (int)sizeof(X), XU = KC / XN, XP = T * XU / kAdThreads;  // values of 16 bytes, those of a row, and those of a thread
             constexpr int WU = KC / 8, WP = kAdChunk * WU / kAdThreads;
             const int xu = tid % XU * XN, xrow = tid / XU, wu = tid % WU * 8, wrow = tid / WU;
+            // Rows past the tile's last one, and ranks past the adapter's, repeat the last one; nothing uses what comes of them.
             const X* src[XP];
-            int have[XP];  // (rows past the last one are zeros)
+            const W* wsrc[WP];
 #pragma unroll
-            for (int p = 0; p < XP; ++p) {
-                const int row = xrow + p * (kAdThreads / XU);
-                src[p] = xp + (int64_t)sh.rows[min(row, n_rows - 1)] * P.ldx + xu + k_from;
-                have[p] = row < n_rows ? KC : 0;
-            }
-            const W* wsrc = wa + (int64_t)(c0 + wrow) * P.a_row + wu + k_from;
-            const int64_t wstep = (int64_t)(kAdThreads / WU) * P.a_row;
+            for (int p = 0; p < XP; ++p) src[p] = xp + (int64_t)sh.rows[min(xrow + p * (kAdThreads / XU), n_rows - 1)] * P.ldx + xu + k_from;
+#pragma unroll
+            for (int p = 0; p < WP; ++p) wsrc[p] = wa + (int64_t)min(c0 + wrow + p * (kAdThreads / WU), r_all - 1) * P.a_row + wu + k_from;
             const auto fill = [&](int i, int slot) {
                 unsigned char* xs = stage + slot * Z::stage1 + xrow * Z::xld + tid % XU * 16;
                 unsigned char* ws = stage + slot * Z::stage1 + T * Z::xld + wrow * Z::ald + tid % WU * 16;
                 const int k = i * KC, left = k_to - k_from - k;
+                if (left >= KC && P.wide_x && P.wide_a) {
 #pragma unroll
-                for (int p = 0; p < XP; ++p) ad_fill16(xs + p * (kAdThreads / XU) * Z::xld, src[p] + k, min(have[p], left - xu), P.wide_x, xp);
+                    for (int p = 0; p < XP; ++p) ad_copy16(xs + p * (kAdThreads / XU) * Z::xld, src[p] + k);
+#pragma unroll
+                    for (int p = 0; p < WP; ++p)
+                        if (wrow + p * (kAdThreads / WU) < 8 * nt) ad_copy16(ws + p * (kAdThreads / WU) * Z::ald, wsrc[p] + k);
+                    return;
+                }
+#pragma unroll
+                for (int p = 0; p < XP; ++p) ad_fill16(xs + p * (kAdThreads / XU) * Z::xld, src[p] + k, left - xu, P.wide_x, xp);
 #pragma unroll
                 for (int p = 0; p < WP; ++p)
-                    if (wrow + p * (kAdThreads / WU) < 8 * nt)
-                        ad_fill16(ws + p * (kAdThreads / WU) * Z::ald, wsrc + p * wstep + k, wrow + p * (kAdThreads / WU) < ranks ? left - wu : 0, P.wide_a, wa);
+                    if (wrow + p * (kAdThreads / WU) < 8 * nt) ad_fill16(ws + p * (kAdThreads / WU) * Z::ald, wsrc[p] + k, left - wu, P.wide_a, wa);
             };
             ad_pipeline<Z::stages>(count, fill, [&](int, int slot) {
                 const unsigned char* xs = stage + slot * Z::stage1 + (16 * mt + g) * Z::xld;
@@ -433,12 +442,16 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             for (int i = tid; i < T * cols / 4; i += kAdThreads) {
                 const int row = i / (cols / 4), c = i % (cols / 4) * 4;
                 float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (c < 8 * nt)
+                if (c < ranks) {
 #pragma unroll
                     for (int p = 0; p < KS; ++p) {
                         const float4 v = *reinterpret_cast<const float4*>(sums + (p * T + row) * kAdSumLd + c);
                         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
                     }
+                    if (c + 1 >= ranks) s.y = 0.f;
+                    if (c + 2 >= ranks) s.z = 0.f;
+                    if (c + 3 >= ranks) s.w = 0.f;
+                }
                 *reinterpret_cast<float4*>(part + row * cap + c0 + c) = s;
             }
         }
@@ -511,8 +524,8 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
     const int count = (max(m_to - m_from, 0) + FB - 1) / FB * chunks;
     const float s0 = r_all ? sh.scale[16 * mt + g] : 0.f, s1 = r_all ? sh.scale[16 * mt + g + 8] : 0.f;
     const bool have0 = 16 * mt + g < n_rows, have1 = 16 * mt + g + 8 < n_rows;
-    X* const o0 = op + (int64_t)sh.rows[min(16 * mt + g, n_rows - 1)] * P.ldout;
-    X* const o1 = op + (int64_t)sh.rows[min(16 * mt + g + 8, n_rows - 1)] * P.ldout;
+    X* o0 = op + (int64_t)sh.rows[min(16 * mt + g, n_rows - 1)] * P.ldout + m_from + FW * ks + 4 * q;  // of this stage
+    X* o1 = op + (int64_t)sh.rows[min(16 * mt + g + 8, n_rows - 1)] * P.ldout + m_from + FW * ks + 4 * q;
     const W* wb = reinterpret_cast<const W*>(P.b) + (has ? a * P.b_slot : 0);
     // units of 16 bytes of a row of B, as a power of two
     const int lw = rc <= 8 ? 0 : rc <= 16 ? 1 : rc <= 32 ? 2 : 3, wu = tid & ((1 << lw) - 1), wrow = tid >> lw, wstep = kAdThreads >> lw;
@@ -520,33 +533,43 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
     const int wat = (wrow & ~15) + (wrow >> 1 & 1) * 8 + (wrow >> 2 & 3) * 2 + (wrow & 1);
     constexpr int XN = 16 / (int)sizeof(X), BU = FB / XN, BP = T * BU / kAdThreads;
     const int bu = tid % BU * XN, brow = tid / BU;
-    const W* wsrc = wb + (int64_t)(m_from + wrow) * P.b_row + 8 * wu;
-    const X* bsrc[BP];
-    bool bhave[BP];
+    const W* wnext = wb + (int64_t)(m_from + wrow) * P.b_row + 8 * wu;  // of the next stage: they are begun in order
+    const int64_t wrows = (int64_t)wstep * P.b_row;
+    const X* bnext[BP];
 #pragma unroll
-    for (int p = 0; p < BP; ++p) {
-        const int row = brow + p * (kAdThreads / BU);
-        bsrc[p] = bp + (bp ? (int64_t)sh.rows[min(row, n_rows - 1)] * P.ldbase + m_from + bu : 0);
-        bhave[p] = bp && row < n_rows;
-    }
+    for (int p = 0; p < BP; ++p) bnext[p] = bp + (bp ? (int64_t)sh.rows[min(brow + p * (kAdThreads / BU), n_rows - 1)] * P.ldbase + m_from + bu : 0);
+    const bool wide_in = P.wide_b && (!bp || P.wide_base);
     const auto fill = [&](int i, int slot) {
         unsigned char* ws = stage + slot * s2;
         unsigned char* bs = ws + FB * wld + brow * Z::bld + tid % BU * 16;
-        const int fb = chunks == 1 ? i : i / chunks, ch = chunks == 1 ? 0 : i % chunks, m = fb * FB, left = m_to - m_from - m, r = ch * kAdChunk + 8 * wu;
+        const int fb = chunks == 1 ? i : i / chunks, ch = chunks == 1 ? 0 : i % chunks, left = m_to - m_from - fb * FB, r = ch * kAdChunk + 8 * wu;
+        const bool whole = wide_in && left >= FB;
         if (r < r16) {
-            const W* from = wsrc + (int64_t)m * P.b_row + ch * kAdChunk;
+            const W* from = wnext + ch * kAdChunk;
             unsigned char* to = ws + wat * wld + wu * 16;
-#pragma unroll 1
+            const int bytes = max(0, min(8, r_all - r)) * 2;
+#pragma unroll 2
             for (int f = wrow; f < FB; f += wstep) {
-                ad_fill16(to, from, f < left ? r_all - r : 0, P.wide_b, wb);
-                from += (int64_t)wstep * P.b_row;
+                if (whole)
+                    ad_copy16(to, bytes ? from : wb, bytes);
+                else
+                    ad_fill16(to, from, f < left ? r_all - r : 0, P.wide_b, wb);
+                from += wrows;
                 to += wstep * wld;
             }
         }
-        if (ch == chunks - 1)
+        if (ch == chunks - 1) {
+            wnext += FB * P.b_row;
+            if (bp)
 #pragma unroll
-            for (int p = 0; p < BP; ++p)
-                if (bhave[p]) ad_fill16(bs + p * (kAdThreads / BU) * Z::bld, bsrc[p] + m, left - bu, P.wide_base, bp);
+                for (int p = 0; p < BP; ++p) {
+                    if (whole)
+                        ad_copy16(bs + p * (kAdThreads / BU) * Z::bld, bnext[p]);
+                    else
+                        ad_fill16(bs + p * (kAdThreads / BU) * Z::bld, bnext[p], left - bu, P.wide_base, bp);
+                    bnext[p] += FB;
+                }
+        }
     };
     float acc[J][4];
     const uint32_t wm = smem_u32(stage) + (FW * ks + (lane & 7) + (lane >> 4) * 8) * wld + (lane >> 3 & 1) * 16;
@@ -574,27 +597,35 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                 }
             }
         if (ch == chunks - 1) {
-            const int m0 = m_from + fb * FB;
+            const int left = m_to - m_from - fb * FB - FW * ks - 4 * q;
+            const bool whole = P.wide_out && m_from + (fb + 1) * FB <= m_to;
+            const unsigned char* b0 = bs + (16 * mt + g) * Z::bld + (FW * ks + 4 * q) * (int)sizeof(X);
 #pragma unroll
             for (int h = 0; h < FW / 16; ++h) {
                 // a lane has four neighbouring outputs of two rows
-                const int f = FW * ks + 16 * h + 4 * q, left = m_to - m0 - f;
                 float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
                 if (bp) {
-                    const unsigned char* b0 = bs + (16 * mt + g) * Z::bld + f * (int)sizeof(X);
                     if constexpr (Z::wide) {
-                        v0 = *reinterpret_cast<const float4*>(b0), v1 = *reinterpret_cast<const float4*>(b0 + 8 * Z::bld);
+                        v0 = *reinterpret_cast<const float4*>(b0 + 64 * h), v1 = *reinterpret_cast<const float4*>(b0 + 8 * Z::bld + 64 * h);
                     } else {
-                        v0 = ad_floats(*reinterpret_cast<const uint2*>(b0), (const X*)nullptr), v1 = ad_floats(*reinterpret_cast<const uint2*>(b0 + 8 * Z::bld), (const X*)nullptr);
+                        v0 = ad_floats(*reinterpret_cast<const uint2*>(b0 + 32 * h), (const X*)nullptr);
+                        v1 = ad_floats(*reinterpret_cast<const uint2*>(b0 + 8 * Z::bld + 32 * h), (const X*)nullptr);
                     }
                 }
                 if (r_all) {
                     v0 = make_float4(fmaf(s0, acc[2 * h][0], v0.x), fmaf(s0, acc[2 * h][1], v0.y), fmaf(s0, acc[2 * h + 1][0], v0.z), fmaf(s0, acc[2 * h + 1][1], v0.w));
                     v1 = make_float4(fmaf(s1, acc[2 * h][2], v1.x), fmaf(s1, acc[2 * h][3], v1.y), fmaf(s1, acc[2 * h + 1][2], v1.z), fmaf(s1, acc[2 * h + 1][3], v1.w));
                 }
-                if (have0 && left > 0) ad_store4(o0 + m0 + f, v0, left, P.wide_out);
-                if (have1 && left > 0) ad_store4(o1 + m0 + f, v1, left, P.wide_out);
+                if (whole) {
+                    if (have0) ad_store4(o0 + 16 * h, v0);
+                    if (have1) ad_store4(o1 + 16 * h, v1);
+                } else {
+                    if (have0) ad_store4(o0 + 16 * h, v0, left - 16 * h, P.wide_out);
+                    if (have1) ad_store4(o1 + 16 * h, v1, left - 16 * h, P.wide_out);
+                }
             }
+            o0 += FB;
+            o1 += FB;
         }
     });
     if (r_all > 0 && S > 1) {
