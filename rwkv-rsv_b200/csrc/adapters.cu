@@ -9,20 +9,27 @@
 
 namespace rsv {
 
-template <typename X, typename W, int MT>
+// Tiles of a block of rows if they are shared evenly among the adapters: about one in two adapters has a tile that is not full.
+static int64_t expected_tiles(const AdapterArgs& P, int T) {
+    const int rows = std::min(P.rows, kAdBlockRows), adapters = std::min(P.slots, rows);
+    return std::max(adapters, rows / T + adapters / 2);
+}
+
+template <typename X, typename W, int MT, int STAGES>
 static void launch_tiles(cudaStream_t stream, int device, AdapterArgs P) {
-    typedef AdShape<X, W, MT> Z;
+    typedef AdShape<X, W, MT, STAGES> Z;
     constexpr int T = Z::T;
     static_assert(T * kAdMaxRank <= kAdMostCells || MT == 4, "only the largest tile depends on the rank");
     P.block_rows = std::min(P.rows, kAdBlockRows);
     const int blocks = (P.rows + P.block_rows - 1) / P.block_rows;
     P.tiles = std::min(P.block_rows, P.block_rows / T + std::min(P.slots + P.copies, P.block_rows));
+    // two CTAs fit on an SM; the tiles that will be there, not those that may be
     P.S = kAdMaxCtas;
-    while (P.S > 1 && (int64_t)blocks * P.tiles * P.S > 148 * 4) P.S /= 2;
+    while (P.S > 1 && blocks * expected_tiles(P, T) * P.S > 2 * 148) P.S /= 2;
     const size_t smem = Z::smem(P.rank_cap);
     static bool configured[64] = {false};
     if (device >= 64 || !configured[device]) {
-        RSV_CUDA(cudaFuncSetAttribute(adapters_kernel<X, W, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Z::smem(std::min(kAdMaxRank, kAdMostCells / T))));
+        RSV_CUDA(cudaFuncSetAttribute(adapters_kernel<X, W, MT, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Z::smem(std::min(MT == 1 && STAGES > 3 ? 32 : kAdMaxRank, kAdMostCells / T))));
         if (device < 64) configured[device] = true;
     }
     cudaLaunchConfig_t cfg = {};
@@ -36,18 +43,22 @@ static void launch_tiles(cudaStream_t stream, int device, AdapterArgs P) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    RSV_CUDA(cudaLaunchKernelEx(&cfg, adapters_kernel<X, W, MT>, P));
+    RSV_CUDA(cudaLaunchKernelEx(&cfg, adapters_kernel<X, W, MT, STAGES>, P));
 }
 
 template <typename X, typename W>
 static void launch_adapters(cudaStream_t stream, int device, AdapterArgs P) {
-    const int each = std::min(P.rows, kAdBlockRows) / std::min(P.slots, std::min(P.rows, kAdBlockRows));  // rows of an adapter, if they are shared evenly
-    if (each >= 48 && 64 * P.rank_cap <= kAdMostCells)
-        launch_tiles<X, W, 4>(stream, device, P);
-    else if (each >= 24)
-        launch_tiles<X, W, 2>(stream, device, P);
+    const int rows = std::min(P.rows, kAdBlockRows), each = rows / std::min(P.slots, rows);  // rows of an adapter, if they are shared evenly
+    // large tiles read the adapters less often, but only if enough of them are left for the GPU
+    const auto fits = [&](int T) { return each >= T * 3 / 4 && T * P.rank_cap <= kAdMostCells && expected_tiles(P, T) * kAdMaxCtas >= 240; };
+    if (fits(64))
+        launch_tiles<X, W, 4, sizeof(X) == 4 ? 2 : 3>(stream, device, P);
+    else if (fits(32))
+        launch_tiles<X, W, 2, 3>(stream, device, P);
+    else if (P.rank_cap <= 32)
+        launch_tiles<X, W, 1, 5>(stream, device, P);
     else
-        launch_tiles<X, W, 1>(stream, device, P);
+        launch_tiles<X, W, 1, 3>(stream, device, P);
 }
 
 void engine_adapters(cudaStream_t stream, int device, int xtype, int wtype, AdapterArgs P) {

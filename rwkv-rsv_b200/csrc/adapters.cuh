@@ -6,8 +6,8 @@
 // this stays short).  So an adapter is read once per tile, not once per row, and the host need not know the indices.
 //   t = A x   the CTAs of the cluster split K, the warps of a CTA split it again; the partial sums meet in shared memory and then in the cluster's.
 //   B t       the CTAs split M; every CTA has all of t.
-// Both products run on the tensor cores with fp32 sums.  16-bit activations are operands as they are; fp32 ones are two tf32 numbers each, rounded to
-// nearest (together 2^-24 off, as fp32 itself), and the 16-bit weights are exact in tf32.  t is two fp16 numbers per value, relative to the row's largest
+// Both products run on the tensor cores with fp32 sums.  16-bit activations are operands as they are; fp32 ones are two tf32 numbers each (ad_split),
+// and the 16-bit weights are exact in tf32.  t is two fp16 numbers per value, relative to the row's largest
 // (2^-25 of it off), or two bf16 ones (2^-17; three, 2^-25, where out is fp32), so that B is an operand as it is.
 #pragma once
 #include <cuda_bf16.h>
@@ -115,16 +115,12 @@ __device__ __forceinline__ void ad_store4(E* p, const float4& v, int n, bool wid
 __device__ __forceinline__ void ad_ldm(uint32_t (&v)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
 }
-__device__ __forceinline__ uint32_t ad_tf32(float v) {
-    uint32_t t;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(t) : "f"(v));
-    return t;
-}
-// v as two tf32 numbers (an infinity has no rest)
+// v as two tf32 numbers: the first rounded to nearest, the rest (of up to 12 bits) cut to 11, so together they are at most 2^-22 of v off and 2^-24 on average.
+// A NaN stays one in the rest, an infinity has no rest.  (The conversion instruction takes several times as long as this.)
 __device__ __forceinline__ void ad_split(float v, uint32_t& hi, uint32_t& lo) {
-    hi = ad_tf32(v);
+    hi = (__float_as_uint(v) + 0x1000u) & 0xFFFFE000u;
     const float h = __uint_as_float(hi);
-    lo = ad_tf32(fabsf(h) == INFINITY ? 0.f : v - h);
+    lo = fabsf(h) == INFINITY ? 0u : __float_as_uint(v - h) & 0xFFFFE000u;
 }
 __device__ __forceinline__ void ad_mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -143,7 +139,7 @@ __device__ __forceinline__ void ad_mma16(float (&c)[4], uint32_t a0, uint32_t a1
 }
 
 // How a tile of 16 MT rows is worked on: the warps are MT groups of rows times KS parts of K or M.
-template <typename X, typename W, int MT>
+template <typename X, typename W, int MT, int STAGES>
 struct AdShape {
     static constexpr bool wide = sizeof(X) == 4;                                                    // fp32 activations
     static constexpr int pieces = sizeof(X) == 4 && std::is_same<W, __nv_bfloat16>::value ? 3 : 2;  // 16-bit numbers for a value of t
@@ -151,18 +147,18 @@ struct AdShape {
     static constexpr int KC = MT == 1 ? 128 : 64;       // k of a stage
     static constexpr int FW = MT == 4 ? 32 : 16;        // outputs of a warp in a stage
     static constexpr int FB = FW * KS;                  // ... and of a stage
-    static constexpr int stages = wide && MT == 4 ? 2 : 3;  // (two CTAs fit on an SM)
+    static constexpr int stages = STAGES;
     // Bytes from row to row.  16-bit operands are read as matrices of eight rows of 16 bytes: rows an odd multiple of 16 bytes apart lie in different banks.
     // Of the others a lane reads four values of the row that is its number over four: the rows of a quarter (16-byte reads) or half (8-byte reads) of a warp
     // lie in different banks when they are 16 or 8 words apart, modulo 32.
     static constexpr int xld = wide ? (KC + 16) * 4 : (KC + 8) * 2, ald = wide ? (KC + 16) * 2 : (KC + 8) * 2, bld = (FB + 16) * (int)sizeof(X);
-    static constexpr int stage1 = T * xld + kAdChunk * ald;
+    __host__ __device__ static constexpr int stage1(int ranks16) { return T * xld + ranks16 * ald; }
     __host__ __device__ static constexpr int wld(int ranks16) { return (ranks16 + 8) * 2; }
     __host__ __device__ static constexpr int stage2(int ranks16) { return FB * wld(ranks16) + T * bld; }
     __host__ __device__ static constexpr size_t part_bytes(int cap) { return (size_t)T * cap * 4; }
     __host__ __device__ static constexpr size_t piece_bytes(int cap) { return (size_t)pieces * T * wld(cap); }
     __host__ __device__ static constexpr size_t smem(int cap) {
-        const int s2 = stage2(cap < kAdChunk ? cap : kAdChunk), st = stages * (stage1 > s2 ? stage1 : s2);
+        const int rc = cap < kAdChunk ? cap : kAdChunk, s1 = stage1(rc), s2 = stage2(rc), st = stages * (s1 > s2 ? s1 : s2);
         return 1024 + part_bytes(cap) + piece_bytes(cap) + (st > (int)kAdSumBytes ? st : kAdSumBytes);
     }
 };
@@ -235,6 +231,8 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
     int group[per_thread];  // of rows tid, tid + 256, ...
 #pragma unroll
     for (int i = 0; i < per_thread; ++i) {
+        group[i] = -1;
+        if (i * kAdThreads >= rows) continue;
         const int row = i * kAdThreads + tid, a = row < rows ? ix[row] : -1;
         group[i] = row < rows ? (a >= 0 && a < P.slots ? a : P.slots) : -1;
     }
@@ -243,7 +241,7 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < per_thread; ++i)
-        if (group[i] >= 0) atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (group[i] >> 1), group[i] & 1 ? 65536u : 1u);  // (no counter passes 4096)
+        if (i * kAdThreads < rows && group[i] >= 0) atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (group[i] >> 1), group[i] & 1 ? 65536u : 1u);  // (no counter passes 4096)
     __syncthreads();
     const int per = (groups + kAdThreads - 1) / kAdThreads, g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     const auto tiles_of = [&](int g) { return g == P.slots && !P.copies ? 0 : ((int)cnt[g] + T - 1) / T; };
@@ -266,12 +264,13 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
     const int mine = sh.slot;
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < per_thread; ++i) n += group[i] == mine;
+    for (int i = 0; i < per_thread; ++i)
+        if (i * kAdThreads < rows) n += group[i] == mine;
     int place = ad_before(n, sh.wsum, all) - sh.skip;
     if (n && place < T && place + n > 0)
 #pragma unroll
         for (int i = 0; i < per_thread; ++i)
-            if (group[i] == mine) {
+            if (i * kAdThreads < rows && group[i] == mine) {
                 if (place >= 0 && place < T) sh.rows[place] = first + i * kAdThreads + tid;
                 ++place;
             }
@@ -327,13 +326,13 @@ __device__ __forceinline__ void ad_pipeline(int count, Fill&& fill, Use&& use) {
     __syncthreads();
 }
 
-template <typename X, typename W, int MT>
+template <typename X, typename W, int MT, int STAGES>
 __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) {
-    typedef AdShape<X, W, MT> Z;
+    typedef AdShape<X, W, MT, STAGES> Z;
     constexpr int T = Z::T, KS = Z::KS, KC = Z::KC, FW = Z::FW, FB = Z::FB, J = FW / 8, pieces = Z::pieces;
     extern __shared__ __align__(16) unsigned char ad_smem[];
     AdTile& sh = *reinterpret_cast<AdTile*>(ad_smem);
-    const int cap = P.rank_cap, pld = Z::wld(cap);
+    const int cap = P.rank_cap, pld = Z::wld(cap), s1 = Z::stage1(min(cap, kAdChunk));
     float* part = reinterpret_cast<float*>(ad_smem + 1024);
     unsigned char* t16 = ad_smem + 1024 + Z::part_bytes(cap);
     unsigned char* stage = t16 + Z::piece_bytes(cap);
@@ -364,7 +363,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             constexpr int XN = 16 / (int)sizeof(X), XU = KC / XN, XP = T * XU / kAdThreads;  // values of 16 bytes, those of a row, and those of a thread
             constexpr int WU = KC / 8, WP = kAdChunk * WU / kAdThreads;
             const int xu = tid % XU * XN, xrow = tid / XU, wu = tid % WU * 8, wrow = tid / WU;
-            // Rows past the tile's last one, and ranks past the adapter's, repeat the last one; nothing uses what comes of them.
+            // (Rows past the tile's last one are not loaded and ranks past the adapter's repeat the last one: nothing uses what comes of them.)
             const X* src[XP];
             const W* wsrc[WP];
 #pragma unroll
@@ -372,12 +371,13 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
 #pragma unroll
             for (int p = 0; p < WP; ++p) wsrc[p] = wa + (int64_t)min(c0 + wrow + p * (kAdThreads / WU), r_all - 1) * P.a_row + wu + k_from;
             const auto fill = [&](int i, int slot) {
-                unsigned char* xs = stage + slot * Z::stage1 + xrow * Z::xld + tid % XU * 16;
-                unsigned char* ws = stage + slot * Z::stage1 + T * Z::xld + wrow * Z::ald + tid % WU * 16;
+                unsigned char* xs = stage + slot * s1 + xrow * Z::xld + tid % XU * 16;
+                unsigned char* ws = stage + slot * s1 + T * Z::xld + wrow * Z::ald + tid % WU * 16;
                 const int k = i * KC, left = k_to - k_from - k;
                 if (left >= KC && P.wide_x && P.wide_a) {
 #pragma unroll
-                    for (int p = 0; p < XP; ++p) ad_copy16(xs + p * (kAdThreads / XU) * Z::xld, src[p] + k);
+                    for (int p = 0; p < XP; ++p)
+                        if (xrow + p * (kAdThreads / XU) < n_rows) ad_copy16(xs + p * (kAdThreads / XU) * Z::xld, src[p] + k);
 #pragma unroll
                     for (int p = 0; p < WP; ++p)
                         if (wrow + p * (kAdThreads / WU) < 8 * nt) ad_copy16(ws + p * (kAdThreads / WU) * Z::ald, wsrc[p] + k);
@@ -390,11 +390,11 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                     if (wrow + p * (kAdThreads / WU) < 8 * nt) ad_fill16(ws + p * (kAdThreads / WU) * Z::ald, wsrc[p] + k, left - wu, P.wide_a, wa);
             };
             ad_pipeline<Z::stages>(count, fill, [&](int, int slot) {
-                const unsigned char* xs = stage + slot * Z::stage1 + (16 * mt + g) * Z::xld;
-                const unsigned char* ws = stage + slot * Z::stage1 + T * Z::xld + g * Z::ald;
+                const unsigned char* xs = stage + slot * s1 + (16 * mt + g) * Z::xld;
+                const unsigned char* ws = stage + slot * s1 + T * Z::xld + g * Z::ald;
                 // (16-bit operands: this lane's row, and which of its two halves)
-                const uint32_t xm = smem_u32(stage + slot * Z::stage1 + (16 * mt + (lane & 15)) * Z::xld + (lane >> 4) * 16);
-                const uint32_t wm = smem_u32(stage + slot * Z::stage1 + T * Z::xld + ((lane & 7) + (lane >> 4) * 8) * Z::ald + (lane >> 3 & 1) * 16);
+                const uint32_t xm = smem_u32(stage + slot * s1 + (16 * mt + (lane & 15)) * Z::xld + (lane >> 4) * 16);
+                const uint32_t wm = smem_u32(stage + slot * s1 + T * Z::xld + ((lane & 7) + (lane >> 4) * 8) * Z::ald + (lane >> 3 & 1) * 16);
                 // fp32: a lane has four consecutive k of every row; the products do not mind in which order the tensor core takes them, as long as both operands agree.
 #pragma unroll
                 for (int s = 0; s < KC / 16 / KS; ++s) {
@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
     const int units = (P.M + 31) / 32, m_from = 32 * (int)((long long)units * rank / S), m_to = min(P.M, 32 * (int)((long long)units * (rank + 1) / S));
     const int chunks = max(1, (r16 + kAdChunk - 1) / kAdChunk), rc = min(r16, kAdChunk), wld = Z::wld(rc), s2 = Z::stage2(rc);
     const int count = (max(m_to - m_from, 0) + FB - 1) / FB * chunks;
-    const float s0 = r_all ? sh.scale[16 * mt + g] : 0.f, s1 = r_all ? sh.scale[16 * mt + g + 8] : 0.f;
+    const float t0 = r_all ? sh.scale[16 * mt + g] : 0.f, t1 = r_all ? sh.scale[16 * mt + g + 8] : 0.f;
     const bool have0 = 16 * mt + g < n_rows, have1 = 16 * mt + g + 8 < n_rows;
     X* o0 = op + (int64_t)sh.rows[min(16 * mt + g, n_rows - 1)] * P.ldout + m_from + FW * ks + 4 * q;  // of this stage
     X* o1 = op + (int64_t)sh.rows[min(16 * mt + g + 8, n_rows - 1)] * P.ldout + m_from + FW * ks + 4 * q;
@@ -563,9 +563,9 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             if (bp)
 #pragma unroll
                 for (int p = 0; p < BP; ++p) {
-                    if (whole)
-                        ad_copy16(bs + p * (kAdThreads / BU) * Z::bld, bnext[p]);
-                    else
+                    if (whole) {
+                        if (brow + p * (kAdThreads / BU) < n_rows) ad_copy16(bs + p * (kAdThreads / BU) * Z::bld, bnext[p]);
+                    } else
                         ad_fill16(bs + p * (kAdThreads / BU) * Z::bld, bnext[p], left - bu, P.wide_base, bp);
                     bnext[p] += FB;
                 }
@@ -613,8 +613,8 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                     }
                 }
                 if (r_all) {
-                    v0 = make_float4(fmaf(s0, acc[2 * h][0], v0.x), fmaf(s0, acc[2 * h][1], v0.y), fmaf(s0, acc[2 * h + 1][0], v0.z), fmaf(s0, acc[2 * h + 1][1], v0.w));
-                    v1 = make_float4(fmaf(s1, acc[2 * h][2], v1.x), fmaf(s1, acc[2 * h][3], v1.y), fmaf(s1, acc[2 * h + 1][2], v1.z), fmaf(s1, acc[2 * h + 1][3], v1.w));
+                    v0 = make_float4(fmaf(t0, acc[2 * h][0], v0.x), fmaf(t0, acc[2 * h][1], v0.y), fmaf(t0, acc[2 * h + 1][0], v0.z), fmaf(t0, acc[2 * h + 1][1], v0.w));
+                    v1 = make_float4(fmaf(t1, acc[2 * h][2], v1.x), fmaf(t1, acc[2 * h][3], v1.y), fmaf(t1, acc[2 * h + 1][2], v1.z), fmaf(t1, acc[2 * h + 1][3], v1.w));
                 }
                 if (whole) {
                     if (have0) ad_store4(o0 + 16 * h, v0);
