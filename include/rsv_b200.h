@@ -33,6 +33,14 @@ typedef struct {
     int64_t w_mid, a_mid, v_mid, g_mid;
 } rsv_model_info;
 
+/* Settings of a token drawn from a given random number (rsv_infer_draw, rsv_draw_tokens; no counterpart in the reference). */
+typedef struct {
+    float temperature; /* <= 0: the largest logit */
+    uint32_t top_k;    /* 0: all */
+    float top_p;       /* <= 0 or >= 1: all */
+    float min_p;       /* <= 0: all */
+} rsv_draw_params;
+
 /* SamplerParams (src/gpu_model.rs:3883-3913).  Defaults: 1.0, 0, 1.0, 0, 1.0, 0.0, 0.0. */
 typedef struct {
     float temperature;
@@ -87,6 +95,19 @@ int rsv_state_slot_copy(rsv_state* dst, int64_t dst_slot, rsv_state* src, int64_
 /* State::reset / Bundle::reset (src/gpu_model.rs:4098-4104, 3759). */
 int rsv_state_reset(rsv_state* s);
 
+/* ---- adapters of sessions ---------------------------------------------------------------------
+ * No counterpart in the reference.  A model can hold low-rank adapters beside its att.output and ffn.value projections: with A [rank, K] and B [n_embd, rank]
+ * of the session's adapter a layer's projection of x gets scale B (A x) added (K = n_embd for att.output, ffn_hidden for ffn.value).  Sessions with different
+ * adapters, and without, share every step (rsv_adapters_apply below).  States, prompts, self-loops and the scheduler work as without; sessions without an
+ * adapter give the results they gave before. */
+enum { RSV_SITE_ATT_OUTPUT = 0, RSV_SITE_FFN_VALUE = 1 };
+/* Room for `slots` adapters (<= 4096) of up to max_rank (<= 256) at both sites of every layer, all of rank 0; once per model. */
+int rsv_model_adapters_new(rsv_model* m, int64_t slots, int64_t max_rank);
+/* One matrix pair of adapter `slot` as fp16 bits, a[rank * K] and b[n_embd * rank]; rank 0 (a and b may be NULL): none here.  Waits for the model's queued work. */
+int rsv_model_adapter_set(rsv_model* m, int64_t slot, int64_t layer, int site, int64_t rank, const uint16_t* a, const uint16_t* b, float scale);
+/* The session in `slot` of the state uses this adapter from the next call on (-1: none, as at first).  Resetting or loading a state does not change it. */
+int rsv_state_set_adapter(rsv_state* s, int64_t slot, int64_t adapter);
+
 /* ---- single-session inference (state must have batch == 1) ----------------------------------- */
 /* Bundle::infer_tokens (src/gpu_model.rs:3729): token-by-token decode path; logits_out[V] of the last token. */
 int rsv_infer_tokens(rsv_model* m, rsv_state* s, const uint32_t* tokens, int64_t n, float* logits_out);
@@ -103,6 +124,9 @@ int rsv_infer_argmax_selfloop(rsv_model* m, rsv_state* s, uint32_t seed, int64_t
 /* Bundle::infer_sample (src/gpu_model.rs:3826): history[nh] feeds the penalties. */
 int rsv_infer_sample(rsv_model* m, rsv_state* s, const uint32_t* tokens, int64_t n, const rsv_sampler_params* sp, const uint32_t* history,
                      int64_t nh, uint32_t* token_out);
+/* As rsv_infer_sample with the caller's random number u in [0, 1) in place of a seed and with min-p; the rules are those of rsv_draw_tokens below.
+ * logprob_out (may be NULL): the token's log-probability among what was kept.  No counterpart in the reference. */
+int rsv_infer_draw(rsv_model* m, rsv_state* s, const uint32_t* tokens, int64_t n, const rsv_draw_params* dp, float u, uint32_t* token_out, float* logprob_out);
 /* Bundle::infer_sample_selfloop (src/gpu_model.rs:3834): RNG seed of round r is `seed + r`, history = the r tokens
  * generated so far (src/gpu_model.rs:790-810). */
 int rsv_infer_sample_selfloop(rsv_model* m, rsv_state* s, uint32_t seed, int64_t n, const rsv_sampler_params* sp, uint32_t* out);
@@ -138,6 +162,8 @@ typedef struct rsv_sched rsv_sched;
 int rsv_sched_new(rsv_model* m, int64_t max_slots, int64_t chunk, int64_t max_rows, int64_t max_new_cap, rsv_sched** out);
 void rsv_sched_free(rsv_sched* s);
 int rsv_sched_submit(rsv_sched* s, const uint32_t* prompt, int64_t n_prompt, int64_t max_new, const rsv_sampler_params* sp, int64_t* id_out);
+/* The same with an adapter of the model for the session (-1: none). */
+int rsv_sched_submit_adapter(rsv_sched* s, const uint32_t* prompt, int64_t n_prompt, int64_t max_new, const rsv_sampler_params* sp, int64_t adapter, int64_t* id_out);
 /* Queues one step.  rows_out: rows packed into it (0 = nothing to do); active_out: sessions not yet finished. */
 int rsv_sched_step(rsv_sched* s, int64_t* rows_out, int64_t* active_out);
 /* Ids of sessions whose tokens have reached the host since the last poll (never blocks). */

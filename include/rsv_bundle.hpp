@@ -35,6 +35,11 @@ struct SamplerParams : rsv_sampler_params {
     SamplerParams() : rsv_sampler_params{1.0f, 0u, 1.0f, 0u, 1.0f, 0.0f, 0.0f} {}  // impl Default, :3901-3912
 };
 
+// settings of a token drawn from a given random number (Bundle::infer_draw; not in the reference)
+struct DrawParams : rsv_draw_params {
+    DrawParams() : rsv_draw_params{1.0f, 0u, 1.0f, 0.0f} {}
+};
+
 enum class RnnOption { Last, Full };
 struct RnnInput {
     std::vector<uint32_t> tokens;
@@ -75,6 +80,8 @@ public:
     void slot_restore(size_t slot, const std::string& path) const { check(rsv_state_slot_restore(h_, (int64_t)slot, path.c_str())); }
     // session migration: slot src_slot of src -> slot `slot` here, device to device (slot_back + slot_load without the host)
     void slot_copy_from(size_t slot, const State& src, size_t src_slot) const { check(rsv_state_slot_copy(h_, (int64_t)slot, src.h_, (int64_t)src_slot)); }
+    // the session in `slot` uses this adapter of the model from now on (-1: none)
+    void set_adapter(size_t slot, int64_t adapter) const { check(rsv_state_set_adapter(h_, (int64_t)slot, adapter)); }
     void reset() const { check(rsv_state_reset(h_)); }
     rsv_state* handle() const { return h_; }
 
@@ -229,6 +236,12 @@ public:
         uint32_t t = 0;
         check(rsv_infer_sample(model.handle(), state.handle(), tokens.data(), (int64_t)tokens.size(), &sp, history.empty() ? nullptr : history.data(),
                                (int64_t)history.size(), &t));
+        return t;
+    }
+    // the next token, drawn with the random number u in [0, 1); logprob (may be null): its log-probability among what was kept
+    uint32_t infer_draw(const std::vector<uint32_t>& tokens, const DrawParams& dp, float u, float* logprob = nullptr) {
+        uint32_t t = 0;
+        check(rsv_infer_draw(model.handle(), state.handle(), tokens.data(), (int64_t)tokens.size(), &dp, u, &t, logprob));
         return t;
     }
     std::vector<uint32_t> infer_sample_selfloop(uint32_t seed, size_t n, const SamplerParams& sp) {

@@ -16,7 +16,7 @@ _PKG = _os.path.dirname(_os.path.abspath(__file__))
 LIB_CUDA = _os.path.join(_PKG, "librsv_b200.so")
 LIB_SYNTH = _os.path.join(_PKG, "librsv_synth.so")
 
-__all__ = ["ModelBuilder", "Bundle", "State", "Scheduler", "SamplerParams", "RnnInput", "RnnOption", "ModelInfo", "RsvError", "write_synthetic", "SHAPES",
+__all__ = ["ModelBuilder", "Bundle", "State", "Scheduler", "SamplerParams", "DrawParams", "RnnInput", "RnnOption", "ModelInfo", "RsvError", "write_synthetic", "SHAPES",
            "quantize_int8", "op_dequant_int8", "op_linear", "op_wkv7", "op_argmax", "op_sample", "draw_params", "draw_tokens", "Adapters", "native", "ABI_SYMBOLS"]
 
 
@@ -34,7 +34,7 @@ ABI_SYMBOLS = [
     "rsv_prof_enable", "rsv_prof_clear", "rsv_prof_dump", "rsv_launch_count", "rsv_timer_start", "rsv_timer_stop", "rsv_synchronize",
     "rsv_sched_new", "rsv_sched_free", "rsv_sched_submit", "rsv_sched_step", "rsv_sched_poll", "rsv_sched_result", "rsv_sched_sync",
     "rsv_sched_stats", "rsv_quantize_int8", "rsv_op_dequant_int8", "rsv_op_linear", "rsv_op_wkv7", "rsv_op_argmax", "rsv_op_sample", "rsv_op_sample_static",
-    "rsv_draw_tokens", "rsv_adapters_apply",
+    "rsv_draw_tokens", "rsv_adapters_apply", "rsv_infer_draw", "rsv_model_adapters_new", "rsv_model_adapter_set", "rsv_state_set_adapter", "rsv_sched_submit_adapter",
 ]
 
 
@@ -51,6 +51,14 @@ class SamplerParams(_c.Structure):
 
     def __init__(self, temperature=1.0, top_k=0, top_p=1.0, seed=0, repetition_penalty=1.0, frequency_penalty=0.0, presence_penalty=0.0):
         super().__init__(temperature, top_k, top_p, seed, repetition_penalty, frequency_penalty, presence_penalty)
+
+
+class DrawParams(_c.Structure):
+    """Settings of a token drawn from a given random number (rsv_draw_params)."""
+    _fields_ = [("temperature", _c.c_float), ("top_k", _c.c_uint32), ("top_p", _c.c_float), ("min_p", _c.c_float)]
+
+    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        super().__init__(temperature, top_k, top_p, min_p)
 
 
 _native = None
@@ -93,6 +101,11 @@ def native():
         L.rsv_infer_chunked.argtypes = [vp, vp, vp, i64, i64, vp]
         L.rsv_infer_argmax_selfloop.argtypes = [vp, vp, u32, i64, vp]
         L.rsv_infer_sample.argtypes = [vp, vp, vp, i64, _c.POINTER(SamplerParams), vp, i64, vp]
+        L.rsv_infer_draw.argtypes = [vp, vp, vp, i64, _c.POINTER(DrawParams), _c.c_float, vp, vp]
+        L.rsv_model_adapters_new.argtypes = [vp, i64, i64]
+        L.rsv_model_adapter_set.argtypes = [vp, i64, i64, _c.c_int, i64, vp, vp, _c.c_float]
+        L.rsv_state_set_adapter.argtypes = [vp, i64, i64]
+        L.rsv_sched_submit_adapter.argtypes = [vp, vp, i64, i64, _c.POINTER(SamplerParams), i64, _c.POINTER(i64)]
         L.rsv_infer_sample_selfloop.argtypes = [vp, vp, u32, i64, _c.POINTER(SamplerParams), vp]
         L.rsv_prefill_batch.argtypes = [vp, vp, vp, vp, i64, i64, vp]
         L.rsv_prefill_batch_mean_hidden.argtypes = [vp, vp, vp, vp, i64, i64, vp]
@@ -246,6 +259,24 @@ class Model:
         _check(native().rsv_sample_selfloop_collect(t, _ptr(out), out.size))
         return out
 
+    # ---- adapters of sessions ----
+    SITES = ("att.output", "ffn.value")
+
+    def adapters_new(self, slots, max_rank):
+        """Room for `slots` low-rank adapters of up to max_rank beside att.output and ffn.value of every layer."""
+        _check(native().rsv_model_adapters_new(self._h, int(slots), int(max_rank)))
+
+    def adapter_set(self, slot, layer, site, A, B, scale=1.0):
+        """Adapter `slot` adds scale B (A x) to the projection `site` ("att.output" or "ffn.value") of a layer; A [rank, K], B [n_embd, rank].  A None: nothing."""
+        if A is None:
+            _check(native().rsv_model_adapter_set(self._h, int(slot), int(layer), self.SITES.index(site), 0, None, None, 1.0))
+            return
+        a, b = _np.ascontiguousarray(A, dtype=_np.float16), _np.ascontiguousarray(B, dtype=_np.float16)
+        K = self._info.num_emb if site == "att.output" else self._info.ffn_hidden
+        if site not in self.SITES or a.ndim != 2 or a.shape[1] != K or b.shape != (self._info.num_emb, a.shape[0]):
+            raise RsvError(f"adapter_set: A {a.shape} and B {b.shape} do not go with {site} of {K} inputs and {self._info.num_emb} outputs")
+        _check(native().rsv_model_adapter_set(self._h, int(slot), int(layer), self.SITES.index(site), a.shape[0], _ptr(a), _ptr(b), float(scale)))
+
     # ---- diagnostics ----
     def prof_enable(self, on=True):
         _check(native().rsv_prof_enable(self._h, 1 if on else 0))
@@ -322,6 +353,10 @@ class State:
         """Session migration: slot `src_slot` of state `src` (any model handle of the same shape, any GPU) -> slot `slot` here."""
         _check(native().rsv_state_slot_copy(self._h, int(slot), src._h, int(src_slot)))
 
+    def set_adapter(self, slot, adapter):
+        """The session in `slot` uses this adapter of the model from now on (-1 or None: none)."""
+        _check(native().rsv_state_set_adapter(self._h, int(slot), -1 if adapter is None else int(adapter)))
+
     def reset(self):
         _check(native().rsv_state_reset(self._h))
 
@@ -389,6 +424,12 @@ class Bundle:
         _check(native().rsv_infer_sample(self.model._h, self.state._h, _ptr(t), t.size, _c.byref(sp), _ptr(h) if h.size else None, h.size, _ptr(out)))
         return int(out[0])
 
+    def infer_draw(self, tokens, params, u):
+        """The next token and its log-probability, drawn with the random number u in [0, 1) after `params` (DrawParams)."""
+        t, out, lp = _tokens(tokens), _np.zeros(1, dtype=_np.uint32), _np.zeros(1, dtype=_np.float32)
+        _check(native().rsv_infer_draw(self.model._h, self.state._h, _ptr(t), t.size, _c.byref(params), float(u), _ptr(out), _ptr(lp)))
+        return int(out[0]), float(lp[0])
+
     def infer_sample_selfloop(self, seed, n, sp):
         out = _np.zeros(int(n), dtype=_np.uint32)
         _check(native().rsv_infer_sample_selfloop(self.model._h, self.state._h, int(seed), int(n), _c.byref(sp), _ptr(out)))
@@ -420,10 +461,11 @@ class Scheduler:
         _check(native().rsv_sched_new(model._h, int(max_slots), int(chunk), int(max_rows), int(max_new_cap), _c.byref(h)))
         self._h, self._model, self._cap = h, model, int(max_new_cap)
 
-    def submit(self, prompt, max_new, sp=None):
+    def submit(self, prompt, max_new, sp=None, adapter=None):
         t = _tokens(prompt)
         rid = _c.c_int64()
-        _check(native().rsv_sched_submit(self._h, _ptr(t), t.size, int(max_new), _c.byref(sp) if sp is not None else None, _c.byref(rid)))
+        _check(native().rsv_sched_submit_adapter(self._h, _ptr(t), t.size, int(max_new), _c.byref(sp) if sp is not None else None, -1 if adapter is None else int(adapter),
+                                                 _c.byref(rid)))
         return int(rid.value)
 
     def step(self):

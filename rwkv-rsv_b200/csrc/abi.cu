@@ -100,7 +100,7 @@ void decode_tokens(Model& m, State& st, const uint32_t* tokens, int64_t n) {
     need(n >= 1 && n <= 0x7fffffff, "empty token list (the count must be between 1 and 2^31 - 1)");
     check_tokens(m, tokens, n);
     RSV_CUDA(cudaSetDevice(m.device));
-    if (!m.prof_on && m.stream_available()) {
+    if (!m.prof_on && !st.adapted(0) && m.stream_available()) {
         m.ensure_workspace(1, 1, 1);
         if (n == 1) {
             m.run_stream(st, 0, 1, true, false, nullptr, nullptr, 0, tokens);
@@ -269,7 +269,7 @@ std::unique_ptr<rsv_ticket> selfloop_submit(Model& m, State& st, const uint32_t*
         else
             engine_argmax(m, m.ws.logits, B, m.ws.tokens, t.seq, t.cnt, (int)n);
     };
-    if (!m.prof_on && B == 1 && m.stream_available()) {
+    if (!m.prof_on && B == 1 && !st.adapted(0) && m.stream_available()) {
         // one session: the weight-streaming kernel runs whole steps (and, for arg-max, the whole self-loop) in one launch
         if (!sp) {
             m.run_stream(st, 0, (int)n, false, true, t.seq, t.cnt, (int)n);
@@ -541,6 +541,39 @@ int rsv_state_slot_copy(rsv_state* dst, int64_t dst_slot, rsv_state* src, int64_
     });
 }
 
+// ---- adapters of sessions ---------------------------------------------------------------------------------
+int rsv_model_adapters_new(rsv_model* mh, int64_t slots, int64_t max_rank) {
+    return guarded([&] {
+        need(mh, "null argument");
+        need(slots >= 1 && slots <= 4096, "adapters_new: slots must be between 1 and 4096");
+        need(max_rank >= 1 && max_rank <= 256, "adapters_new: max_rank must be between 1 and 256");
+        mh->m->new_adapters((int)slots, (int)max_rank);
+    });
+}
+int rsv_model_adapter_set(rsv_model* mh, int64_t slot, int64_t layer, int site, int64_t rank, const uint16_t* a, const uint16_t* b, float scale) {
+    return guarded([&] {
+        need(mh, "null argument");
+        Model& m = *mh->m;
+        need(m.adapters.mem, "adapter_set: the model has no adapters (rsv_model_adapters_new)");
+        need(slot >= 0 && slot < m.adapters.slots, "adapter_set: slot out of range");
+        need(layer >= 0 && layer < m.cfg.n_layer, "adapter_set: layer out of range");
+        need(site == RSV_SITE_ATT_OUTPUT || site == RSV_SITE_FFN_VALUE, "adapter_set: site must be RSV_SITE_ATT_OUTPUT or RSV_SITE_FFN_VALUE");
+        need(rank >= 0 && rank <= m.adapters.max_rank, "adapter_set: rank out of range");
+        need(rank == 0 || (a && b), "null argument");
+        m.set_adapter((int)slot, (int)layer, site, (int)rank, a, b, scale);
+    });
+}
+int rsv_state_set_adapter(rsv_state* sh, int64_t slot, int64_t adapter) {
+    return guarded([&] {
+        need(sh, "null argument");
+        State& s = sh->s;
+        need(slot >= 0 && slot < s.cap, "set_adapter: slot >= batch");
+        need(adapter == -1 || (adapter >= 0 && adapter < s.model->adapters.slots), "set_adapter: the model has no such adapter");
+        RSV_CUDA(cudaSetDevice(s.model->device));
+        s.set_adapter(slot, (int32_t)adapter);
+    });
+}
+
 int rsv_state_reset(rsv_state* sh) {
     return guarded([&] {
         need(sh, "null argument");
@@ -622,6 +655,33 @@ int rsv_infer_sample(rsv_model* mh, rsv_state* s, const uint32_t* tokens, int64_
         cudaFree(d_row);
         if (d_hist) cudaFree(d_hist);
         if (rc) throw std::runtime_error(g_err);
+    });
+}
+int rsv_infer_draw(rsv_model* mh, rsv_state* s, const uint32_t* tokens, int64_t n, const rsv_draw_params* dp, float u, uint32_t* token_out, float* logprob_out) {
+    return guarded([&] {
+        need(mh && s && tokens && dp && token_out, "null argument");
+        need(u >= 0.0f && u < 1.0f, "infer_draw: u must be in [0, 1)");
+        Model& m = *mh->m;
+        need(m.cfg.vocab <= 1 << 22, "infer_draw: vocabularies of up to 2^22 tokens");
+        decode_tokens(m, s->s, tokens, n);
+        struct {
+            rsv_draw_params p;
+            float u;
+            uint32_t token;
+            float logprob;
+        } row = {*dp, u, 0u, 0.f}, *dev = nullptr;
+        RSV_CUDA(device_malloc(&dev, sizeof(row)));
+        int rc = guarded([&] {
+            RSV_CUDA(cudaMemcpyAsync(dev, &row, sizeof(row), cudaMemcpyHostToDevice, m.stream));
+            engine_draw_row(m, &dev->p.temperature, &dev->u, &dev->token, &dev->logprob);
+            RSV_CUDA(cudaMemcpyAsync(&row, dev, sizeof(row), cudaMemcpyDeviceToHost, m.stream));
+            m.check_status();
+        });
+        cudaStreamSynchronize(m.stream);  // (nothing writes to `row` after an error either)
+        cudaFree(dev);
+        if (rc) throw std::runtime_error(g_err);
+        *token_out = row.token;
+        if (logprob_out) *logprob_out = row.logprob;
     });
 }
 int rsv_infer_sample_selfloop(rsv_model* m, rsv_state* s, uint32_t seed, int64_t n, const rsv_sampler_params* sp, uint32_t* out) {

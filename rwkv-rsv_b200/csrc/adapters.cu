@@ -61,7 +61,11 @@ static void launch_adapters(cudaStream_t stream, int device, AdapterArgs P) {
         launch_tiles<X, W, 1, 3>(stream, device, P);
 }
 
-void engine_adapters(cudaStream_t stream, int device, int xtype, int wtype, AdapterArgs P) {
+void engine_apply_adapters(cudaStream_t stream, int device, const rsv_adapters& ad, int xtype, const void* x, int64_t x_stride, int64_t rows, const int32_t* index,
+                           const void* base, int64_t base_stride, void* out, int64_t out_stride) {
+    AdapterArgs P = {x, index, ad.a, ad.b, ad.ranks, ad.scales, base, out, x_stride, base_stride, out_stride, ad.a_slot, ad.a_row, ad.b_slot, ad.b_row, (int)rows, (int)ad.K, (int)ad.M,
+                     (int)ad.slots, (int)ad.max_rank};
+    const int wtype = ad.dtype;
     const int xs = xtype == RSV_F32 ? 4 : 2;
     const auto at = [](int bytes, const void* p, int64_t size, std::initializer_list<int64_t> strides) {  // rows start at multiples of `bytes`
         bool ok = (uintptr_t)p % bytes == 0;
@@ -122,8 +126,6 @@ extern "C" int rsv_adapters_apply(int device, void* stream, const rsv_adapters* 
             if (o0 < p1 && p0 < o1) throw std::runtime_error("adapters: out and base overlap without being the same rows");
         }
         DeviceScope on(device);
-        AdapterArgs P = {x_dev, index_dev, ad->a, ad->b, ad->ranks, ad->scales, base_dev, out_dev, x_stride, base_stride, out_stride, ad->a_slot, ad->a_row, ad->b_slot, ad->b_row,
-                         (int)rows, (int)ad->K, (int)ad->M, (int)ad->slots, (int)ad->max_rank};
-        engine_adapters((cudaStream_t)stream, device, xtype, ad->dtype, P);
+        engine_apply_adapters((cudaStream_t)stream, device, *ad, xtype, x_dev, x_stride, rows, index_dev, base_dev, base_stride, out_dev, out_stride);
     });
 }

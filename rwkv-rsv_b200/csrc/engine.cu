@@ -433,7 +433,7 @@ std::unique_ptr<Model> Model::create_bare(int device) {
 }
 
 static void free_workspace(Workspace& w) {
-    void* ptrs[] = {w.x, w.x2, w.delta, w.r, w.k, w.v, w.w, w.a, w.g, w.yg, w.xb, w.mid, w.h, w.vfirst, w.logits, w.staging_t, w.staging_c, w.ymax, w.hmax, w.tokens, w.row_meta, w.seg_meta, w.out_rows, w.samp_temp, w.samp_cnt};
+    void* ptrs[] = {w.x, w.x2, w.delta, w.r, w.k, w.v, w.w, w.a, w.g, w.yg, w.xb, w.mid, w.h, w.vfirst, w.logits, w.staging_t, w.staging_c, w.ymax, w.hmax, w.tokens, w.row_adapter, w.row_meta, w.seg_meta, w.out_rows, w.samp_temp, w.samp_cnt};
     for (void* p : ptrs)
         if (p) cudaFree(p);
     int* status = w.status;
@@ -458,6 +458,7 @@ Model::~Model() {
     if (ws.tok_pos) cudaFree(ws.tok_pos);
     if (ws.tok_list) cudaFree(ws.tok_list);
     for (void* p : allocs) cudaFree(p);
+    if (adapters.mem) cudaFree(adapters.mem);
     if (ws.op_mem) cudaFree(ws.op_mem);
     ws.wkv_tmp.release();
     for (void* p : {sctx.d_layers, sctx.wstream, sctx.hstream, (void*)sctx.exchange, (void*)sctx.cand_val, (void*)sctx.cand_idx, (void*)sctx.grid_bar})
@@ -479,6 +480,68 @@ State::~State() {
     if (!wkv) return;
     cudaSetDevice(pool->device);
     pool->give(bytes, wkv);
+    if (adapter_dev) cudaFree(adapter_dev);
+}
+
+static __global__ void set_int_kernel(int32_t* p, int32_t v) { *p = v; }
+static __global__ void row_adapters_kernel(const RowMeta* __restrict__ rows, const int32_t* __restrict__ of_slot, int R, int32_t* __restrict__ out) {
+    const int r = blockIdx.x * blockDim.x + threadIdx.x;
+    if (r < R) out[r] = of_slot[rows[r].slot];
+}
+
+void State::set_adapter(int64_t slot, int32_t adapter_index) {
+    if (adapter.empty()) {
+        if (adapter_index < 0) return;
+        RSV_CUDA(device_malloc(&adapter_dev, (size_t)cap * sizeof(int32_t)));
+        RSV_CUDA(cudaMemsetAsync(adapter_dev, 0xFF, (size_t)cap * sizeof(int32_t), model->stream));
+        adapter.assign((size_t)cap, -1);
+    }
+    if (adapter[(size_t)slot] == adapter_index) return;
+    set_int_kernel<<<1, 1, 0, model->stream>>>(adapter_dev + slot, adapter_index);
+    RSV_CUDA(cudaGetLastError());
+    adapter[(size_t)slot] = adapter_index;
+}
+
+void Model::new_adapters(int slots, int max_rank) {
+    if (adapters.mem) throw std::runtime_error("adapters_new: this model has its adapters already");
+    RSV_CUDA(cudaSetDevice(device));
+    const size_t C = cfg.n_embd, F = cfg.ffn_hidden;
+    const auto aligned = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+    size_t total = 0;
+    for (size_t K : {C, F}) total += aligned((size_t)slots * max_rank * K * 2) + aligned((size_t)slots * max_rank * C * 2) + 2 * aligned((size_t)slots * 4);
+    total *= (size_t)cfg.n_layer;
+    char* p = nullptr;
+    RSV_CUDA(device_malloc(&p, total));
+    adapters.mem = p;
+    RSV_CUDA(cudaMemsetAsync(p, 0, total, stream));  // (rank 0 everywhere)
+    adapters.layers.resize((size_t)cfg.n_layer);
+    for (auto& layer : adapters.layers)
+        for (int site = 0; site < 2; ++site) {
+            ModelAdapters::Site& s = layer[(size_t)site];
+            s.K = site == RSV_SITE_ATT_OUTPUT ? (int)C : (int)F;
+            s.a = reinterpret_cast<__half*>(p), p += aligned((size_t)slots * max_rank * s.K * 2);
+            s.b = reinterpret_cast<__half*>(p), p += aligned((size_t)slots * max_rank * C * 2);
+            s.ranks = reinterpret_cast<int32_t*>(p), p += aligned((size_t)slots * 4);
+            s.scales = reinterpret_cast<float*>(p), p += aligned((size_t)slots * 4);
+        }
+    adapters.slots = slots;
+    adapters.max_rank = max_rank;
+    RSV_CUDA(cudaStreamSynchronize(stream));
+}
+
+void Model::set_adapter(int slot, int layer, int site, int rank, const uint16_t* a, const uint16_t* b, float scale) {
+    RSV_CUDA(cudaSetDevice(device));
+    ModelAdapters::Site& s = adapters.layers[(size_t)layer][(size_t)site];
+    const size_t C = cfg.n_embd, most = (size_t)adapters.max_rank;
+    const int32_t r = rank;
+    RSV_CUDA(cudaStreamSynchronize(stream));
+    if (rank > 0) {
+        RSV_CUDA(cudaMemcpyAsync(s.a + slot * most * s.K, a, (size_t)rank * s.K * 2, cudaMemcpyHostToDevice, stream));
+        RSV_CUDA(cudaMemcpy2DAsync(s.b + slot * most * C, most * 2, b, (size_t)rank * 2, (size_t)rank * 2, C, cudaMemcpyHostToDevice, stream));
+    }
+    RSV_CUDA(cudaMemcpyAsync(s.ranks + slot, &r, 4, cudaMemcpyHostToDevice, stream));
+    RSV_CUDA(cudaMemcpyAsync(s.scales + slot, &scale, 4, cudaMemcpyHostToDevice, stream));
+    RSV_CUDA(cudaStreamSynchronize(stream));
 }
 
 void State::allocate(Model* m, int64_t slots) {
@@ -539,6 +602,7 @@ void Model::ensure_workspace(int rows, int outs, int segs) {
     }
     RSV_CUDA(device_malloc(&ws.tokens, R * sizeof(uint32_t)));
     RSV_CUDA(cudaMemsetAsync(ws.tokens, 0, R * sizeof(uint32_t), stream));
+    RSV_CUDA(device_malloc(&ws.row_adapter, R * sizeof(int32_t)));
     RSV_CUDA(device_malloc(&ws.row_meta, R * sizeof(RowMeta)));
     RSV_CUDA(device_malloc(&ws.seg_meta, (size_t)segs * sizeof(SegMeta)));
     RSV_CUDA(device_malloc(&ws.out_rows, (size_t)std::max(outs, 1) * sizeof(int)));
@@ -984,6 +1048,19 @@ void Model::forward_rows(State& st, const StepPlan& plan, bool use_cursor) {
                                                         ws.x, ws.status);
         check_launch("embed_ln0");
     }
+    // the sessions' adapters beside a projection, added to what it gave
+    const bool adapted = std::any_of(st.adapter.begin(), st.adapter.end(), [](int32_t a) { return a >= 0; });
+    if (adapted) LAUNCH(*this, "row_adapters") {
+            row_adapters_kernel<<<(R + 255) / 256, 256, 0, stream>>>(ws.row_meta, st.adapter_dev, R, ws.row_adapter);
+            check_launch("row_adapters");
+        }
+    const auto adapt = [&](int layer, int site, const float* x) {
+        if (!adapted) return;
+        const ModelAdapters::Site& s = adapters.layers[(size_t)layer][(size_t)site];
+        const int64_t most = adapters.max_rank;
+        const rsv_adapters ad = {RSV_F16, adapters.slots, most, s.K, C, s.a, most * s.K, s.K, s.b, most * C, most, s.ranks, s.scales};
+        LAUNCH(*this, "adapters") engine_apply_adapters(stream, device, ad, RSV_F32, x, s.K, R, ws.row_adapter, ws.delta, C, ws.delta, C);
+    };
     // The residual stream ping-pongs between two buffers: each LayerNorm kernel folds in the pending residual of the
     // linear layer before it (x_cur + pending -> x_alt) so that no linear epilogue has to read-modify-write x.
     float *x_cur = ws.x, *x_alt = ws.x2;
@@ -1139,6 +1216,7 @@ void Model::forward_rows(State& st, const StepPlan& plan, bool use_cursor) {
             run_rows_linear(*this, name, &q, 1, tn);
         };
         linear_known("linear_att_out", RlReq{&L.Wo, nullptr, ws.delta, C, EPI_STORE}, ws.yg, C, ws.ymax, yparts, ops.y);
+        adapt(l, RSV_SITE_ATT_OUTPUT, ws.yg);
         pending = ws.delta;
         {
             LnOperandsArgs A = ln_args(L.ln2_w, L.ln2_b, cmix_x, ws.staging_c, ws.staging_t, tmix_x);
@@ -1155,6 +1233,7 @@ void Model::forward_rows(State& st, const StepPlan& plan, bool use_cursor) {
             run_rows_linear(*this, "linear_ffn_key", &q, 1, tk);
         }
         linear_known("linear_ffn_value", RlReq{&L.Wfv, nullptr, ws.delta, C, EPI_STORE}, ws.h, F, ws.hmax, (F + kRlTileM - 1) / kRlTileM, ops.h);
+        adapt(l, RSV_SITE_FFN_VALUE, ws.h);
         pending = ws.delta;
     }
     LAUNCH(*this, "commit_shift") {
@@ -1495,6 +1574,10 @@ void engine_sample(Model& m, const float* logits_dev, int rows, const float* sam
         launch_sample(m.stream, logits_dev, rows, m.cfg.vocab, sampler8_dev, hist_dev, hist_stride, round_cnt_dev, m.ws.samp_temp, m.ws.samp_cnt, next_tok_dev, seq_dev,
                       seq_cnt_dev, seq_cap, row_map_dev);
     }
+}
+
+void engine_draw_row(Model& m, const float* params4_dev, const float* uniform_dev, uint32_t* token_dev, float* logprob_dev) {
+    LAUNCH(m, "draw") engine_draw(m.stream, m.device, RSV_F32, m.ws.logits, 1, m.cfg.vocab, m.cfg.vocab, params4_dev, uniform_dev, token_dev, logprob_dev);
 }
 
 void engine_sample_raw(cudaStream_t stream, const float* logits_dev, int rows, int V, const float* sampler8_dev, const uint32_t* hist_dev,

@@ -14,6 +14,7 @@
 
 #include "common.cuh"
 #include "device_memory.hpp"
+#include "rsv_b200.h"
 #include "stream_sequence.hpp"
 
 namespace rsv {
@@ -52,6 +53,19 @@ struct LayerW {
     std::array<const LinearW*, 6> big() const { return {&Wr, &Wk, &Wv, &Wo, &Wfk, &Wfv}; }  // the matrices that have any format
 };
 
+// Low-rank adapters beside a model's att.output and ffn.value projections (adapters.cuh), one allocation.
+struct ModelAdapters {
+    int slots = 0, max_rank = 0;
+    void* mem = nullptr;
+    struct Site {
+        __half *a = nullptr, *b = nullptr;  // [slots][max_rank][K], [slots][C][max_rank]
+        int32_t* ranks = nullptr;
+        float* scales = nullptr;
+        int K = 0;
+    };
+    std::vector<std::array<Site, 2>> layers;
+};
+
 struct Workspace {
     int rows = 0, outs = 0, segs = 0;  // capacities
     const float *final_x = nullptr, *final_delta = nullptr;  // after forward_rows: the last layer's residual stream of row i is final_x[i] + final_delta[i]
@@ -68,6 +82,7 @@ struct Workspace {
     uint32_t* tokens = nullptr;    // [rows] input token of every row (device-resident between self-loop rounds)
     uint32_t* tok_list = nullptr;  // token cursor mode: [tok_list_cap]
     size_t tok_list_cap = 0;
+    int32_t* row_adapter = nullptr;  // [rows] adapter of every row, where the model has some
     RowMeta* row_meta = nullptr;
     SegMeta* seg_meta = nullptr;
     int* out_rows = nullptr;
@@ -110,6 +125,11 @@ struct State {
     std::shared_ptr<StatePool> pool;
     CUtensorMap wkv_map;      // all layers' WKV states as one 2-D tensor [layers x slots x heads x 64][64] fp32 (TMA boxes of 64 rows x 32 columns)
     bool wkv_map_ok = false;  // encoded on first use
+    // the sessions' adapters (-1: none), allocated with the first one
+    int32_t* adapter_dev = nullptr;  // [cap]
+    std::vector<int32_t> adapter;
+    void set_adapter(int64_t slot, int32_t adapter_index);  // queued on the model's stream
+    bool adapted(int64_t slot) const { return !adapter.empty() && adapter[(size_t)slot] >= 0; }
     void allocate(Model* m, int64_t slots);
     void clear();  // zeros, on the model's stream
     ~State();
@@ -130,6 +150,9 @@ struct Model {
     __half* emb = nullptr;
     float *ln0_w = nullptr, *ln0_b = nullptr, *ln_out_w = nullptr, *ln_out_b = nullptr;
     LinearW head;
+    ModelAdapters adapters;
+    void new_adapters(int slots, int max_rank);
+    void set_adapter(int slot, int layer, int site, int rank, const uint16_t* a, const uint16_t* b, float scale);
     std::vector<LayerW> layers;
     std::vector<int> format_layers;  // the first layer of every combination of weight formats (one, as a rule)
     std::vector<void*> allocs;  // every weight allocation, freed in the destructor
@@ -208,6 +231,13 @@ void engine_op_linear(Model& m, int path, int wtype, const void* w_host, const u
 // vgate, vfirst ([nseg T, H 64] each; the last two null for the first layer); par[] = k_k, k_a, r_k, lnx_w, lnx_b ([H 64]);
 // state [nseg, H, 64, 64] is updated in place; y = (GroupNorm(S r) + (r . k~ r_k) v) g.  variant: 0 automatic, 1-4 one kernel each.
 void engine_op_wkv7(int device, int variant, int nseg, int T, int H, const float* const in[8], const float* const par[5], float* state_host, float* y_host);
+// Operators on device memory (adapters.cu, draw.cu).
+void engine_apply_adapters(cudaStream_t stream, int device, const rsv_adapters& ad, int xtype, const void* x, int64_t x_stride, int64_t rows, const int32_t* index,
+                           const void* base, int64_t base_stride, void* out, int64_t out_stride);
+void engine_draw(cudaStream_t stream, int device, int dtype, const void* logits_dev, int64_t rows, int64_t V, int64_t row_stride, const float* params4_dev,
+                 const float* uniforms_dev, uint32_t* tokens_dev, float* logprobs_dev);
+// ... of the last forward pass's first row
+void engine_draw_row(Model& m, const float* params4_dev, const float* uniform_dev, uint32_t* token_dev, float* logprob_dev);
 // acc[slot of segment][c] += sum over the segment's rows, in row order, of the last layer's residual stream left by forward_rows
 void engine_segment_sums(Model& m, int n_segments, float* acc_dev);
 void engine_quantize_int8(cudaStream_t stream, const float* w_dev, size_t M, size_t K, uint8_t* idx_dev, uint32_t* sz_dev);

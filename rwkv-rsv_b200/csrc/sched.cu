@@ -36,6 +36,7 @@ struct Request {
     int64_t max_new = 0;
     bool sample = false;
     rsv_sampler_params sp{};
+    int32_t adapter = -1;
     // progress
     int slot = -1;
     int64_t fed = 0;        // prompt tokens already given to the model
@@ -203,8 +204,12 @@ int rsv_sched_new(rsv_model* mh, int64_t max_slots, int64_t chunk, int64_t max_r
 void rsv_sched_free(rsv_sched* s) { delete s; }
 
 int rsv_sched_submit(rsv_sched* S, const uint32_t* prompt, int64_t n_prompt, int64_t max_new, const rsv_sampler_params* sp, int64_t* id_out) {
+    return rsv_sched_submit_adapter(S, prompt, n_prompt, max_new, sp, -1, id_out);
+}
+int rsv_sched_submit_adapter(rsv_sched* S, const uint32_t* prompt, int64_t n_prompt, int64_t max_new, const rsv_sampler_params* sp, int64_t adapter, int64_t* id_out) {
     return guarded([&] {
         need(S && prompt && id_out, "null argument");
+        need(adapter == -1 || (adapter >= 0 && adapter < S->m->adapters.slots), "sched_submit: the model has no such adapter");
         need(n_prompt >= 1, "sched_submit: empty prompt");
         need(max_new >= 1 && max_new <= S->seq_cap, "sched_submit: max_new must be in [1, max_new_cap]");
         for (int64_t i = 0; i < n_prompt; ++i)
@@ -215,6 +220,7 @@ int rsv_sched_submit(rsv_sched* S, const uint32_t* prompt, int64_t n_prompt, int
         r.max_new = max_new;
         r.sample = sp != nullptr;
         if (sp) r.sp = *sp;
+        r.adapter = (int32_t)adapter;
         *id_out = r.id;
         S->waiting.push_back(r.id);
         S->reqs.emplace(r.id, std::move(r));
@@ -238,6 +244,7 @@ int rsv_sched_step(rsv_sched* Sp, int64_t* rows_out, int64_t* active_out) {
             if (S.retiring[r.slot]) harvest(S, r.slot);  // the slot's previous tokens must have left its pinned area
             S.slot_owner[r.slot] = r.id;
             zero_slot(S, r.slot);
+            S.st.set_adapter(r.slot, r.adapter);
             if (!r.sample) {  // arg-max as a sampler row: keep only the largest logit
                 r.sp = rsv_sampler_params{1.0f, 1u, 1.0f, 0u, 1.0f, 0.0f, 0.0f};
             }
@@ -310,7 +317,7 @@ int rsv_sched_step(rsv_sched* Sp, int64_t* rows_out, int64_t* active_out) {
             }
             RSV_CUDA(cudaEventRecord(S.pin_ev[area], m.stream));
             engine_merge_tokens(m, S.host_tok_dev, S.slot_tok, R);
-            if (R == 1 && O == 1 && !m.prof_on && m.stream_available()) {
+            if (R == 1 && O == 1 && !m.prof_on && !S.st.adapted(p.rows[0].slot) && m.stream_available()) {
                 // one decoding session and nothing else (the tail of a workload): one launch of the weight-streaming kernel
                 m.run_stream(S.st, p.rows[0].slot, 1, false, false, nullptr, nullptr, 0);
             } else {

@@ -65,3 +65,10 @@ def test_draw_params_rows():
     assert np.array_equal(p.view(np.uint32)[:, 1], [50, 50]) and np.array_equal(p[:, 3], np.float32([0, 0.1])) and np.array_equal(p[:, 0], np.float32([0.5, 1]))
     with pytest.raises(rsv.RsvError, match="top_k"):
         rsv.draw_params(top_k=-1)
+
+
+def test_model_entry_points_refuse_null():
+    L = rsv.native()
+    for rc in (L.rsv_model_adapters_new(None, 1, 1), L.rsv_model_adapter_set(None, 0, 0, 0, 0, None, None, 1.0), L.rsv_state_set_adapter(None, 0, -1),
+               L.rsv_sched_submit_adapter(None, None, 0, 1, None, -1, None), L.rsv_infer_draw(None, None, None, 0, None, 0.5, None, None)):
+        assert rc != 0 and L.rsv_last_error().decode() == "null argument"
