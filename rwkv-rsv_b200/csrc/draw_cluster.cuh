@@ -4,12 +4,12 @@
 // found without sorting the row:
 //   list    Every thread keeps the largest of its own logits.  The k-th largest of a CTA's 256 such maxima is a lower bound of the row's k-th largest
 //           logit, and so is the smallest over the CTAs of the (k / CTAs)-th; the logits from the larger of the two on are collected (k and a few more) and
-//           sorted by value and index, and the cut lies among them.  With top-p and no top-k the 256 largest are tried: their weight tells whether
+//           sorted by value and index, and the cut lies among them.  With top-p and no top-k the 128 largest are tried: their weight tells whether
 //           the cut lies among them.
 //   region  Otherwise the cut lies in a stretch of values known from the pass that summed the weights (three stretches, divided by bounds from the threads'
 //           maxima).  A histogram of that stretch in 512 linear bins says near which bin the cut is; the logits of that bin and its neighbours are
 //           collected and sorted, the weight of all larger ones is summed exactly, and the sums tell whether the cut is there.
-//   neither Where a collection would not fit 512 entries (many equal logits) one CTA does the row by radix passes (dw_row_plain).
+//   neither Where a collection would not fit 384 entries (many equal logits) one CTA does the row by radix passes (dw_row_plain).
 // Without top-k and top-p no cut is needed: min-p's is a value that follows from the maximum.
 //
 // The draw: sums of the kept weights per warp, whose logits follow each other in the vocabulary, then the one warp's stretch again, split over a CTA.
@@ -22,14 +22,14 @@
 
 namespace rsv {
 
-constexpr int kDcList = 512;  // entries of a collection
-constexpr int kDcPer = kDcList / kDwThreads;
+constexpr int kDcList = 384;  // entries of a collection
+constexpr int kDcPer = 2;     // at most, of a thread
 constexpr int kDcBins = 512;
 constexpr int kDcBinsPer = kDcBins / kDwThreads;
 static_assert(kDcBinsPer == 2, "bins are read in pairs");
-constexpr int kDcFastK = 300;                   // most entries of top-k that are collected whole
+constexpr int kDcFastK = 160;                   // most entries of top-k that are collected whole
 constexpr int kDcMostPart = kDwThreads * 7 / 8;  // most of a CTA's thread maxima that are asked for
-constexpr int kDcTryK = 256;                     // entries tried for top-p alone,
+constexpr int kDcTryK = 128;                     // entries tried for top-p alone,
 constexpr int kDcTryPart = kDwThreads * 3 / 8;   // and of one CTA's thread maxima
 constexpr int kDcMaxCtas = 8;
 constexpr int kDcMarked = 8;  // vectors a thread can mark the logits of
@@ -50,13 +50,15 @@ struct DcShared {
     int n_list[3];                    // entries of the collections below (one after the other)
     alignas(16) u64 list[kDcList];    // key << 32 | ~index
     // read by the other CTAs
-    alignas(16) uint32_t hist[kDcBins];
+    alignas(16) uint2 hist[kDcBins];  // logits of a bin, and their weights relative to that of its upper end
     // this CTA's own
-    alignas(16) u64 mine[kDcList];
+    union {
+        alignas(16) u64 mine[kDcList];
+        alignas(16) uint32_t tmhist[256];  // (before anything is collected)
+    };
     double tab[16], rate, least;
     u64 wsum[kDwWarps], seg_a[kDwWarps], seg_c[kDwWarps], before, target, sum;
     float red[kDwWarps], redmin[kDwWarps], thr_all, thr_part, floor_l, min_l;
-    alignas(16) uint32_t tmhist[256];
     uint32_t first;
     int n_mine, n_above[kDwWarps], bin, bins, found;
 };
@@ -89,9 +91,9 @@ __device__ __forceinline__ uint32_t dc_map(const void* p, int rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
 }
-__device__ __forceinline__ uint2 dc_u32x2(const void* p, int rank) {
-    uint2 v;
-    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(dc_map(p, rank)) : "memory");
+__device__ __forceinline__ uint4 dc_u32x4(const void* p, int rank) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(dc_map(p, rank)) : "memory");
     return v;
 }
 __device__ __forceinline__ void dc_put(int rank, int* p, int v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dc_map(p, rank)), "r"(v) : "memory"); }
@@ -193,47 +195,26 @@ __device__ __forceinline__ u64 dc_before(u64 v, u64* wsum, u64& all) {
     all = t.y;
     return t.x;
 }
-// keys[0 .. n) in falling order, all different; up to a thread's number by counting the larger ones, more by a bitonic network (space for a power of two).
+// keys[0 .. n) in falling order, all different: a key's place is the number of larger ones.
 __device__ __noinline__ void dc_sort(u64* keys, int n) {
     const int tid = threadIdx.x;
-    if (n <= kDwThreads) {
-        u64 mine = tid < n ? keys[tid] : 0ull;
-        if (tid == 0 && n < kDwThreads) keys[n] = 0;  // (pairs are read)
-        __syncthreads();
-        int place = 0;
-        if (tid < n)
-#pragma unroll 4
-            for (int j = 0; j < n; j += 2) {
-                const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&keys[j]);
-                place += (k.x > mine) + (k.y > mine);
-            }
-        __syncthreads();
-        if (tid < n) keys[place] = mine;
-        __syncthreads();
-        return;
-    }
-    int np = kDwThreads;
-    while (np < n) np <<= 1;
-    for (int i = n + tid; i < np; i += kDwThreads) keys[i] = 0;
+    u64 mine[kDcPer];
+    int place[kDcPer];
+#pragma unroll
+    for (int e = 0; e < kDcPer; ++e) mine[e] = tid + e * kDwThreads < n ? keys[tid + e * kDwThreads] : ~0ull, place[e] = 0;
+    if (tid == 0 && n < kDcList) keys[n] = 0;  // (pairs are read)
     __syncthreads();
-#pragma unroll 1
-    for (int k = 2; k <= np; k <<= 1)
-#pragma unroll 1
-        for (int j = k >> 1; j > 0; j >>= 1) {
-#pragma unroll 1
-            for (int i = tid; i < np / 2; i += kDwThreads) {
-                const int a = 2 * i - (i & (j - 1)), b = a + j;
-                const u64 va = keys[a], vb = keys[b];
-                if ((a & k) == 0 ? va < vb : va > vb) {
-                    keys[a] = vb;
-                    keys[b] = va;
-                }
-            }
-            if (j > 32 || (j == 1 && k >= 64))  // (pairs up to 32 apart stay within 64 entries, which are always the same warp's)
-                __syncthreads();
-            else
-                __syncwarp();
+    if (tid < n)
+#pragma unroll 4
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&keys[j]);
+#pragma unroll
+            for (int e = 0; e < kDcPer; ++e) place[e] += (k.x > mine[e]) + (k.y > mine[e]);
         }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kDcPer; ++e)
+        if (tid + e * kDwThreads < n) keys[place[e]] = mine[e];
     __syncthreads();
 }
 // The least logit l (lowest finite .. max) with (l - max) c >= ymin, by a half warp: the quotient, and sixteen floats around it.
@@ -275,27 +256,51 @@ struct DcRow {
             f(v, dc_largest(v), warp * seg + o, i++);
         }
     }
-    // The marks of a vector's logits that `which` names (bit 4 i + e: logit e of a group of four of vector i).
-    template <class F>
-    __device__ __forceinline__ void mark(uint32_t (&marks)[N / 4], const float (&v)[N], int i, F&& which) const {
+    // The marks of a vector's logits from `least` on (bit 4 i + e: logit e of a group of four of vector i).
+    __device__ __forceinline__ void mark(uint32_t (&marks)[N / 4], const float (&v)[N], int i, float least) const {
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (which(v[e])) marks[e / 4] |= 1u << (e & 3) << 4 * i;
+        for (int g = 0; g < N / 4; ++g) {
+            uint32_t s[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) asm("set.ge.u32.f32 %0, %1, %2;" : "=r"(s[e]) : "f"(v[4 * g + e]), "f"(least));
+            marks[g] |= ((s[0] & 1u) | (s[1] & 2u) | (s[2] & 4u) | (s[3] & 8u)) << (4 * i);
+        }
     }
-    // f(logit, place) for the marked ones, or, where a stretch is too long for marks, for all.
+    // f(four logits, their places) for the marked ones, or, where a stretch is too long for marks, for all; -inf where there are no more.  (Four at a time: one
+    // after the other each would wait for the one before it.)
     template <class F>
     __device__ __forceinline__ void each(const uint32_t (&marks)[N / 4], F&& f) const {
         if (seg <= 32 * N * kDcMarked) {
 #pragma unroll
-            for (int g = 0; g < N / 4; ++g)
+            for (int g = 0; g < N / 4; ++g) {
+                uint32_t m = marks[g];
+                const int first = warp * seg + lane * N + 4 * g;
 #pragma unroll 1
-                for (uint32_t m = marks[g]; m; m &= m - 1) {
-                    const int b = __ffs(m) - 1, place = warp * seg + (b >> 2) * 32 * N + lane * N + 4 * g + (b & 3);
-                    f(dw_f32(slice[place]), place);
+                while (__any_sync(0xffffffffu, m != 0u)) {
+                    float l[4];
+                    int at[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int b = m ? __ffs(m) - 1 : 0;
+                        at[e] = first + (b >> 2) * 32 * N + (b & 3);
+                        l[e] = m ? dw_f32(slice[at[e]]) : -INFINITY;
+                        m &= m - 1;
+                    }
+                    f(l, at);
                 }
+            }
         } else {
 #pragma unroll 1
-            for (int o = lane; o < seg; o += 32) f(dw_f32(slice[warp * seg + o]), warp * seg + o);
+            for (int o = 0; o < seg; o += 128) {
+                float l[4];
+                int at[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    at[e] = warp * seg + o + 32 * e + lane;  // (a stretch is a multiple of 128 logits)
+                    l[e] = dw_f32(slice[at[e]]);
+                }
+                f(l, at);
+            }
         }
     }
     // g(logit, weight) for all logits of the vectors where a lane's largest is from `least` on (weights of logits under floor_l are any number).  Four chains at
@@ -585,7 +590,7 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
     // ---- the row, its largest logit, bounds of what is kept
     const float tm = R.load([&] {
         uint4* h = reinterpret_cast<uint4*>(sh.hist);
-        for (int i = tid; i < kDcBins / 4; i += kDwThreads) h[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < kDcBins / 2; i += kDwThreads) h[i] = make_uint4(0, 0, 0, 0);
         sh.tmhist[tid] = 0u;
         dw_fill_table(sh.tab, r.F);
         if (tid == 0) {
@@ -665,16 +670,26 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
     uint32_t marks[N / 4] = {};           // logits from from_l on
     const bool marked = R.seg <= 32 * N * kDcMarked;
     // The bin of a logit from from_l on and under to_l; in the last one: all that is further down.
-    float top_l = 0.f, per_bin = 0.f;
+    float top_l = 0.f, per_bin = 0.f, bin_y = 0.f;  // (bin_y: what y changes by from bin to bin)
+    const bool weighed = binned_k && r.top_p > 0.f;  // bins are weighed; otherwise a bin's weight is taken in its middle, which is good enough without the largest logits
+    const float rel_unit = marked ? 131072.0f : 16384.0f;  // (8192 or, of 16 bits, 16384 logits of a marked slice stay under 2^32, and up to 98304 of a long one)
     const auto set_bins = [&] {
         top_l = fminf(to_l, mx);
         const float span = fminf(top_l - from_l, 2.5f * (mx - mn));
         per_bin = span > 0.f ? fminf(((float)kDcBins - 1.0f) / span, 1e30f) : 1e30f;
+        bin_y = -(float)r.c / per_bin;
     };
     const auto where = [&](float l) { return fminf((top_l - l) * per_bin, (float)kDcBins - 0.5f); };
     const auto count = [&] {
-        R.each(marks, [&](float l, int) {
-            if (l >= from_l && l < to_l) atomicAdd(&sh.hist[(int)where(l)], 1u);
+        R.each(marks, [&](const float (&l)[4], const int (&)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (l[e] >= from_l && l[e] < to_l) {
+                    const float q = where(l[e]);
+                    const int i = (int)q;
+                    atomicAdd(&sh.hist[i].x, 1u);
+                    if (weighed) atomicAdd(&sh.hist[i].y, (uint32_t)(exp2f((q - (float)i) * bin_y) * rel_unit));
+                }
         });
     };
     if (list) {
@@ -692,7 +707,7 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
                     if (l >= l_a) own_a += w;
                     if (l >= l_c) own_c += w;
                 });
-                if (marked) R.mark(marks, v, i, [&](float l) { return l >= l_c; });
+                if (marked) R.mark(marks, v, i, l_c);
             }
         });
         if (list_p) {
@@ -744,31 +759,40 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
 #pragma unroll
             for (int g = 0; g < N / 4; ++g) marks[g] = 0;
             R.scan([&](const float (&v)[N], float largest, int, int i) {
-                if (largest >= from_l) R.mark(marks, v, i, [&](float l) { return l >= from_l; });
+                if (largest >= from_l) R.mark(marks, v, i, from_l);
             });
         }
         count();
         dc_sync(S);
         uint32_t cnt[kDcBinsPer] = {};
+        u64 rel[kDcBinsPer] = {};
 #pragma unroll
         for (int c = 0; c < kDcMaxCtas; ++c)
             if (c < S) {
-                const uint2 h = dc_u32x2(&sh.hist[kDcBinsPer * tid], c);
-                cnt[0] += h.x, cnt[1] += h.y;
+                const uint4 h = dc_u32x4(&sh.hist[kDcBinsPer * tid], c);
+                cnt[0] += h.x, cnt[1] += h.z;
+                rel[0] += h.y, rel[1] += h.w;
             }
         // The logits of bins b1 .. b2 to list number c, and the weights of the warps' stretches before them to segs, all in the first CTA.
         const auto region = [&](int c, int b1, int b2) {
             const float q1 = (float)b1, q2 = (float)(b2 + 1);
             double own = 0;
             int above = 0;
-            R.each(marks, [&](float l, int place) {
-                const float q = where(l);
-                if (l >= from_l && l < to_l && q < q2) {
-                    if (q < q1)
-                        own += dw_whole(r, l, sh.tab), ++above;
-                    else
-                        R.collect(l, place);
+            R.each(marks, [&](const float (&l)[4], const int (&at)[4]) {
+                double w[4];
+                bool a[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] = l[e] >= from_l && l[e] < to_l && where(l[e]) < q1;
+                if (__any_sync(0xffffffffu, a[0] || a[1] || a[2] || a[3])) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = dw_whole(r, l[e], sh.tab);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (a[e]) own += w[e], ++above;
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!a[e] && l[e] >= from_l && l[e] < to_l && where(l[e]) < q2) R.collect(l[e], at[e]);
             });
             const u64 sum = dc_warp_sum((u64)own) + (base ? base[warp] : 0ull);
             above = __reduce_add_sync(0xffffffffu, above);
@@ -794,7 +818,7 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
             for (int i = 0; i < kDcBinsPer; ++i) {
                 if (at < want && at + (u64)v[i] >= want) {
                     sh.bin = kDcBinsPer * tid + i;
-                    sh.bins = max(1, min(64, 90 * 64 / (near_by + 64)));  // neighbours that make about two hundred logits
+                    sh.bins = max(1, min(16, 70 * 64 / (near_by + 64)));  // neighbours that make up to 150 logits
                 }
                 at += (u64)v[i];
             }
@@ -852,14 +876,14 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
             P = dw_share(r.top_p, total);
         }
         {
-            // top-p's cut: the bin that the middles of the bins say, and some on each side
+            // top-p's cut: the bin that the bins' weights say, and some on each side
             const double unit = exp2(24.0 - (double)r.F);
-            const float step = -(float)r.c / per_bin, first = -(float)((r.mxd - (double)top_l) * r.c);
+            const float first = -(float)((r.mxd - (double)top_l) * r.c), scale = 16777216.0f / rel_unit, mid = rel_unit * exp2f(0.5f * bin_y);
             float near[kDcBinsPer];
             u64 sum = 0, all;
 #pragma unroll
             for (int i = 0; i < kDcBinsPer; ++i) {
-                near[i] = rintf((float)cnt[i] * exp2f(first + ((float)(kDcBinsPer * tid + i) + 0.5f) * step) * 16777216.0f);
+                near[i] = rintf((weighed ? (float)rel[i] : (float)cnt[i] * mid) * exp2f(first + (float)(kDcBinsPer * tid + i) * bin_y) * scale);
                 sum += (u64)near[i];
             }
             const u64 before = dc_before(sum, sh.wsum, all), want = (u64)((double)(P - base_all) * unit);
