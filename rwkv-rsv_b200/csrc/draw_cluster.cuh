@@ -60,7 +60,7 @@ struct DcShared {
     u64 wsum[kDwWarps], seg_a[kDwWarps], seg_c[kDwWarps], before, target, sum;
     float red[kDwWarps], redmin[kDwWarps], thr_all, thr_part, floor_l, min_l;
     uint32_t first;
-    int n_mine, n_above[kDwWarps], bin, bins, found;
+    int n_mine, n_above[kDwWarps], bin, bin_to, found;
 };
 
 __device__ __forceinline__ uint32_t dc_rank() {
@@ -204,13 +204,14 @@ __device__ __noinline__ void dc_sort(u64* keys, int n) {
     for (int e = 0; e < kDcPer; ++e) mine[e] = tid + e * kDwThreads < n ? keys[tid + e * kDwThreads] : ~0ull, place[e] = 0;
     if (tid == 0 && n < kDcList) keys[n] = 0;  // (pairs are read)
     __syncthreads();
-    if (tid < n)
-#pragma unroll 4
-        for (int j = 0; j < n; j += 2) {
-            const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&keys[j]);
 #pragma unroll
-            for (int e = 0; e < kDcPer; ++e) place[e] += (k.x > mine[e]) + (k.y > mine[e]);
-        }
+    for (int e = 0; e < kDcPer; ++e)
+        if (tid + e * kDwThreads < n)
+#pragma unroll 4
+            for (int j = 0; j < n; j += 2) {
+                const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&keys[j]);
+                place[e] += (k.x > mine[e]) + (k.y > mine[e]);
+            }
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < kDcPer; ++e)
@@ -809,21 +810,20 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
             }
             dc_sync(S);
         };
-        const auto find_bin = [&](u64 before, const auto (&v)[kDcBinsPer], u64 want) {  // the bin where the running sum reaches `want`
-            if (tid == 0) sh.bin = kDcBins - 1, sh.bins = 1;
+        // The bins where the running sum reaches `want` and `to`: sh.bin and sh.bin_to.
+        const auto find_bins = [&](u64 before, const auto (&v)[kDcBinsPer], u64 want, u64 to) {
+            if (tid == 0) sh.bin = sh.bin_to = kDcBins - 1;
             __syncthreads();
             u64 at = before;
-            const int near_by = (int)__reduce_add_sync(0xffffffffu, cnt[0] + cnt[1]);  // logits of the warp's 64 bins
+            if (tid == 0 && before >= want) sh.bin = 0;
 #pragma unroll
             for (int i = 0; i < kDcBinsPer; ++i) {
-                if (at < want && at + (u64)v[i] >= want) {
-                    sh.bin = kDcBinsPer * tid + i;
-                    sh.bins = max(1, min(16, 70 * 64 / (near_by + 64)));  // neighbours that make up to 150 logits
-                }
-                at += (u64)v[i];
+                const u64 next = at + (u64)v[i];
+                if (at < want && next >= want) sh.bin = kDcBinsPer * tid + i;
+                if (at < to && next >= to) sh.bin_to = kDcBinsPer * tid + i;
+                at = next;
             }
             __syncthreads();
-            return sh.bin;
         };
         u64 P = 0;
         if (binned_k) {
@@ -837,7 +837,11 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
                 dc_sync(S);  // (the histograms are being read)
                 return left_to_passes();
             }
-            const int b = cut_k ? find_bin(before, cnt, r.top_k) : kDcBins;
+            int b = kDcBins;
+            if (cut_k) {
+                find_bins(before, cnt, r.top_k, r.top_k);
+                b = sh.bin;
+            }
             if (!(r.top_p > 0.f) && where(R.min_l) < (float)b) goto by_min_p;  // min-p's cut is the stricter one
             region(1, b, b);
             u64 key[kDcPer], w[kDcPer];
@@ -876,7 +880,7 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
             P = dw_share(r.top_p, total);
         }
         {
-            // top-p's cut: the bin that the bins' weights say, and some on each side
+            // top-p's cut: between the bins that the bins' weights say
             const double unit = exp2(24.0 - (double)r.F);
             const float first = -(float)((r.mxd - (double)top_l) * r.c), scale = 16777216.0f / rel_unit, mid = rel_unit * exp2f(0.5f * bin_y);
             float near[kDcBinsPer];
@@ -887,10 +891,13 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
                 sum += (u64)near[i];
             }
             const u64 before = dc_before(sum, sh.wsum, all), want = (u64)((double)(P - base_all) * unit);
-            const int b = find_bin(before, near, want > 0 ? want : 1), wide = sh.bins, b1 = max(b - wide, 0);
+            // Weighed bins are 2^-17 of them off at most; in the others the weights of 128 tokens and more average, but the cut may lie among a few that come first.
+            const u64 off = weighed ? want >> 15 : (want >> 12) + (u64)(exp2f(first) * (0.01f * 16777216.0f));
+            find_bins(before, near, want > off ? want - off : 1, want + off);
+            const int b1 = sh.bin, b2 = sh.bin_to;
             limit = P;
             if (where(R.min_l) < (float)b1 || R.min_l >= to_l) goto by_min_p;
-            region(2, b1, b + wide);
+            region(2, b1, b2);
             if (rank != 0) return;
             const int n = sh.n_list[2];
             u64 above = 0;
