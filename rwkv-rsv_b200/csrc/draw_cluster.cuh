@@ -9,7 +9,11 @@
 //   region  Otherwise the cut lies in a stretch of values known from the pass that summed the weights (three stretches, divided by bounds from the threads'
 //           maxima).  A histogram of that stretch in 512 linear bins says near which bin the cut is; the logits of that bin and its neighbours are
 //           collected and sorted, the weight of all larger ones is summed exactly, and the sums tell whether the cut is there.
-//   neither Where a collection would not fit 384 entries (many equal logits) one CTA does the row by radix passes (dw_row_plain).
+//   zoom    Bins with more than 384 logits (a flat row, a large vocabulary, 16-bit logits) are divided into 512 bins again, up to four times; of equal logits
+//           as many are kept as the weight left, or the number, needs.  74 rows of 131072 logits with a deviation of 0.3 and top-p 0.9: 0.16 ms, where one
+//           CTA a row took 2.1 ms; 65536 logits of bf16 rounded to few values: under 0.15 ms and 1.1 ms.
+//   neither Where that misses (the weight of a bin is estimated from its middle), or more than top-k are equal, one CTA does the row by radix passes
+//           (dw_row_plain).
 // Without top-k and top-p no cut is needed: min-p's is a value that follows from the maximum.
 //
 // The draw: sums of the kept weights per warp, whose logits follow each other in the vocabulary, then the one warp's stretch again, split over a CTA.
@@ -32,6 +36,7 @@ constexpr int kDcMostPart = kDwThreads * 7 / 8;  // most of a CTA's thread maxim
 constexpr int kDcTryK = 128;                     // entries tried for top-p alone,
 constexpr int kDcTryPart = kDwThreads * 3 / 8;   // and of one CTA's thread maxima
 constexpr int kDcMaxCtas = 8;
+constexpr int kDcZooms = 4;   // times that bins are divided again
 constexpr int kDcMarked = 8;  // vectors a thread can mark the logits of
 static_assert(kDcMaxCtas * kDwWarps == 64 && kDwWarps == 8, "two stretches a lane; warps add up among eight lanes");
 constexpr int kDcSliceBytes = 32 * 1024;  // a CTA's part of a row, as long as eight CTAs suffice
@@ -40,12 +45,18 @@ constexpr int kDcMostSliceBytes = 192 * 1024;
 struct DcSums {
     u64 total, n, from_a, from_c;  // weight of the slice, entries collected, weights from the two bounds on
 };
+struct DcZoom {  // what a cut in bins with too many logits goes on from
+    float mx, mn, from_l, to_l;
+    const u64* base;
+    u64 base_all, total;
+};
 struct DcShared {
     // written by the other CTAs
     float4 top[kDcMaxCtas];  // largest logit (NaN: there is one), smallest of the threads' maxima, two lower bounds
     DcSums sums[kDcMaxCtas];
     u64 segs[kDcMaxCtas * kDwWarps];  // weights of the warps' stretches
     int above[kDcMaxCtas];            // logits above a region
+    int ties[kDcMaxCtas * kDwWarps];  // and in it, of the warps' stretches
     u64 left, cut_p;                  // what top-k leaves; 0: the row is done
     int n_list[3];                    // entries of the collections below (one after the other)
     alignas(16) u64 list[kDcList];    // key << 32 | ~index
@@ -60,7 +71,8 @@ struct DcShared {
     u64 wsum[kDwWarps], seg_a[kDwWarps], seg_c[kDwWarps], before, target, sum;
     float red[kDwWarps], redmin[kDwWarps], thr_all, thr_part, floor_l, min_l;
     uint32_t first;
-    int n_mine, n_above[kDwWarps], bin, bin_to, found;
+    int n_mine, n_above[kDwWarps], bin, bin_to, n_in, found;
+    DcZoom zoom;
 };
 
 __device__ __forceinline__ uint32_t dc_rank() {
@@ -232,6 +244,13 @@ __device__ __forceinline__ float dc_threshold(const DwRow& r, double ymin) {
     return half ? __shfl_sync(0xffffffffu, v, (threadIdx.x & 16) + __ffs(half) - 1) : t;
 }
 
+// How a row is finished: not by this CTA, by min-p's cut, by the cut in `cut`, by radix passes.
+enum DcEnd { kDcDone, kDcByMinP, kDcByCut, kDcByPasses };
+struct DcCut {
+    u64 cut, limit;  // key << 32 | ~index of the last kept; by min-p: with more weight than the limit top-p's cut is further up after all
+    int kept;        // listed entries that are kept
+};
+
 template <typename T>
 struct DcRow {
     const DrawArgs& A;
@@ -341,7 +360,7 @@ struct DcRow {
     // Row to shared memory; this thread's largest logit (NaN where there is one).  `meanwhile` runs while the first loads are on their way.
     template <class F>
     __device__ __forceinline__ float load(F&& meanwhile) {
-        constexpr int B = 8;
+        constexpr int B = 6;  // (8 need more registers than there are, and spill: 4.8 instead of 4.5 us for the largest logit of 65536)
         const T* lg = reinterpret_cast<const T*>(A.logits) + (size_t)row * A.ld;
         off = (int)((reinterpret_cast<uintptr_t>(lg) & 15) / sizeof(T));  // places count from the 16 bytes that the row starts in
         const bool whole = rank * n_slice >= off && (rank + 1) * n_slice - off <= A.V;
@@ -499,10 +518,56 @@ struct DcRow {
         }
     }
 
+    // (On the first CTA.)  The first m of the logits that are v, of which the warps' stretches have sh.ties: their weights to sh.segs, and the last one's key.
+    __device__ __forceinline__ u64 cut_of_ties(float v, u64 m, u64 w) {
+        if (warp == 0) {
+            const int n = S * kDwWarps;
+            const int n0 = 2 * lane < n ? sh.ties[2 * lane] : 0, n1 = 2 * lane + 1 < n ? sh.ties[2 * lane + 1] : 0;
+            int upto = n0 + n1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += t;
+            }
+            const int from = upto - n0 - n1, k0 = min(n0, max(0, (int)m - from)), k1 = min(n1, max(0, (int)m - from - n0));
+            if (k0) sh.segs[2 * lane] += (u64)k0 * w;
+            if (k1) sh.segs[2 * lane + 1] += (u64)k1 * w;
+            if (from < (int)m && upto >= (int)m) {
+                sh.found = 2 * lane + (k1 > 0);
+                sh.n_in = k1 > 0 ? k1 : k0;
+            }
+        }
+        __syncthreads();
+        const int f = sh.found, need = sh.n_in, c = f / kDwWarps;
+        const T* lg = reinterpret_cast<const T*>(A.logits) + (size_t)row * A.ld;
+        const int lo = f % kDwWarps * seg + (int)((unsigned)seg * (unsigned)tid / (unsigned)kDwThreads),
+                  hi = f % kDwWarps * seg + (int)((unsigned)seg * (unsigned)(tid + 1) / (unsigned)kDwThreads);
+        u64 own = 0, all;
+        uint32_t index = 0;
+#pragma unroll 1
+        for (int turn = 0; turn < 2; ++turn) {
+            int at_most = turn ? need - (int)own : 0x7FFFFFFF;
+            u64 seen = 0;
+#pragma unroll 1
+            for (int i = lo; i < hi && (int)seen < at_most; ++i) {
+                const int at = c * n_slice + i - off;
+                if (at >= 0 && at < A.V && dw_f32(lg[at]) == v) ++seen, index = (uint32_t)at;
+            }
+            if (!turn) {
+                own = dc_before(seen, sh.wsum, all);
+                if (!((int)own < need && (int)(own + seen) >= need)) break;
+            } else {
+                sh.first = index;
+            }
+        }
+        __syncthreads();
+        return (u64)dw_key(v) << 32 | (uint32_t)~sh.first;
+    }
+
     // The draw among all logits down to `cut` (key << 32 | ~index) and min_l, from the weights of the warps' stretches in sh.segs, to which those of the first
-    // `kept` listed entries are added.  `alone`: one CTA for the row, with that stretch from global memory; otherwise the CTA that has it.  Sums over `limit`:
-    // left to radix passes.
-    __device__ __forceinline__ void draw_segments(u64 cut, int kept, bool alone, u64 limit) {
+    // `kept` listed entries are added.  `alone`: one CTA for the row, with that stretch from global memory; otherwise the CTA that has it.  False: they are over
+    // `limit`.
+    __device__ __forceinline__ bool draw_segments(u64 cut, int kept, bool alone, u64 limit) {
         const int n = S * kDwWarps;
 #pragma unroll 1
         for (int i = tid; i < kept; i += kDwThreads) {
@@ -533,13 +598,10 @@ struct DcRow {
         }
         __syncthreads();
         const u64 total = sh.sum;
-        if (total > limit) {
-            if (rank == 0) dw_row_plain<T>(A, row, *reinterpret_cast<DwPlainShared*>(slice));
-            return;
-        }
+        if (total > limit) return false;
         const u64 U = sh.target;
         const int f = sh.found, c = f / kDwWarps;
-        if (c != rank && !alone) return;
+        if (c != rank && !alone) return true;
         // that stretch again: consecutive logits per thread
         const T* lg = reinterpret_cast<const T*>(A.logits) + (size_t)row * A.ld;
         const int lo = f % kDwWarps * seg + (int)((unsigned)seg * (unsigned)tid / (unsigned)kDwThreads),
@@ -563,16 +625,382 @@ struct DcRow {
                     }
                 }
             }
-            if (turn) return;
+            if (turn) return true;
             u64 all;
             b = sh.before + dc_before(sum, sh.wsum, all);
-            if (!(sum && b <= U && b + sum > U)) return;
+            if (!(sum && b <= U && b + sum > U)) return true;
         }
+        return true;
+    }
+
+    __device__ __forceinline__ void finish(DcEnd end, DcCut c) {
+        if (end == kDcByMinP) {
+            double own = 0;
+            scan([&](const float (&v)[N], float largest, int, int) {
+                weights(v, largest, min_l, [&](float l, double w) {
+                    if (l >= min_l) own += w;
+                });
+            });
+            const u64 sum = dc_warp_sum((u64)own);
+            if (lane < S) dc_put(lane, &sh.segs[rank * kDwWarps + warp], sum);
+            dc_sync(S);
+            c.cut = 0, c.kept = 0;
+        }
+        if (end == kDcByMinP || end == kDcByCut)
+            if (!draw_segments(c.cut, c.kept, end == kDcByCut, c.limit)) end = kDcByPasses;
+        if (end == kDcByPasses && rank == 0) dw_row_plain<T>(A, row, *reinterpret_cast<DwPlainShared*>(slice));
     }
 };
 
+// A stretch of values that a cut lies in, and its histogram.
 template <typename T>
-__global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A, int S, int n_slice) {
+struct DcStretch {
+    DcRow<T>& R;
+    static constexpr int N = DcVec<T>::n;
+    static constexpr float kTolerance = sizeof(T) == 2 ? 1.0f / 512.0f : 1.0f / 2048.0f;
+    float mn;               // the smallest of the threads' largest logits
+    bool marked, weighed;   // marked: the slice is short enough for marks; weighed: the bins are, otherwise a bin's weight is taken in its middle, which is good
+                            // enough without the largest logits
+    float rel_unit;         // (8192 or, of 16 bits, 16384 logits of a marked slice stay under 2^32, and up to 98304 of a long one)
+    float from_l, to_l;     // the cut lies from here on, under this
+    const u64* base;        // weights of the warps' stretches from to_l on (null: none),
+    u64 base_all, base_n;   // of all, and their number (for top-k's cut)
+    uint32_t marks[N / 4];  // logits from from_l on
+    float top_l, per_bin, bin_y;  // (bin_y: what y changes by from bin to bin)
+    uint32_t cnt[kDcBinsPer];
+    u64 rel[kDcBinsPer];
+
+    __device__ __forceinline__ void begin(float smallest) {
+        mn = smallest;
+        marked = R.seg <= 32 * N * kDcMarked;
+        weighed = R.r.top_k && R.r.top_p > 0.f;
+        rel_unit = marked ? 131072.0f : 16384.0f;
+    }
+    __device__ __forceinline__ void whole(float from) { from_l = from, to_l = INFINITY, base = nullptr, base_all = base_n = 0; }
+    __device__ __forceinline__ void mark() {
+        if (!marked) return;
+#pragma unroll
+        for (int g = 0; g < N / 4; ++g) marks[g] = 0;
+        R.scan([&](const float (&v)[N], float largest, int, int i) {
+            if (largest >= from_l) R.mark(marks, v, i, from_l);
+        });
+    }
+    __device__ __forceinline__ void set_bins() {
+        top_l = fminf(to_l, R.r.mx);
+        const float span = fminf(top_l - from_l, 2.5f * (R.r.mx - mn));
+        per_bin = span > 0.f ? fminf(((float)kDcBins - 1.0f) / span, 1e30f) : 1e30f;
+        bin_y = -(float)R.r.c / per_bin;
+    }
+    // The bin of a logit from from_l on and under to_l; in the last one: all that is further down.
+    __device__ __forceinline__ float where(float l) const { return fminf((top_l - l) * per_bin, (float)kDcBins - 0.5f); }
+    __device__ __forceinline__ bool in(float l) const { return l >= from_l && l < to_l; }
+    // All CTAs' histograms, two bins a thread.
+    __device__ __forceinline__ void count() {
+        R.each(marks, [&](const float (&l)[4], const int (&)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (in(l[e])) {
+                    const float q = where(l[e]);
+                    const int i = (int)q;
+                    atomicAdd(&R.sh.hist[i].x, 1u);
+                    if (weighed) atomicAdd(&R.sh.hist[i].y, (uint32_t)(exp2f((q - (float)i) * bin_y) * rel_unit));
+                }
+        });
+        dc_sync(R.S);
+#pragma unroll
+        for (int i = 0; i < kDcBinsPer; ++i) cnt[i] = 0, rel[i] = 0;
+#pragma unroll
+        for (int c = 0; c < kDcMaxCtas; ++c)
+            if (c < R.S) {
+                const uint4 h = dc_u32x4(&R.sh.hist[kDcBinsPer * R.tid], c);
+                cnt[0] += h.x, cnt[1] += h.z;
+                rel[0] += h.y, rel[1] += h.w;
+            }
+    }
+    // The bins where the running sum reaches `want` and `to`, b1 and b2, and the number of logits from the one to the other.
+    template <typename V>
+    __device__ __forceinline__ int find_bins(u64 before, const V (&v)[kDcBinsPer], u64 want, u64 to, int& b1, int& b2) {
+        DcShared& sh = R.sh;
+        if (R.tid == 0) sh.bin = sh.bin_to = kDcBins - 1, sh.n_in = 0;
+        __syncthreads();
+        u64 at = before;
+        if (R.tid == 0 && before >= want) sh.bin = 0;
+#pragma unroll
+        for (int i = 0; i < kDcBinsPer; ++i) {
+            const u64 next = at + (u64)v[i];
+            if (at < want && next >= want) sh.bin = kDcBinsPer * R.tid + i;
+            if (at < to && next >= to) sh.bin_to = kDcBinsPer * R.tid + i;
+            at = next;
+        }
+        __syncthreads();
+        b1 = sh.bin, b2 = sh.bin_to;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kDcBinsPer; ++i)
+            if (kDcBinsPer * R.tid + i >= b1 && kDcBinsPer * R.tid + i <= b2) n += (int)cnt[i];
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (R.lane == 0 && n) atomicAdd(&sh.n_in, n);
+        __syncthreads();
+        return sh.n_in;
+    }
+    // Top-k's cut: whether there is one here, and its bin (kDcBins: none).
+    __device__ __forceinline__ bool find_k(int& b1, int& n_in) {
+        u64 sum = 0, all;
+#pragma unroll
+        for (int i = 0; i < kDcBinsPer; ++i) sum += cnt[i];
+        const u64 before = base_n + dc_before(sum, R.sh.wsum, all);
+        b1 = kDcBins, n_in = 0;
+        if (base_n + all < (u64)R.r.top_k) return false;
+        int b2;
+        n_in = find_bins(before, cnt, R.r.top_k, R.r.top_k, b1, b2);
+        return true;
+    }
+    // Top-p's cut: between the bins that the bins' weights say, in units of 2^-24 of the largest one here.
+    __device__ __forceinline__ int find_p(u64 P, float tolerance, int& b1, int& b2) {
+        const DwRow& r = R.r;
+        const double unit = exp2(24.0 - (double)r.F + (r.mxd - (double)top_l) * r.c);
+        const float scale = 16777216.0f / rel_unit, mid = rel_unit * exp2f(0.5f * bin_y);
+        float near[kDcBinsPer];
+        u64 sum = 0, all;
+#pragma unroll
+        for (int i = 0; i < kDcBinsPer; ++i) {
+            near[i] = rintf((weighed ? (float)rel[i] : (float)cnt[i] * mid) * exp2f((float)(kDcBinsPer * R.tid + i) * bin_y) * scale);
+            sum += (u64)near[i];
+        }
+        const u64 before = dc_before(sum, R.sh.wsum, all), want = P > base_all ? (u64)fmin((double)(P - base_all) * unit, 1e18) : 0ull;
+        // Weighed bins are 2^-17 of them off at most; in the others the weights of many tokens average, but the cut may lie among a few that come first.
+        const u64 off = weighed ? want >> 15 : (u64)((float)want * tolerance) + (16777216u / 100u);
+        return find_bins(before, near, want > off ? want - off : 1, want + off, b1, b2);
+    }
+    // min-p's cut comes before bin b.
+    __device__ __forceinline__ bool min_p_before(int b) const { return where(R.min_l) < (float)b || R.min_l >= to_l; }
+
+    // The weights of the warps' stretches in front of bins b1 .. b2 to segs, their number to above, and the logits of the bins to list number c, all in the first
+    // CTA; or (ZOOM) what they weigh and how many they are together, and the largest and the smallest in the bins, to all CTAs.
+    template <bool ZOOM>
+    __device__ __forceinline__ void region(int c, int b1, int b2) {
+        DcShared& sh = R.sh;
+        const int rank = R.rank, warp = R.warp, lane = R.lane;
+        const float q1 = (float)b1, q2 = (float)(b2 + 1);
+        double own = 0;
+        int above = 0, n = 0;
+        float hi = -INFINITY, lo = INFINITY;
+        R.each(marks, [&](const float (&l)[4], const int (&at)[4]) {
+            double w[4];
+            bool a[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = in(l[e]) && where(l[e]) < q1;
+            if (__any_sync(0xffffffffu, a[0] || a[1] || a[2] || a[3])) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = dw_whole(R.r, l[e], sh.tab);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (a[e]) own += w[e], ++above;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!a[e] && in(l[e]) && where(l[e]) < q2) {
+                    if (ZOOM)
+                        hi = fmaxf(hi, l[e]), lo = fminf(lo, l[e]), ++n;
+                    else
+                        R.collect(l[e], at[e]);
+                }
+        });
+        const u64 sum = dc_warp_sum((u64)own) + (base ? base[warp] : 0ull);
+        above = __reduce_add_sync(0xffffffffu, above);
+        if (lane == 0) {
+            dc_put(0, &sh.segs[rank * kDwWarps + warp], sum);
+            sh.n_above[warp] = above;
+        }
+        if (ZOOM) {
+            n = __reduce_add_sync(0xffffffffu, n);
+            hi = dc_warp_max(hi), lo = dc_warp_min(lo);
+            if (lane == 0) {
+                dc_put(0, &sh.ties[rank * kDwWarps + warp], n);
+                sh.seg_a[warp] = sum;
+                sh.red[warp] = hi, sh.redmin[warp] = lo;
+            }
+            __syncthreads();
+            if (warp == 0) {
+                const u64 t = dc_all(sh.seg_a[lane & 7], DcAdd());
+                const int all = dc_all(sh.n_above[lane & 7], DcAdd());
+                hi = dc_warp_max(sh.red[lane & 7]), lo = dc_warp_min(sh.redmin[lane & 7]);
+                if (lane < R.S) {
+                    dc_put(lane, &sh.sums[rank].total, t);
+                    dc_put(lane, &sh.sums[rank].n, (u64)all);
+                    dc_put(lane, &sh.top[rank], make_float4(hi, lo, 0.f, 0.f));
+                }
+            }
+        } else {
+            R.hand_in(c);
+            if (R.tid == 0) {
+                int t = 0;
+#pragma unroll
+                for (int i = 0; i < kDwWarps; ++i) t += sh.n_above[i];
+                dc_put(0, &sh.above[rank], t);
+            }
+        }
+        dc_sync(R.S);
+    }
+    // (All CTAs.)  Top-k's cut in bin b1 (!here: further down than all logits here), with top-p's where that comes later.  False: top-p's lies further up, before P.
+    __device__ __forceinline__ bool cut_at_k(int b1, bool here, u64& total, u64& P, DcEnd& end, DcCut& c) {
+        DcShared& sh = R.sh;
+        const DwRow& r = R.r;
+        region<false>(1, b1, b1);
+        end = kDcDone;
+        if (R.rank != 0) {
+            if (r.top_p <= 0.f) return true;
+            dc_sync(R.S);
+        } else {
+            u64 key[kDcPer], w[kDcPer], above = 0;
+            const int n = sh.n_list[1];
+            (void)dc_before(R.tid < R.S * kDwWarps ? sh.segs[R.tid] : 0ull, sh.wsum, above);
+            const int n_above = (int)base_n + dc_all((R.lane & 7) < R.S ? sh.above[R.lane & 7] : 0, DcAdd());
+            const bool fits = n <= kDcList;
+            if (fits) {
+                R.sorted(n, key);
+                c.kept = R.cut_of(key, n, here ? (int)r.top_k - n_above : 0, above, r.top_p, 0, w, P, total);
+                c.cut = c.kept ? sh.list[c.kept - 1] : 0ull;
+            }
+            end = fits ? kDcByCut : kDcByPasses;
+            if (r.top_p <= 0.f) return true;  // (the others have left)
+            // Where top-p's cut lies further up the others are told what it is a share of.
+            const bool done = !fits || above < P;
+            const bool by_min = fits && above < P && min_p_before(b1);  // top-p's cut is here, min-p's further up
+            if (R.tid < R.S) {
+                dc_put(R.tid, &sh.left, total);
+                dc_put(R.tid, &sh.cut_p, by_min ? ~0ull : done ? 0ull : P);
+            }
+            dc_sync(R.S);
+        }
+        total = sh.left;
+        P = sh.cut_p;
+        if (P == ~0ull) end = kDcByMinP;
+        return P == 0 || P == ~0ull;
+    }
+    // Top-p's cut in bins b1 .. b2.
+    __device__ __forceinline__ DcEnd cut_at_p(int b1, int b2, u64 total, u64 P, DcCut& c) {
+        DcShared& sh = R.sh;
+        region<false>(2, b1, b2);
+        if (R.rank != 0) return kDcDone;
+        const int n = sh.n_list[2];
+        u64 above = 0;
+        (void)dc_before(R.tid < R.S * kDwWarps ? sh.segs[R.tid] : 0ull, sh.wsum, above);
+        if (n > kDcList || above >= P) return kDcByPasses;
+        u64 key[kDcPer], w[kDcPer], P2, upto;
+        R.sorted(n, key);
+        c.kept = R.cut_of(key, n, n, above, R.r.top_p, total, w, P2, upto);
+        if (upto < P) return kDcByPasses;  // the cut lies further down
+        c.cut = sh.list[c.kept - 1];
+        return kDcByCut;
+    }
+};
+
+// A cut whose bins b1 .. b2 of the stretch from_l .. to_l hold n_in logits, too many to sort: they are divided into 512 bins again, and so on.  (All CTAs of the
+// row.  A function of its own, which begins with what is in shared memory, so that the rows without it have its registers.)
+template <typename T>
+__device__ __noinline__ void dc_zoomed(const DrawArgs& A, int S, int n_slice, bool by_k) {
+    extern __shared__ __align__(16) unsigned char dc_smem[];
+    DcShared& sh = *reinterpret_cast<DcShared*>(dc_smem);
+    DcRow<T> R = {A, sh, reinterpret_cast<T*>(dc_smem + sizeof(DcShared))};
+    R.tid = threadIdx.x, R.lane = R.tid & 31, R.warp = R.tid >> 5;
+    R.S = S;
+    R.rank = S > 1 ? (int)dc_rank() : 0;
+    R.row = (int)blockIdx.x / S;
+    R.n_slice = n_slice;
+    R.seg = n_slice / kDwWarps;
+    R.off = (int)((reinterpret_cast<uintptr_t>(reinterpret_cast<const T*>(A.logits) + (size_t)R.row * A.ld) & 15) / sizeof(T));
+    R.r = dw_asked(A, R.row);
+    DwRow& r = R.r;
+    __syncthreads();
+    r.mx = sh.zoom.mx, r.mxd = (double)r.mx, r.c = sh.rate, r.ymin = sh.least;
+    R.floor_l = sh.floor_l, R.min_l = sh.min_l;
+    DcStretch<T> D = {R};
+    D.begin(sh.zoom.mn);
+    const float from_all = sh.zoom.from_l;
+    D.whole(from_all);
+    D.to_l = sh.zoom.to_l, D.base = sh.zoom.base, D.base_all = sh.zoom.base_all;
+    D.mark();
+    D.set_bins();
+    u64 total = sh.zoom.total;
+    int b1 = sh.bin, b2 = sh.bin_to, n_in = sh.n_in;
+    __syncthreads();
+    u64 P = by_k ? 0ull : dw_share(r.top_p, total);
+    int zooms = 0;
+    bool here = true;
+    DcCut c = {0, ~0ull, 0};
+    DcEnd end = kDcByPasses;
+#pragma unroll 1
+    while (true) {
+        if (n_in > kDcList) {
+            if (zooms++ == kDcZooms) {
+                dc_sync(S);  // (the histograms are being read)
+                break;
+            }
+            D.template region<true>(0, b1, b2);
+            const bool one = (R.lane & 7) < S;
+            D.base = sh.seg_a;
+            D.base_all = dc_all(one ? sh.sums[R.lane & 7].total : 0ull, DcAdd());
+            D.base_n += dc_all(one ? sh.sums[R.lane & 7].n : 0ull, DcAdd());
+            const float hi = dc_warp_max(one ? sh.top[R.lane & 7].x : -INFINITY), lo = dc_warp_min(one ? sh.top[R.lane & 7].y : INFINITY);
+            D.from_l = lo, D.to_l = nextafterf(hi, INFINITY);
+            if (!(lo < hi)) {
+                // equal ones: as many of them as the weight or the number left needs
+                const u64 w = R.weight(lo);
+                u64 m = by_k ? (u64)r.top_k - D.base_n : (u64)n_in;
+                if (by_k && r.top_p > 0.f) total = D.base_all + m * w, P = dw_share(r.top_p, total);
+                if (r.top_p > 0.f && D.base_all >= P) {  // top-p's cut lies further up
+                    if (!by_k) break;
+                    by_k = false;
+                    D.whole(from_all);
+                } else {
+                    if (r.top_p > 0.f) {
+                        const u64 t = (P - D.base_all + w - 1) / w;
+                        if (t > (u64)n_in) break;
+                        if (t < m) m = t;
+                    }
+                    end = R.min_l > lo ? kDcByMinP : R.rank == 0 ? kDcByCut : kDcDone;
+                    if (end == kDcByCut) c.cut = R.cut_of_ties(lo, m, w);
+                    break;
+                }
+            }
+        } else if (by_k) {
+            if (D.cut_at_k(b1, here, total, P, end, c)) break;
+            by_k = false;
+            end = kDcByPasses, c.kept = 0;
+            D.whole(from_all);
+        } else {
+            end = D.cut_at_p(b1, b2, total, P, c);
+            break;
+        }
+        D.set_bins();
+        reinterpret_cast<uint4*>(sh.hist)[R.tid] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        D.count();
+        if (by_k) {
+            here = D.find_k(b1, n_in);
+            b2 = b1;
+            if (!here) {
+                dc_sync(S);
+                break;
+            }
+            if (!(r.top_p > 0.f) && D.min_p_before(b1)) {
+                end = kDcByMinP;
+                break;
+            }
+        } else {
+            n_in = D.find_p(P, D.base ? 1.0f / 4096.0f : D.kTolerance, b1, b2);
+            if (D.min_p_before(b1)) {
+                end = kDcByMinP, c.limit = P;
+                break;
+            }
+        }
+    }
+    R.finish(end, c);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(const __grid_constant__ DrawArgs A, int S, int n_slice) {
     extern __shared__ __align__(16) unsigned char dc_smem[];
     DcShared& sh = *reinterpret_cast<DcShared*>(dc_smem);
     DcRow<T> R = {A, sh, reinterpret_cast<T*>(dc_smem + sizeof(DcShared))};
@@ -593,7 +1021,7 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
         uint4* h = reinterpret_cast<uint4*>(sh.hist);
         for (int i = tid; i < kDcBins / 2; i += kDwThreads) h[i] = make_uint4(0, 0, 0, 0);
         sh.tmhist[tid] = 0u;
-        dw_fill_table(sh.tab, r.F);
+        dw_fill_table(sh.tab, A.F);
         if (tid == 0) {
             sh.n_list[0] = sh.n_list[1] = sh.n_list[2] = sh.n_mine = 0;
             sh.first = ~0u;
@@ -604,14 +1032,14 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
             if (lane == 0) sh.rate = c, sh.least = y;
         }
     });
+    float mx = dc_warp_max(tm), mn = dc_warp_min(tm > -INFINITY ? tm : INFINITY);
+    if (lane == 0) sh.red[warp] = mx, sh.redmin[warp] = mn;
+    __syncthreads();
     const bool small = A.V <= kDcList;
     const bool list_k = !r.greedy && !small && r.top_k && r.top_k <= (uint32_t)min(kDcFastK, S * kDcMostPart);
     const bool list_p = !r.greedy && !small && !r.top_k && r.top_p > 0.f;
     const bool list = !r.greedy && (small || list_k || list_p);
     const bool binned_k = !r.greedy && !list && r.top_k;
-    float mx = dc_warp_max(tm), mn = dc_warp_min(tm > -INFINITY ? tm : INFINITY);
-    if (lane == 0) sh.red[warp] = mx, sh.redmin[warp] = mn;
-    __syncthreads();
     mx = dc_warp_max(sh.red[lane & (kDwWarps - 1)]);
     mn = dc_warp_min(sh.redmin[lane & (kDwWarps - 1)]);
     if (list_k || list_p || binned_k) R.bounds(tm, mx, mn, list_p ? min(kDcTryK, S * kDcTryPart) : (int)r.top_k);
@@ -645,10 +1073,7 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
         if (tid == 0) dw_result(A, R.row, R.index_of((int)sh.first), 0.f);
         return;
     }
-    const auto left_to_passes = [&] {
-        if (rank == 0) dw_row_plain<T>(A, R.row, *reinterpret_cast<DwPlainShared*>(R.slice));
-    };
-    if (mx == INFINITY) return left_to_passes();
+    if (mx == INFINITY) return R.finish(kDcByPasses, {});
     r.mx = mx;
     r.mxd = (double)mx;
     r.c = sh.rate;
@@ -661,38 +1086,14 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
     R.floor_l = sh.floor_l;
     R.min_l = sh.min_l;
 
-    u64 limit = ~0ull;  // (more weight than this in min-p's hands: top-p's cut is further up after all)
     // ---- list
     bool binned_p = false, done_marks = false;
-    u64 total = 0;                        // weight of all that top-k leaves
-    float from_l = thr, to_l = INFINITY;  // the cut lies from here on, under this
-    const u64* base = nullptr;            // weights of the warps' stretches from to_l on (null: none),
-    u64 base_all = 0;                     // and of all
-    uint32_t marks[N / 4] = {};           // logits from from_l on
-    const bool marked = R.seg <= 32 * N * kDcMarked;
-    // The bin of a logit from from_l on and under to_l; in the last one: all that is further down.
-    float top_l = 0.f, per_bin = 0.f, bin_y = 0.f;  // (bin_y: what y changes by from bin to bin)
-    const bool weighed = binned_k && r.top_p > 0.f;  // bins are weighed; otherwise a bin's weight is taken in its middle, which is good enough without the largest logits
-    const float rel_unit = marked ? 131072.0f : 16384.0f;  // (8192 or, of 16 bits, 16384 logits of a marked slice stay under 2^32, and up to 98304 of a long one)
-    const auto set_bins = [&] {
-        top_l = fminf(to_l, mx);
-        const float span = fminf(top_l - from_l, 2.5f * (mx - mn));
-        per_bin = span > 0.f ? fminf(((float)kDcBins - 1.0f) / span, 1e30f) : 1e30f;
-        bin_y = -(float)r.c / per_bin;
-    };
-    const auto where = [&](float l) { return fminf((top_l - l) * per_bin, (float)kDcBins - 0.5f); };
-    const auto count = [&] {
-        R.each(marks, [&](const float (&l)[4], const int (&)[4]) {
+    u64 total = 0;  // weight of all that top-k leaves
+    DcStretch<T> D = {R};
+    D.begin(mn);
+    D.whole(thr);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (l[e] >= from_l && l[e] < to_l) {
-                    const float q = where(l[e]);
-                    const int i = (int)q;
-                    atomicAdd(&sh.hist[i].x, 1u);
-                    if (weighed) atomicAdd(&sh.hist[i].y, (uint32_t)(exp2f((q - (float)i) * bin_y) * rel_unit));
-                }
-        });
-    };
+    for (int g = 0; g < N / 4; ++g) D.marks[g] = 0;
     if (list) {
         // the smallest of the threads' maxima bounds the other stretches of values: a fifth of normally distributed logits is larger
         const float l_a = fmaxf(thr, R.floor_l), l_c = fmaxf(fminf(mn, thr), R.floor_l);
@@ -708,7 +1109,7 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
                     if (l >= l_a) own_a += w;
                     if (l >= l_c) own_c += w;
                 });
-                if (marked) R.mark(marks, v, i, l_c);
+                if (D.marked) R.mark(D.marks, v, i, l_c);
             }
         });
         if (list_p) {
@@ -733,16 +1134,16 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
             const bool over = dc_all(one ? o.n : 0ull, DcAdd()) > (u64)kDcList;
             binned_p = over || P > sum_a;
             done_marks = P <= sum_c;
-            from_l = l_c, to_l = l_a, base = sh.seg_a, base_all = sum_a;
-            if (P <= sum_a) to_l = INFINITY, base = nullptr, base_all = 0;
-            if (P > sum_c) from_l = R.floor_l, to_l = l_c, base = sh.seg_c, base_all = sum_c;
+            D.from_l = l_c, D.to_l = l_a, D.base = sh.seg_a, D.base_all = sum_a;
+            if (P <= sum_a) D.whole(l_c);
+            if (P > sum_c) D.from_l = R.floor_l, D.to_l = l_c, D.base = sh.seg_c, D.base_all = sum_c;
         }
         if (!binned_p) {
             if (rank != 0) return;
             const int n = sh.n_list[0];
             if (n > kDcList || n < (int)(list_k ? r.top_k : 0u)) {
                 // (fewer than top-k asks for: there are no more, or the bound was rounded up)
-                if (n > kDcList || thr > -3.402823466e38f) return left_to_passes();
+                if (n > kDcList || thr > -3.402823466e38f) return R.finish(kDcByPasses, {});
             }
             u64 key[kDcPer], w[kDcPer], P, sum;
             R.sorted(n, key);
@@ -751,178 +1152,48 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(DrawArgs A,
             return;
         }
     }
-    from_l = fmaxf(from_l, R.floor_l);
+    D.from_l = fmaxf(D.from_l, R.floor_l);
 
     // ---- region
+    DcCut c = {0, ~0ull, 0};
+    DcEnd end = kDcByMinP;
     if (binned_p || binned_k) {
-        set_bins();
-        if (marked && !done_marks) {
-#pragma unroll
-            for (int g = 0; g < N / 4; ++g) marks[g] = 0;
-            R.scan([&](const float (&v)[N], float largest, int, int i) {
-                if (largest >= from_l) R.mark(marks, v, i, from_l);
-            });
-        }
-        count();
-        dc_sync(S);
-        uint32_t cnt[kDcBinsPer] = {};
-        u64 rel[kDcBinsPer] = {};
-#pragma unroll
-        for (int c = 0; c < kDcMaxCtas; ++c)
-            if (c < S) {
-                const uint4 h = dc_u32x4(&sh.hist[kDcBinsPer * tid], c);
-                cnt[0] += h.x, cnt[1] += h.z;
-                rel[0] += h.y, rel[1] += h.w;
-            }
-        // The logits of bins b1 .. b2 to list number c, and the weights of the warps' stretches before them to segs, all in the first CTA.
-        const auto region = [&](int c, int b1, int b2) {
-            const float q1 = (float)b1, q2 = (float)(b2 + 1);
-            double own = 0;
-            int above = 0;
-            R.each(marks, [&](const float (&l)[4], const int (&at)[4]) {
-                double w[4];
-                bool a[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = l[e] >= from_l && l[e] < to_l && where(l[e]) < q1;
-                if (__any_sync(0xffffffffu, a[0] || a[1] || a[2] || a[3])) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = dw_whole(r, l[e], sh.tab);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (a[e]) own += w[e], ++above;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (!a[e] && l[e] >= from_l && l[e] < to_l && where(l[e]) < q2) R.collect(l[e], at[e]);
-            });
-            const u64 sum = dc_warp_sum((u64)own) + (base ? base[warp] : 0ull);
-            above = __reduce_add_sync(0xffffffffu, above);
-            if (lane == 0) {
-                dc_put(0, &sh.segs[rank * kDwWarps + warp], sum);
-                sh.n_above[warp] = above;
-            }
-            R.hand_in(c);
-            if (tid == 0) {
-                int t = 0;
-#pragma unroll
-                for (int i = 0; i < kDwWarps; ++i) t += sh.n_above[i];
-                dc_put(0, &sh.above[rank], t);
-            }
-            dc_sync(S);
-        };
-        // The bins where the running sum reaches `want` and `to`: sh.bin and sh.bin_to.
-        const auto find_bins = [&](u64 before, const auto (&v)[kDcBinsPer], u64 want, u64 to) {
-            if (tid == 0) sh.bin = sh.bin_to = kDcBins - 1;
-            __syncthreads();
-            u64 at = before;
-            if (tid == 0 && before >= want) sh.bin = 0;
-#pragma unroll
-            for (int i = 0; i < kDcBinsPer; ++i) {
-                const u64 next = at + (u64)v[i];
-                if (at < want && next >= want) sh.bin = kDcBinsPer * tid + i;
-                if (at < to && next >= to) sh.bin_to = kDcBinsPer * tid + i;
-                at = next;
-            }
-            __syncthreads();
-        };
+        D.set_bins();
+        if (!done_marks) D.mark();
+        D.count();
+        int b1, b2, n_in = 0;
         u64 P = 0;
+        bool at_p = !binned_k, zoom = false;
         if (binned_k) {
-            u64 sum = 0, all;
-#pragma unroll
-            for (int i = 0; i < kDcBinsPer; ++i) sum += cnt[i];
-            const u64 before = dc_before(sum, sh.wsum, all);
             // Where fewer logits have a weight (or the bound was rounded up) there is no cut of top-k among them.
-            const bool cut_k = all >= (u64)r.top_k;
-            if (!cut_k && thr >= R.floor_l) {
+            const bool here = D.find_k(b1, n_in);
+            if (!here && thr >= R.floor_l) {
                 dc_sync(S);  // (the histograms are being read)
-                return left_to_passes();
+                end = kDcByPasses;
+            } else if (r.top_p > 0.f || !D.min_p_before(b1)) {  // (otherwise min-p's cut is the stricter one)
+                zoom = n_in > kDcList;
+                if (!zoom) at_p = !D.cut_at_k(b1, here, total, P, end, c);
             }
-            int b = kDcBins;
-            if (cut_k) {
-                find_bins(before, cnt, r.top_k, r.top_k);
-                b = sh.bin;
-            }
-            if (!(r.top_p > 0.f) && where(R.min_l) < (float)b) goto by_min_p;  // min-p's cut is the stricter one
-            region(1, b, b);
-            u64 key[kDcPer], w[kDcPer];
-            int n = 0, kept = 0;
-            if (rank == 0) {
-                n = sh.n_list[1];
-                u64 above = 0;
-                (void)dc_before(tid < S * kDwWarps ? sh.segs[tid] : 0ull, sh.wsum, above);
-                const int n_above = dc_all((lane & 7) < S ? sh.above[lane & 7] : 0, DcAdd());
-                const bool fits = n <= kDcList;
-                if (fits) {
-                    R.sorted(n, key);
-                    kept = R.cut_of(key, n, cut_k ? (int)r.top_k - n_above : 0, above, r.top_p, 0, w, P, total);
-                }
-                // Where top-p's cut lies further up the others are told what it is a share of.
-                const bool done = !fits || r.top_p <= 0.f || above < P;
-                const bool by_min = fits && r.top_p > 0.f && above < P && where(R.min_l) < (float)b;  // top-p's cut is here, min-p's further up
-                if (r.top_p > 0.f) {  // (without top-p they have left)
-                    if (tid < S) {
-                        dc_put(tid, &sh.left, total);
-                        dc_put(tid, &sh.cut_p, by_min ? ~0ull : done ? 0ull : P);
-                    }
-                    dc_sync(S);
-                }
-                if (!fits) return left_to_passes();
-                if (done && !by_min) return R.draw_segments(kept ? sh.list[kept - 1] : 0ull, kept, true, ~0ull);
-            } else {
-                if (r.top_p <= 0.f) return;
-                dc_sync(S);
-            }
-            P = sh.cut_p;
-            total = sh.left;
-            if (P == 0) return;
-            if (P == ~0ull) goto by_min_p;
         } else {
             P = dw_share(r.top_p, total);
         }
-        {
-            // top-p's cut: between the bins that the bins' weights say
-            const double unit = exp2(24.0 - (double)r.F);
-            const float first = -(float)((r.mxd - (double)top_l) * r.c), scale = 16777216.0f / rel_unit, mid = rel_unit * exp2f(0.5f * bin_y);
-            float near[kDcBinsPer];
-            u64 sum = 0, all;
-#pragma unroll
-            for (int i = 0; i < kDcBinsPer; ++i) {
-                near[i] = rintf((weighed ? (float)rel[i] : (float)cnt[i] * mid) * exp2f(first + (float)(kDcBinsPer * tid + i) * bin_y) * scale);
-                sum += (u64)near[i];
+        if (at_p) {
+            n_in = D.find_p(P, D.kTolerance, b1, b2);
+            end = kDcByMinP;
+            if (D.min_p_before(b1)) {
+                c.limit = P;
+            } else {
+                zoom = n_in > kDcList;
+                if (!zoom) end = D.cut_at_p(b1, b2, total, P, c);
             }
-            const u64 before = dc_before(sum, sh.wsum, all), want = (u64)((double)(P - base_all) * unit);
-            // Weighed bins are 2^-17 of them off at most; in the others the weights of 128 tokens and more average, but the cut may lie among a few that come first.
-            const u64 off = weighed ? want >> 15 : (want >> 12) + (u64)(exp2f(first) * (0.01f * 16777216.0f));
-            find_bins(before, near, want > off ? want - off : 1, want + off);
-            const int b1 = sh.bin, b2 = sh.bin_to;
-            limit = P;
-            if (where(R.min_l) < (float)b1 || R.min_l >= to_l) goto by_min_p;
-            region(2, b1, b2);
-            if (rank != 0) return;
-            const int n = sh.n_list[2];
-            u64 above = 0;
-            (void)dc_before(tid < S * kDwWarps ? sh.segs[tid] : 0ull, sh.wsum, above);
-            if (n > kDcList || above >= P) return left_to_passes();
-            u64 key[kDcPer], w[kDcPer], P2, upto;
-            R.sorted(n, key);
-            const int kept = R.cut_of(key, n, n, above, r.top_p, total, w, P2, upto);
-            if (upto < P) return left_to_passes();  // the cut lies further down
-            return R.draw_segments(sh.list[kept - 1], kept, true, ~0ull);
         }
+        if (zoom) {
+            if (tid == 0) sh.zoom = {mx, D.mn, D.from_l, D.to_l, D.base, D.base_all, total};
+            return dc_zoomed<T>(A, S, n_slice, !at_p);
+        }
+        if (end == kDcDone) return;
     }
-by_min_p: {
-    // ---- min-p's cut, or none
-    double own = 0;
-    R.scan([&](const float (&v)[N], float largest, int, int) {
-        R.weights(v, largest, R.min_l, [&](float l, double w) {
-            if (l >= R.min_l) own += w;
-        });
-    });
-    const u64 sum = dc_warp_sum((u64)own);
-    if (lane < S) dc_put(lane, &sh.segs[rank * kDwWarps + warp], sum);
-    dc_sync(S);
-    R.draw_segments(0, 0, false, limit);
-}
+    R.finish(end, c);
 }
 
 }  // namespace rsv

@@ -87,6 +87,13 @@ def inputs(V, dtype, kind, seed, offset=0, stride=None, rows=None):
         l = g.integers(-3, 4, (R, V)) * 0.5
     elif kind == "wide":
         l = g.standard_normal((R, V)) * 30
+    elif kind == "flat":
+        l = g.standard_normal((R, V)) * 0.3
+    elif kind == "low":  # a few large logits in front of a flat rest
+        l = g.standard_normal((R, V)) * 0.5
+        l[np.arange(R)[:, None], g.integers(0, V, (R, 20))] += g.random((R, 20)) * 10
+    elif kind == "fine":  # steps of 1/1000, two next to each other with most of the logits
+        l = np.where(g.random((R, V)) < 0.8, 1.0 + 1e-3 * g.integers(0, 2, (R, V)), np.round(g.standard_normal((R, V)), 3))
     elif kind == "masked":
         l = np.where(g.random((R, V)) < 0.97, -np.inf, g.standard_normal((R, V)) * 3)
         l[:, g.integers(0, V)] = 1.0
@@ -118,6 +125,17 @@ def test_sixteen_bits(V, kind, dtype):
 def test_large_vocabularies(V):
     import torch
     l, par, u = inputs(V, torch.float32, "peaked", V, rows=[(1.0, 50, 0.9, 0.0), (1.0, 0, 0.9, 0.0), (0.8, 0, 1.0, 0.0), (1.0, 2000, 0.99, 0.01), (0.0, 0, 1.0, 0.0), (1.5, 0, 1.0, 0.05)])
+    check(l, par, u, *run(l, par, u))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("V,kind", [(8192, "flat"), (32000, "low"), (50003, "flat"), (65536, "low"), (65536, "fine"), (131072, "flat"), (131072, "low"), (300001, "flat"), (65536, "steps")])
+def test_cuts_among_many_close_logits(V, kind, dtype):
+    """Thousands of logits so near the cut, or equal to it, that no collection around it is small."""
+    import torch
+    rows = [(T, k, p, m) for T in (1.0, 0.7, 2.0) for k, p, m in ((0, 0.5, 0.0), (0, 0.9, 0.0), (0, 0.99, 0.0), (700, 1.0, 0.0), (1000, 0.9, 0.0), (3000, 0.95, 0.0), (0, 0.9, 0.3), (3000, 0.99, 0.7),
+                                                                      (3000, 1.0, 0.5), (4000, 1.0, 0.9))]
+    l, par, u = inputs(V, getattr(torch, dtype), kind, V + 3, rows=rows)
     check(l, par, u, *run(l, par, u))
 
 
