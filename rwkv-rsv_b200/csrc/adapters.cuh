@@ -47,7 +47,8 @@ constexpr int kAdChunk = 64;  // ranks whose sums a warp holds at a time
 
 constexpr size_t kAdSumBytes = (size_t)kAdWarps * 16 * (kAdChunk + 8) * 4;
 constexpr int kAdMostCells = 8192;  // rows x rank_cap of a tile: t lies where the sums were
-static_assert((kAdMaxSlots + 2) * 2 <= kAdSumBytes && kAdMostCells * 4 <= kAdSumBytes, "the counters lie where the sums go later, and t after them");
+constexpr int kAdGroupAt = kAdMaxSlots + 64;  // the groups of the rows behind the counters
+static_assert((kAdGroupAt + kAdBlockRows) * 2 <= kAdSumBytes && kAdMostCells * 4 <= kAdSumBytes, "the counters lie where the sums go later, and t after them");
 
 __device__ __forceinline__ float ad_f32(float v) { return v; }
 __device__ __forceinline__ float ad_f32(__half v) { return __half2float(v); }
@@ -227,21 +228,24 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
         __syncthreads();
         return true;
     }
-    constexpr int per_thread = kAdBlockRows / kAdThreads;
-    int group[per_thread];  // of rows tid, tid + 256, ...
-#pragma unroll
-    for (int i = 0; i < per_thread; ++i) {
-        group[i] = -1;
-        if (i * kAdThreads >= rows) continue;
-        const int row = i * kAdThreads + tid, a = row < rows ? ix[row] : -1;
-        group[i] = row < rows ? (a >= 0 && a < P.slots ? a : P.slots) : -1;
-    }
+    unsigned short* group = cnt + kAdGroupAt;  // of every row
     for (int i = tid; i < (groups + 1) / 2; i += kAdThreads) reinterpret_cast<uint32_t*>(cnt)[i] = 0;
     if (tid == 0) sh.slot = -1;
     __syncthreads();
+    // (Loops of a few rows rather than all sixteen of a thread unrolled: this runs once, and its instructions have to be fetched.)
+#pragma unroll 1
+    for (int o = tid; o < rows; o += 4 * kAdThreads) {
+        int a[4];
 #pragma unroll
-    for (int i = 0; i < per_thread; ++i)
-        if (i * kAdThreads < rows && group[i] >= 0) atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (group[i] >> 1), group[i] & 1 ? 65536u : 1u);  // (no counter passes 4096)
+        for (int e = 0; e < 4; ++e) a[e] = o + e * kAdThreads < rows ? ix[o + e * kAdThreads] : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (o + e * kAdThreads < rows) {
+                const int to = a[e] >= 0 && a[e] < P.slots ? a[e] : P.slots;
+                group[o + e * kAdThreads] = (unsigned short)to;
+                atomicAdd(reinterpret_cast<uint32_t*>(cnt) + (to >> 1), to & 1 ? 65536u : 1u);  // (no counter passes 4096)
+            }
+    }
     __syncthreads();
     const int per = (groups + kAdThreads - 1) / kAdThreads, g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     const auto tiles_of = [&](int g) { return g == P.slots && !P.copies ? 0 : ((int)cnt[g] + T - 1) / T; };
@@ -263,15 +267,14 @@ __device__ __forceinline__ bool ad_find_tile(const AdapterArgs& P, int first, in
     __syncthreads();
     const int mine = sh.slot;
     int n = 0;
-#pragma unroll
-    for (int i = 0; i < per_thread; ++i)
-        if (i * kAdThreads < rows) n += group[i] == mine;
+#pragma unroll 4
+    for (int o = tid; o < rows; o += kAdThreads) n += group[o] == mine;
     int place = ad_before(n, sh.wsum, all) - sh.skip;
     if (n && place < T && place + n > 0)
-#pragma unroll
-        for (int i = 0; i < per_thread; ++i)
-            if (i * kAdThreads < rows && group[i] == mine) {
-                if (place >= 0 && place < T) sh.rows[place] = first + i * kAdThreads + tid;
+#pragma unroll 4
+        for (int o = tid; o < rows; o += kAdThreads)
+            if (group[o] == mine) {
+                if (place >= 0 && place < T) sh.rows[place] = first + o;
                 ++place;
             }
     __syncthreads();
@@ -306,7 +309,7 @@ __device__ __forceinline__ void ad_wait() {
 // `count` stages: fill(i, slot) begins to load stage i, use(i, slot) works on it.
 template <int STAGES, class Fill, class Use>
 __device__ __forceinline__ void ad_pipeline(int count, Fill&& fill, Use&& use) {
-#pragma unroll
+#pragma unroll 1  // (the code that begins a stage has to be fetched: twice, not once per stage)
     for (int i = 0; i < STAGES - 1; ++i) {
         if (i < count) fill(i, i);
         ad_commit();
@@ -356,9 +359,6 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
 #pragma unroll 1
         for (int c0 = 0; c0 < r_all; c0 += kAdChunk) {
             const int ranks = min(kAdChunk, r_all - c0), nt = (ranks + 7) / 8;
-            float acc[kAdChunk / 8][4];
-#pragma unroll
-            for (int j = 0; j < kAdChunk / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
             __syncthreads();  // (the counters, or the sums before these, have been read)
             constexpr int XN = 16 / (int)sizeof(X), XU = KC / XN, XP = T * XU / kAdThreads;  // values of 16 bytes, those of a row, and those of a thread
             constexpr int WU = KC / 8, WP = kAdChunk * WU / kAdThreads;
@@ -389,59 +389,110 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                 for (int p = 0; p < WP; ++p)
                     if (wrow + p * (kAdThreads / WU) < 8 * nt) ad_fill16(ws + p * (kAdThreads / WU) * Z::ald, wsrc[p] + k, left - wu, P.wide_a, wa);
             };
-            ad_pipeline<Z::stages>(count, fill, [&](int, int slot) {
-                const unsigned char* xs = stage + slot * s1 + (16 * mt + g) * Z::xld;
-                const unsigned char* ws = stage + slot * s1 + T * Z::xld + g * Z::ald;
-                // (16-bit operands: this lane's row, and which of its two halves)
-                const uint32_t xm = smem_u32(stage + slot * s1 + (16 * mt + (lane & 15)) * Z::xld + (lane >> 4) * 16);
-                const uint32_t wm = smem_u32(stage + slot * s1 + T * Z::xld + ((lane & 7) + (lane >> 4) * 8) * Z::ald + (lane >> 3 & 1) * 16);
-                // fp32: a lane has four consecutive k of every row; the products do not mind in which order the tensor core takes them, as long as both operands agree.
+            // NT groups of eight ranks (SOME: of which some may be missing; without a branch per group their products run side by side).  The tensor core takes
+            // sixteen of one operand and eight of the other: rows and ranks, or, where there are few rows (FEW: up to eight), ranks and rows, which is half
+            // the products and half the splitting.
+            const auto products = [&](auto groups_of_8, auto some_missing, auto few_rows) {
+                constexpr int NT = decltype(groups_of_8)::value;
+                constexpr bool SOME = decltype(some_missing)::value, FEW = decltype(few_rows)::value;
+                constexpr int G = FEW ? 2 : 1, NG = NT / G;  // groups of eight that a product takes
+                float acc[NG][4];
 #pragma unroll
-                for (int s = 0; s < KC / 16 / KS; ++s) {
-                    const int k = 16 * (ks + KS * s) + 4 * q;
-                    if constexpr (Z::wide) {
-                        const float4 y0 = *reinterpret_cast<const float4*>(xs + k * 4), y1 = *reinterpret_cast<const float4*>(xs + 8 * Z::xld + k * 4);
-                        const float f[2][4] = {{y0.x, y0.y, y0.z, y0.w}, {y1.x, y1.y, y1.z, y1.w}};
-                        uint32_t hi[2][4], lo[2][4];
+                for (int j = 0; j < NG; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+                ad_pipeline<Z::stages>(count, fill, [&](int, int slot) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) ad_split(f[e >> 2][e & 3], hi[e >> 2][e & 3], lo[e >> 2][e & 3]);
+                    for (int s = 0; s < KC / 16 / KS; ++s) {
+                        if constexpr (Z::wide) {
+                            // A lane has four consecutive k of every row; the products do not mind in which order the tensor core takes them, as long as both
+                            // operands agree.
+                            const int k = 16 * (ks + KS * s) + 4 * q;
+                            const unsigned char* xs = stage + slot * s1 + (16 * mt + g) * Z::xld + k * 4;
+                            const unsigned char* ws = stage + slot * s1 + T * Z::xld + g * Z::ald + k * 2;
+                            uint32_t hi[2][4], lo[2][4];
 #pragma unroll
-                        for (int j = 0; j < kAdChunk / 8; ++j)
-                            if (j < nt) {
-                                const float4 b = ad_floats(*reinterpret_cast<const uint2*>(ws + 8 * j * Z::ald + k * 2), (const W*)nullptr);
-                                const uint32_t b0 = __float_as_uint(b.x), b1 = __float_as_uint(b.y), b2 = __float_as_uint(b.z), b3 = __float_as_uint(b.w);
-                                // The tensor core cuts its sums, always towards zero: sixteen k by themselves, which are then added with rounding (10240 k of random
-                                // numbers, 64 adapters: outputs 7.7e-7 off without this, 0.9e-7 with it).
-                                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                                ad_mma_tf32(c, lo[0][0], lo[1][0], lo[0][1], lo[1][1], b0, b1);
-                                ad_mma_tf32(c, lo[0][2], lo[1][2], lo[0][3], lo[1][3], b2, b3);
-                                ad_mma_tf32(c, hi[0][0], hi[1][0], hi[0][1], hi[1][1], b0, b1);
-                                ad_mma_tf32(c, hi[0][2], hi[1][2], hi[0][3], hi[1][3], b2, b3);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) acc[j][e] += c[e];
+                            for (int h = 0; h < (FEW ? 1 : 2); ++h) {
+                                const float4 y = *reinterpret_cast<const float4*>(xs + 8 * h * Z::xld);
+                                ad_split(y.x, hi[h][0], lo[h][0]);
+                                ad_split(y.y, hi[h][1], lo[h][1]);
+                                ad_split(y.z, hi[h][2], lo[h][2]);
+                                ad_split(y.w, hi[h][3], lo[h][3]);
                             }
-                    } else {
-                        uint32_t y[4];
-                        ad_ldm(y, xm + 32 * (ks + KS * s));
 #pragma unroll
-                        for (int j = 0; j < kAdChunk / 8; j += 2)
-                            if (j < nt) {  // (a second one past the last rank: zeros or numbers that nothing uses)
-                                uint32_t b[4];
-                                ad_ldm(b, wm + 8 * j * Z::ald + 32 * (ks + KS * s));
-                                ad_mma16(acc[j], y[0], y[1], y[2], y[3], b[0], b[1], (const W*)nullptr);
-                                ad_mma16(acc[j + 1], y[0], y[1], y[2], y[3], b[2], b[3], (const W*)nullptr);
-                            }
+                            for (int j = 0; j < NG; ++j)
+                                if (!SOME || G * j < nt) {
+                                    uint32_t b[G][4];
+#pragma unroll
+                                    for (int h = 0; h < G; ++h) {
+                                        const float4 v = ad_floats(*reinterpret_cast<const uint2*>(ws + 8 * (G * j + h) * Z::ald), (const W*)nullptr);
+                                        b[h][0] = __float_as_uint(v.x), b[h][1] = __float_as_uint(v.y), b[h][2] = __float_as_uint(v.z), b[h][3] = __float_as_uint(v.w);
+                                    }
+                                    // The tensor core cuts its sums, always towards zero: sixteen k by themselves, which are then added with rounding (10240 k of
+                                    // random numbers, 64 adapters: outputs 7.7e-7 off without this, 0.9e-7 with it).
+                                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                    for (int p = 0; p < 2; ++p) {
+                                        const auto& x = p ? hi : lo;
+#pragma unroll
+                                        for (int e = 0; e < 4; e += 2) {
+                                            if constexpr (FEW)
+                                                ad_mma_tf32(c, b[0][e], b[1][e], b[0][e + 1], b[1][e + 1], x[0][e], x[0][e + 1]);
+                                            else
+                                                ad_mma_tf32(c, x[0][e], x[1][e], x[0][e + 1], x[1][e + 1], b[0][e], b[0][e + 1]);
+                                        }
+                                    }
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) acc[j][e] += c[e];
+                                }
+                        } else {
+                            // (this lane's row of the operands, and which of its two halves)
+                            const uint32_t xm = smem_u32(stage + slot * s1 + (16 * mt + (lane & 15)) * Z::xld + (lane >> 4) * 16);
+                            const uint32_t wm = smem_u32(stage + slot * s1 + T * Z::xld + ((lane & 7) + (lane >> 4) * 8) * Z::ald + (lane >> 3 & 1) * 16);
+                            uint32_t y[4];
+                            ad_ldm(y, xm + 32 * (ks + KS * s));
+#pragma unroll
+                            for (int j = 0; j < NT; j += 2)
+                                if (!SOME || j < nt) {  // (a second one past the last rank: zeros or numbers that nothing uses)
+                                    uint32_t b[4];
+                                    ad_ldm(b, wm + 8 * j * Z::ald + 32 * (ks + KS * s));
+                                    if constexpr (FEW) {
+                                        ad_mma16(acc[j / 2], b[0], b[2], b[1], b[3], y[0], y[2], (const W*)nullptr);
+                                    } else {
+                                        ad_mma16(acc[j], y[0], y[1], y[2], y[3], b[0], b[1], (const W*)nullptr);
+                                        ad_mma16(acc[j + 1], y[0], y[1], y[2], y[3], b[2], b[3], (const W*)nullptr);
+                                    }
+                                }
+                        }
                     }
-                }
-            });
-            // the warps' sums meet: sums[ks][row][rank]
+                });
+                // the warps' sums meet: sums[ks][row][rank]
 #pragma unroll
-            for (int j = 0; j < kAdChunk / 8; ++j)
-                if (j < nt) {
-                    float* s0 = sums + ((ks * T + 16 * mt + g) * kAdSumLd + 8 * j + 2 * q);
-                    *reinterpret_cast<float2*>(s0) = make_float2(acc[j][0], acc[j][1]);
-                    *reinterpret_cast<float2*>(s0 + 8 * kAdSumLd) = make_float2(acc[j][2], acc[j][3]);
-                }
+                for (int j = 0; j < NG; ++j)
+                    if (G * j < nt) {
+                        if constexpr (FEW) {
+                            float* s0 = sums + ((ks * T + 2 * q) * kAdSumLd + 16 * j + g);
+                            s0[0] = acc[j][0], s0[kAdSumLd] = acc[j][1];
+                            s0[8] = acc[j][2], s0[kAdSumLd + 8] = acc[j][3];
+                        } else {
+                            float* s0 = sums + ((ks * T + 16 * mt + g) * kAdSumLd + 8 * j + 2 * q);
+                            *reinterpret_cast<float2*>(s0) = make_float2(acc[j][0], acc[j][1]);
+                            *reinterpret_cast<float2*>(s0 + 8 * kAdSumLd) = make_float2(acc[j][2], acc[j][3]);
+                        }
+                    }
+            };
+            const auto by_ranks = [&](auto few) {
+                if (nt <= 2)
+                    products(std::integral_constant<int, 2>(), std::false_type(), few);
+                else if (nt <= 4)
+                    products(std::integral_constant<int, 4>(), std::false_type(), few);
+                else if (nt == 8)
+                    products(std::integral_constant<int, 8>(), std::false_type(), few);
+                else
+                    products(std::integral_constant<int, 8>(), std::true_type(), few);
+            };
+            if (MT == 1 && n_rows <= 8)
+                by_ranks(std::integral_constant<bool, MT == 1>());
+            else
+                by_ranks(std::false_type());
             __syncthreads();
             const int cols = (ranks + 15) / 16 * 16;  // (ranks behind the last one: zeros)
             for (int i = tid; i < T * cols / 4; i += kAdThreads) {
@@ -576,63 +627,83 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                 }
         }
     };
-    float acc[J][4];
     const uint32_t wm = smem_u32(stage) + (FW * ks + (lane & 7) + (lane >> 4) * 8) * wld + (lane >> 3 & 1) * 16;
     const uint32_t tm = smem_u32(t16) + (16 * mt + (lane & 15)) * pld + (lane >> 4) * 16;
-    ad_pipeline<Z::stages>(count, fill, [&](int i, int slot) {
-        const uint32_t ws = wm + slot * s2;
-        const unsigned char* bs = stage + slot * s2 + FB * wld;
-        const int fb = chunks == 1 ? i : i / chunks, ch = chunks == 1 ? 0 : i % chunks, steps = min(kAdChunk, r16 - ch * kAdChunk) / 16;
-        if (ch == 0)
+    // SK groups of sixteen ranks, whose operand of t a warp keeps (0: any number, read again)
+    const auto outputs = [&](auto groups_of_16) {
+        constexpr int SK = decltype(groups_of_16)::value;
+        uint32_t kept[SK ? SK : 1][pieces][4];
 #pragma unroll
-            for (int j = 0; j < J; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        const uint32_t tp = tm + ch * kAdChunk * 2;
+        for (int k = 0; k < SK; ++k)
 #pragma unroll
-        for (int k = 0; k < kAdChunk / 16; ++k)
-            if (k < steps) {
-                uint32_t w[J / 2][4];
+            for (int p = 0; p < pieces; ++p) ad_ldm(kept[k][p], tm + p * T * pld + 32 * k);
+        float acc[J][4];
+        ad_pipeline<Z::stages>(count, fill, [&](int i, int slot) {
+            const uint32_t ws = wm + slot * s2;
+            const unsigned char* bs = stage + slot * s2 + FB * wld;
+            const int fb = SK || chunks == 1 ? i : i / chunks, ch = SK || chunks == 1 ? 0 : i % chunks, steps = SK ? SK : min(kAdChunk, r16 - ch * kAdChunk) / 16;
+            if (ch == 0)
 #pragma unroll
-                for (int j = 0; j < J / 2; ++j) ad_ldm(w[j], ws + 16 * j * wld + 32 * k);
+                for (int j = 0; j < J; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+            const uint32_t tp = tm + ch * kAdChunk * 2;
 #pragma unroll
-                for (int p = pieces - 1; p >= 0; --p) {
-                    uint32_t t[4];
-                    ad_ldm(t, tp + p * T * pld + 32 * k);
+            for (int k = 0; k < (SK ? SK : kAdChunk / 16); ++k)
+                if (SK || k < steps) {
+                    uint32_t w[J / 2][4];
 #pragma unroll
-                    for (int j = 0; j < J; ++j) ad_mma16(acc[j], t[0], t[1], t[2], t[3], w[j / 2][j % 2 * 2], w[j / 2][j % 2 * 2 + 1], (const W*)nullptr);
-                }
-            }
-        if (ch == chunks - 1) {
-            const int left = m_to - m_from - fb * FB - FW * ks - 4 * q;
-            const bool whole = P.wide_out && m_from + (fb + 1) * FB <= m_to;
-            const unsigned char* b0 = bs + (16 * mt + g) * Z::bld + (FW * ks + 4 * q) * (int)sizeof(X);
+                    for (int j = 0; j < J / 2; ++j) ad_ldm(w[j], ws + 16 * j * wld + 32 * k);
 #pragma unroll
-            for (int h = 0; h < FW / 16; ++h) {
-                // a lane has four neighbouring outputs of two rows
-                float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
-                if (bp) {
-                    if constexpr (Z::wide) {
-                        v0 = *reinterpret_cast<const float4*>(b0 + 64 * h), v1 = *reinterpret_cast<const float4*>(b0 + 8 * Z::bld + 64 * h);
-                    } else {
-                        v0 = ad_floats(*reinterpret_cast<const uint2*>(b0 + 32 * h), (const X*)nullptr);
-                        v1 = ad_floats(*reinterpret_cast<const uint2*>(b0 + 8 * Z::bld + 32 * h), (const X*)nullptr);
+                    for (int p = pieces - 1; p >= 0; --p) {
+                        uint32_t t[4];
+                        if constexpr (SK)
+                            t[0] = kept[k % SK][p][0], t[1] = kept[k % SK][p][1], t[2] = kept[k % SK][p][2], t[3] = kept[k % SK][p][3];
+                        else
+                            ad_ldm(t, tp + p * T * pld + 32 * k);
+#pragma unroll
+                        for (int j = 0; j < J; ++j) ad_mma16(acc[j], t[0], t[1], t[2], t[3], w[j / 2][j % 2 * 2], w[j / 2][j % 2 * 2 + 1], (const W*)nullptr);
                     }
                 }
-                if (r_all) {
-                    v0 = make_float4(fmaf(t0, acc[2 * h][0], v0.x), fmaf(t0, acc[2 * h][1], v0.y), fmaf(t0, acc[2 * h + 1][0], v0.z), fmaf(t0, acc[2 * h + 1][1], v0.w));
-                    v1 = make_float4(fmaf(t1, acc[2 * h][2], v1.x), fmaf(t1, acc[2 * h][3], v1.y), fmaf(t1, acc[2 * h + 1][2], v1.z), fmaf(t1, acc[2 * h + 1][3], v1.w));
+            if (ch == chunks - 1) {
+                const int left = m_to - m_from - fb * FB - FW * ks - 4 * q;
+                const bool whole = P.wide_out && m_from + (fb + 1) * FB <= m_to;
+                const unsigned char* b0 = bs + (16 * mt + g) * Z::bld + (FW * ks + 4 * q) * (int)sizeof(X);
+#pragma unroll
+                for (int h = 0; h < FW / 16; ++h) {
+                    // a lane has four neighbouring outputs of two rows
+                    float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
+                    if (bp) {
+                        if constexpr (Z::wide) {
+                            v0 = *reinterpret_cast<const float4*>(b0 + 64 * h), v1 = *reinterpret_cast<const float4*>(b0 + 8 * Z::bld + 64 * h);
+                        } else {
+                            v0 = ad_floats(*reinterpret_cast<const uint2*>(b0 + 32 * h), (const X*)nullptr);
+                            v1 = ad_floats(*reinterpret_cast<const uint2*>(b0 + 8 * Z::bld + 32 * h), (const X*)nullptr);
+                        }
+                    }
+                    if (r_all) {
+                        v0 = make_float4(fmaf(t0, acc[2 * h][0], v0.x), fmaf(t0, acc[2 * h][1], v0.y), fmaf(t0, acc[2 * h + 1][0], v0.z), fmaf(t0, acc[2 * h + 1][1], v0.w));
+                        v1 = make_float4(fmaf(t1, acc[2 * h][2], v1.x), fmaf(t1, acc[2 * h][3], v1.y), fmaf(t1, acc[2 * h + 1][2], v1.z), fmaf(t1, acc[2 * h + 1][3], v1.w));
+                    }
+                    if (whole) {
+                        if (have0) ad_store4(o0 + 16 * h, v0);
+                        if (have1) ad_store4(o1 + 16 * h, v1);
+                    } else {
+                        if (have0) ad_store4(o0 + 16 * h, v0, left - 16 * h, P.wide_out);
+                        if (have1) ad_store4(o1 + 16 * h, v1, left - 16 * h, P.wide_out);
+                    }
                 }
-                if (whole) {
-                    if (have0) ad_store4(o0 + 16 * h, v0);
-                    if (have1) ad_store4(o1 + 16 * h, v1);
-                } else {
-                    if (have0) ad_store4(o0 + 16 * h, v0, left - 16 * h, P.wide_out);
-                    if (have1) ad_store4(o1 + 16 * h, v1, left - 16 * h, P.wide_out);
-                }
+                o0 += FB;
+                o1 += FB;
             }
-            o0 += FB;
-            o1 += FB;
-        }
-    });
+        });
+    };
+    if (r16 == 16)
+        outputs(std::integral_constant<int, 1>());
+    else if (r16 == 32)
+        outputs(std::integral_constant<int, 2>());
+    else if (r16 == 64)
+        outputs(std::integral_constant<int, 4>());
+    else
+        outputs(std::integral_constant<int, 0>());
     if (r_all > 0 && S > 1) {
         __syncwarp();
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // no CTA leaves while its part may be read
