@@ -149,6 +149,7 @@ struct AdShape {
     static constexpr int FW = MT == 4 ? 32 : 16;        // outputs of a warp in a stage
     static constexpr int FB = FW * KS;                  // ... and of a stage
     static constexpr int stages = STAGES;
+    static constexpr int most_rank = MT == 1 && STAGES > 3 ? 32 : kAdMaxRank < kAdMostCells / T ? kAdMaxRank : kAdMostCells / T;
     // Bytes from row to row.  16-bit operands are read as matrices of eight rows of 16 bytes: rows an odd multiple of 16 bytes apart lie in different banks.
     // Of the others a lane reads four values of the row that is its number over four: the rows of a quarter (16-byte reads) or half (8-byte reads) of a warp
     // lie in different banks when they are 16 or 8 words apart, modulo 32.
@@ -482,12 +483,14 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             const auto by_ranks = [&](auto few) {
                 if (nt <= 2)
                     products(std::integral_constant<int, 2>(), std::false_type(), few);
-                else if (nt <= 4)
+                else if (Z::most_rank <= 32 || nt <= 4)
                     products(std::integral_constant<int, 4>(), std::false_type(), few);
-                else if (nt == 8)
-                    products(std::integral_constant<int, 8>(), std::false_type(), few);
-                else
-                    products(std::integral_constant<int, 8>(), std::true_type(), few);
+                else if constexpr (Z::most_rank > 32) {
+                    if (nt == 8)
+                        products(std::integral_constant<int, 8>(), std::false_type(), few);
+                    else
+                        products(std::integral_constant<int, 8>(), std::true_type(), few);
+                }
             };
             if (MT == 1 && n_rows <= 8)
                 by_ranks(std::integral_constant<bool, MT == 1>());
@@ -700,8 +703,8 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
         outputs(std::integral_constant<int, 1>());
     else if (r16 == 32)
         outputs(std::integral_constant<int, 2>());
-    else if (r16 == 64)
-        outputs(std::integral_constant<int, 4>());
+    else if (Z::most_rank > 32 && r16 == 64)
+        outputs(std::integral_constant<int, (Z::most_rank > 32 ? 4 : 0)>());
     else
         outputs(std::integral_constant<int, 0>());
     if (r_all > 0 && S > 1) {
