@@ -12,7 +12,7 @@
 //   zoom    Bins with more than 384 logits (a flat row, a large vocabulary, 16-bit logits) are divided into 512 bins again, up to four times; of equal logits
 //           as many are kept as the weight left, or the number, needs.  74 rows of 131072 logits with a deviation of 0.3 and top-p 0.9: 0.16 ms, where one
 //           CTA a row took 2.1 ms; 65536 logits of bf16 rounded to few values: under 0.15 ms and 1.1 ms.
-//   neither Where that misses (the weight of a bin is estimated from its middle), or more than top-k are equal, one CTA does the row by radix passes
+//   neither Where more than 384 logits are equal to a small top-k's last, or four divisions were not enough, one CTA does the row by radix passes
 //           (dw_row_plain).
 // Without top-k and top-p no cut is needed: min-p's is a value that follows from the maximum.
 //
@@ -657,10 +657,8 @@ template <typename T>
 struct DcStretch {
     DcRow<T>& R;
     static constexpr int N = DcVec<T>::n;
-    static constexpr float kTolerance = sizeof(T) == 2 ? 1.0f / 512.0f : 1.0f / 2048.0f;
     float mn;               // the smallest of the threads' largest logits
-    bool marked, weighed;   // marked: the slice is short enough for marks; weighed: the bins are, otherwise a bin's weight is taken in its middle, which is good
-                            // enough without the largest logits
+    bool marked, weighed;   // marked: the slice is short enough for marks; weighed: the bins are (for top-p)
     float rel_unit;         // (8192 or, of 16 bits, 16384 logits of a marked slice stay under 2^32, and up to 98304 of a long one)
     float from_l, to_l;     // the cut lies from here on, under this
     const u64* base;        // weights of the warps' stretches from to_l on (null: none),
@@ -673,7 +671,7 @@ struct DcStretch {
     __device__ __forceinline__ void begin(float smallest) {
         mn = smallest;
         marked = R.seg <= 32 * N * kDcMarked;
-        weighed = R.r.top_k && R.r.top_p > 0.f;
+        weighed = R.r.top_p > 0.f;
         rel_unit = marked ? 131072.0f : 16384.0f;
     }
     __device__ __forceinline__ void whole(float from) { from_l = from, to_l = INFINITY, base = nullptr, base_all = base_n = 0; }
@@ -756,20 +754,21 @@ struct DcStretch {
         return true;
     }
     // Top-p's cut: between the bins that the bins' weights say, in units of 2^-24 of the largest one here.
-    __device__ __forceinline__ int find_p(u64 P, float tolerance, int& b1, int& b2) {
+    __device__ __forceinline__ int find_p(u64 P, int& b1, int& b2) {
         const DwRow& r = R.r;
         const double unit = exp2(24.0 - (double)r.F + (r.mxd - (double)top_l) * r.c);
-        const float scale = 16777216.0f / rel_unit, mid = rel_unit * exp2f(0.5f * bin_y);
+        const float scale = 16777216.0f / rel_unit;
         float near[kDcBinsPer];
         u64 sum = 0, all;
 #pragma unroll
         for (int i = 0; i < kDcBinsPer; ++i) {
-            near[i] = rintf((weighed ? (float)rel[i] : (float)cnt[i] * mid) * exp2f((float)(kDcBinsPer * R.tid + i) * bin_y) * scale);
+            near[i] = rintf((float)rel[i] * exp2f((float)(kDcBinsPer * R.tid + i) * bin_y) * scale);
             sum += (u64)near[i];
         }
         const u64 before = dc_before(sum, R.sh.wsum, all), want = P > base_all ? (u64)fmin((double)(P - base_all) * unit, 1e18) : 0ull;
-        // Weighed bins are 2^-17 of them off at most; in the others the weights of many tokens average, but the cut may lie among a few that come first.
-        const u64 off = weighed ? want >> 15 : (u64)((float)want * tolerance) + (16777216u / 100u);
+        // A logit's weight in its bin is cut at 2^-17 (or 2^-14) of the bin's upper end.  (Bins that are only counted, with the weight of their middle, made
+        // rows of 1024 x 65536 with top-p 0.9 1 % faster, but missed the cut where logits have few values: one bf16 row in some hundreds, of 1 ms.)
+        const u64 off = (want >> (marked ? 15 : 12)) + 512;
         return find_bins(before, near, want > off ? want - off : 1, want + off, b1, b2);
     }
     // min-p's cut comes before bin b.
@@ -989,7 +988,7 @@ __device__ __noinline__ void dc_zoomed(const DrawArgs& A, int S, int n_slice, bo
                 break;
             }
         } else {
-            n_in = D.find_p(P, D.base ? 1.0f / 4096.0f : D.kTolerance, b1, b2);
+            n_in = D.find_p(P, b1, b2);
             if (D.min_p_before(b1)) {
                 end = kDcByMinP, c.limit = P;
                 break;
@@ -1178,7 +1177,7 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(const __gri
             P = dw_share(r.top_p, total);
         }
         if (at_p) {
-            n_in = D.find_p(P, D.kTolerance, b1, b2);
+            n_in = D.find_p(P, b1, b2);
             end = kDcByMinP;
             if (D.min_p_before(b1)) {
                 c.limit = P;
