@@ -19,7 +19,6 @@ template <typename X, typename W, int MT, int STAGES>
 static void launch_tiles(cudaStream_t stream, int device, AdapterArgs P) {
     typedef AdShape<X, W, MT, STAGES> Z;
     constexpr int T = Z::T;
-    static_assert(T * kAdMaxRank <= kAdMostCells || MT == 4, "only the largest tile depends on the rank");
     P.block_rows = std::min(P.rows, kAdBlockRows);
     const int blocks = (P.rows + P.block_rows - 1) / P.block_rows;
     P.tiles = std::min(P.block_rows, P.block_rows / T + std::min(P.slots + P.copies, P.block_rows));
@@ -51,12 +50,18 @@ static void launch_tiles(cudaStream_t stream, int device, AdapterArgs P) {
 template <typename X, typename W>
 static void launch_adapters(cudaStream_t stream, int device, AdapterArgs P) {
     const int rows = std::min(P.rows, kAdBlockRows), each = rows / std::min(P.slots, rows);  // rows of an adapter, if they are shared evenly
-    // large tiles read the adapters less often, but only if enough of them are left for the GPU
-    const auto fits = [&](int T) { return each >= T * 3 / 4 && T * P.rank_cap <= kAdMostCells && expected_tiles(P, T) * kAdMaxCtas >= 240; };
-    if (fits(64))
+    // Larger tiles read the adapters less often, but leave fewer CTAs side by side and split x more often: where sixteen rows' activations are under two thirds of
+    // an adapter, and enough tiles are left for the GPU.  us with tiles of 16, 32 and 64 rows, by that proportion: bf16, 4096 rows, 64 ranks, 2560 x 10240 (0.45)
+    // 100, 87, 76; 2048 rows, 256 ranks, 2560 x 2560 (0.1) 84, 76; 128 ranks (0.2) 49, 44, 96 (one CTA per SM: so 64 rows for up to 64 ranks); fp32, 4096 rows, 64
+    // ranks (0.75) 56, 53, 57; 1024 rows, 32 ranks (1.5) 17.3, 18.7; 4096 rows, 16 ranks (3) 37, 55, 51.  Fewer tiles than the 240 CTAs: 1024 rows, 32 ranks in
+    // tiles of 64 rows 26.5.
+    const int64_t xs = sizeof(X), adapter = (int64_t)P.rank_cap * (P.K + P.M) * 2, sixteen = 16 * xs * (P.K + (int64_t)P.M * (P.base ? 2 : 1));
+    const auto fits = [&](int T) { return 2 * adapter >= 3 * sixteen && each >= T * 3 / 4 && expected_tiles(P, T) * kAdMaxCtas >= 240; };
+    if (P.rank_cap <= kAdChunk && fits(64))
         launch_tiles<X, W, 4, sizeof(X) == 4 ? 2 : 3>(stream, device, P);
     else if (fits(32))
         launch_tiles<X, W, 2, 3>(stream, device, P);
+    // five stages where they fit twice on an SM: 64 sessions of 10240 k 19.9 us, with three 20.7
     else if (P.rank_cap <= 32)
         launch_tiles<X, W, 1, 5>(stream, device, P);
     else

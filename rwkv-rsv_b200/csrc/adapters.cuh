@@ -137,7 +137,8 @@ struct AdShape {
     static constexpr int FW = MT == 4 ? 32 : 16;        // outputs of a warp in a stage
     static constexpr int FB = FW * KS;                  // ... and of a stage
     static constexpr int stages = STAGES;
-    static constexpr int most_rank = MT == 1 && STAGES > 3 ? 32 : kAdMaxRank < kAdMostCells / T ? kAdMaxRank : kAdMostCells / T;
+    static constexpr int most_rank = MT == 1 && STAGES > 3 ? 32 : MT == 4 ? kAdChunk : kAdMaxRank;
+    static_assert(T * most_rank <= kAdMostCells, "t lies where the sums were");
     // Bytes from row to row.  16-bit operands are read as matrices of eight rows of 16 bytes: rows an odd multiple of 16 bytes apart lie in different banks.
     // Of the others a lane reads four values of the row that is its number over four: the rows of a quarter (16-byte reads) or half (8-byte reads) of a warp
     // lie in different banks when they are 16 or 8 words apart, modulo 32.
@@ -621,18 +622,19 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
     const X* bnext[BP];
 #pragma unroll
     for (int p = 0; p < BP; ++p) bnext[p] = bp + (bp ? (int64_t)sh.rows[min(brow + p * (kAdThreads / BU), n_rows - 1)] * P.ldbase + m_from + bu : 0);
+    const bool wide_in = P.wide_b && (!bp || P.wide_base);  // (one condition: with two, 4096 rows of bf16 take 78 instead of 75 us)
     const auto fill = [&](int i, int slot) {
         unsigned char* ws = stage + slot * s2;
         unsigned char* bs = ws + FB * wld + brow * Z::bld + tid % BU * 16;
         const int fb = chunks == 1 ? i : i / chunks, ch = chunks == 1 ? 0 : i % chunks, left = m_to - m_from - fb * FB, r = ch * kAdChunk + 8 * wu;
-        const bool whole_b = P.wide_b && left >= FB, whole_base = P.wide_base && left >= FB;
+        const bool whole = wide_in && left >= FB;
         if (r < r16) {
             const W* from = wnext + ch * kAdChunk;
             unsigned char* to = ws + wat * wld + wu * 16;
             const int bytes = max(0, min(8, r_all - r)) * 2;
 #pragma unroll 2
             for (int f = wrow; f < FB; f += wstep) {
-                if (whole_b)
+                if (whole)
                     ad_copy16(to, bytes ? from : wb, bytes);
                 else
                     ad_fill16(to, from, f < left ? r_all - r : 0, P.wide_b);
@@ -645,7 +647,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             if (bp)
 #pragma unroll
                 for (int p = 0; p < BP; ++p) {
-                    if (whole_base) {
+                    if (whole) {
                         if (brow + p * (kAdThreads / BU) < n_rows) ad_copy16(bs + p * (kAdThreads / BU) * Z::bld, bnext[p]);
                     } else
                         ad_fill16(bs + p * (kAdThreads / BU) * Z::bld, bnext[p], left - bu, P.wide_base);

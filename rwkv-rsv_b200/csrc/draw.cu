@@ -28,7 +28,7 @@ static void launch_draw(cudaStream_t stream, int device, int64_t rows, const Dra
         return;
     }
     // few rows: over more CTAs, as long as the GPU has room for them
-    while (S < kDcMaxCtas && rows * S * 2 <= 592 && places > (int64_t)S * 4 * unit) S *= 2;
+    while (S < kDcMaxCtas && rows * S * 2 <= 2 * 148 && places > (int64_t)S * 4 * unit) S *= 2;
     const int slice = (int)((places + (int64_t)S * unit - 1) / ((int64_t)S * unit)) * unit;
     const size_t smem = sizeof(DcShared) + std::max((size_t)slice * sizeof(T), sizeof(DwPlainShared));
     static bool configured[64] = {false};
