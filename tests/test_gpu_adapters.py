@@ -88,6 +88,24 @@ def test_exact_in_whole_numbers(rows, K, M, slots, most, x, w):
 
 
 @pytest.mark.parametrize("x,w", TYPES)
+@pytest.mark.parametrize("pad", [(0, 0, 0, 0), (3, 5, 7, 9), (4, 8, 8, 4)])
+@pytest.mark.parametrize("rows,K,M,slots,most", [(2000, 640, 96, 4, 64), (2100, 1000, 52, 3, 48), (1000, 256, 320, 4, 128), (1111, 333, 77, 2, 256), (4200, 128, 64, 5, 64)])
+def test_many_rows_of_large_adapters(rows, K, M, slots, most, pad, x, w):
+    """Tiles of 32 and 64 rows."""
+    d = make(rows, K, M, slots, most, x, w, pad=pad)
+    check(d, apply(d))
+
+
+@pytest.mark.parametrize("x,w", TYPES)
+@pytest.mark.parametrize("rows,slots", [(1, 1), (7, 1), (8, 1), (9, 1), (16, 2), (17, 2), (33, 4), (40, 40)])
+@pytest.mark.parametrize("most", [1, 8, 9, 16, 17, 33, 64, 65, 100])
+def test_few_rows_of_an_adapter(rows, slots, most, x, w):
+    """Up to eight rows of an adapter are the smaller operand."""
+    d = make(rows, 200, 72, slots, most, x, w, ranks=rows != 8, none=False)
+    check(d, apply(d))
+
+
+@pytest.mark.parametrize("x,w", TYPES)
 @pytest.mark.parametrize("order", ["sorted", "one", "shuffled"])
 def test_orders_of_rows(order, x, w):
     d = make(300, 512, 256, 7, 16, x, w, order=order, none=order == "shuffled")
