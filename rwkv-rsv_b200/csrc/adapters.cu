@@ -22,7 +22,7 @@ static void launch_tiles(cudaStream_t stream, int device, AdapterArgs P) {
     P.block_rows = std::min(P.rows, kAdBlockRows);
     const int blocks = (P.rows + P.block_rows - 1) / P.block_rows;
     P.tiles = std::min(P.block_rows, P.block_rows / T + std::min(P.slots + P.copies, P.block_rows));
-    // Two CTAs fit on an SM, and one round of them is the fastest: 64 sessions of 10240 k on 64 adapters take 19 us as 256 CTAs (20 with three on an SM, whose
+    // Two CTAs fit on an SM, and one round of them is the fastest: 64 sessions of 10240 k on 64 adapters take 20 us as 256 CTAs (25 with three on an SM, whose
     // registers spill).  Any number of CTAs is a cluster: 50 such sessions take 17.2 us with five CTAs each and 19.0 with four.  (The tiles that will be there,
     // not those that may be.)
     P.S = kAdMaxCtas;

@@ -9,6 +9,10 @@
 // Both products run on the tensor cores with fp32 sums.  16-bit activations are operands as they are; fp32 ones are two tf32 numbers each (ad_split),
 // and the 16-bit weights are exact in tf32.  t is two fp16 numbers per value, relative to the row's largest
 // (2^-25 of it off), or two bf16 ones (2^-17; three, 2^-25, where out is fp32), so that B is an operand as it is.
+//
+// Bound by its instructions: a scheduler issues in 35 to 48 % of the cycles, four warps of it waiting for fixed latencies, and in short calls for instructions that
+// are fetched for the first time.  4096 bf16 rows, 16 adapters of 64 ranks, 2560 x 10240: 78 us, 2.6 TB/s (the second product 50 of them); 64 sessions of 10240 k with 64
+// adapters of 16 ranks, fp32: 20 us, 1.0 TB/s; one session of 2560 x 2560: 10 us, all latency.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -94,8 +98,6 @@ template <typename E>
 __device__ __forceinline__ void ad_store4(E* p, const float4& v, int n, bool wide) {
     if (wide && n >= 4)
         ad_store4(p, v);
-    else if (n >= 4)
-        p[0] = ad_round<E>(v.x), p[1] = ad_round<E>(v.y), p[2] = ad_round<E>(v.z), p[3] = ad_round<E>(v.w);
     else
         ad_store_some(p, v, n);
 }
@@ -284,7 +286,7 @@ __device__ __forceinline__ void ad_copy(uint32_t dst, const void* src, int bytes
 }
 // `n` values (none for n <= 0) of a row from src on to 16 bytes of shared memory, zeros behind them; `wide`: src is at 16 bytes.  Rows that are not go in pieces
 // of 8 or 4 bytes, asynchronously as well; 16-bit ones that begin inside a word are put together from the words in between.  (4040 rows of 3126 fp32: 117 us value
-// by value, 76 so; 1631 rows of 13847 fp32 outputs with 2 ranks: 326 and 160 us.)
+// by value, 42 so; 1631 rows of 13847 fp32 outputs with 2 ranks: 326 and 152 us.)
 template <typename E>
 __device__ __noinline__ void ad_fill16(void* dst, const E* src, int n, bool wide) {
     constexpr int N = 16 / (int)sizeof(E);
@@ -622,7 +624,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
     const X* bnext[BP];
 #pragma unroll
     for (int p = 0; p < BP; ++p) bnext[p] = bp + (bp ? (int64_t)sh.rows[min(brow + p * (kAdThreads / BU), n_rows - 1)] * P.ldbase + m_from + bu : 0);
-    const bool wide_in = P.wide_b && (!bp || P.wide_base);  // (one condition: with two, 4096 rows of bf16 take 78 instead of 75 us)
+    const bool wide_in = P.wide_b && (!bp || P.wide_base);
     const auto fill = [&](int i, int slot) {
         unsigned char* ws = stage + slot * s2;
         unsigned char* bs = ws + FB * wld + brow * Z::bld + tid % BU * 16;

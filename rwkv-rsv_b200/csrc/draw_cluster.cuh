@@ -20,6 +20,9 @@
 //
 // What the CTAs tell each other is written into the receiver's shared memory before a cluster barrier, so that nobody has to stay for others to read: one
 // CTA finishes a row while the others' places go to the next rows.
+//
+// Rows of 65536 fp32 logits, us on the GPU: one row 4.7 (greedy), 10.5 (top-k 50, top-p 0.9), 24 (top-p 0.9), bound by barriers and one CTA's chain; 1024 rows 78 (3.4 TB/s),
+// 129 and 432, bound by instructions.  Five CTAs of 48 registers on an SM.
 #pragma once
 #include "draw.cuh"
 #include "tc_ptx.cuh"
