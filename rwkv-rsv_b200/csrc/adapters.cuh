@@ -7,8 +7,12 @@
 //   t = A x   the CTAs of the cluster split K, the warps of a CTA split it again; the partial sums meet in shared memory and then in the cluster's.
 //   B t       the CTAs split M; every CTA has all of t.
 // Both products run on the tensor cores with fp32 sums.  16-bit activations are operands as they are; fp32 ones are two tf32 numbers each (ad_split),
-// and the 16-bit weights are exact in tf32.  t is two fp16 numbers per value, relative to the row's largest
-// (2^-25 of it off), or two bf16 ones (2^-17; three, 2^-25, where out is fp32), so that B is an operand as it is.
+// and the 16-bit weights are exact in tf32.  t is two fp16 numbers per value, or two bf16 ones (2^-17 of it off; three, 2^-25, where out is fp32), so that B is an
+// operand as it is.  fp16 ends early: the row's largest value is brought to 2^14 .. 2^15, and one down to 2^-20 of it is at most 2^-20 of itself off (2^-23 and 2^-17
+// where out has 16 bits).  A tile with a value further down whose parts are all that small (one that cancelled is no more exact than its parts), or with a row's largest
+// outside 2^-100 .. 2^100, has t as two tf32 numbers (2^-22 of any value) and the second product in tf32: what a rank adds keeps its precision whatever the other
+// ranks add, as it has to where outputs use few of them.  (With all tiles of that kind: one fp32 session of 2560 x 2560 11.2 us instead of 8.4, 512 rows with 64 ranks of
+// 2560 x 10240 39 instead of 25.)
 //
 // Bound by its instructions: a scheduler issues in 35 to 48 % of the cycles, four warps of it waiting for fixed latencies, and in short calls for instructions that
 // are fetched for the first time.  4096 bf16 rows, 16 adapters of 64 ranks, 2560 x 10240: 78 us, 2.6 TB/s (the second product 50 of them); 64 sessions of 10240 k with 64
@@ -107,11 +111,12 @@ __device__ __forceinline__ void ad_ldm(uint32_t (&v)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
 }
 // v as two tf32 numbers: the first rounded to nearest, the rest (of up to 12 bits) cut to 11, so together they are at most 2^-22 of v off and 2^-24 on average.
-// A NaN stays one in the rest, an infinity has no rest.  (The conversion instruction takes several times as long as this.)
+// The first is always finite: next to the largest float it is the largest tf32 number, and infinities and NaN are in the rest.  (The conversion instruction takes several
+// times as long as this.)
 __device__ __forceinline__ void ad_split(float v, uint32_t& hi, uint32_t& lo) {
-    hi = (__float_as_uint(v) + 0x1000u) & 0xFFFFE000u;
-    const float h = __uint_as_float(hi);
-    lo = fabsf(h) == INFINITY ? 0u : __float_as_uint(v - h) & 0xFFFFE000u;
+    const float most = __uint_as_float(0x7F7FE000u), h = fminf(fmaxf(__uint_as_float((__float_as_uint(v) + 0x1000u) & 0xFFFFE000u), -most), most);
+    hi = __float_as_uint(h);
+    lo = __float_as_uint(v - h) & 0xFFFFE000u;
 }
 __device__ __forceinline__ void ad_mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -159,7 +164,7 @@ constexpr int kAdSumLd = kAdChunk + 8;  // (rows eight banks apart)
 struct AdTile {
     int rows[64];
     float scale[64];  // 2^e of the row's t, times the adapter's scale
-    int slot, n, skip, wsum[kAdWarps];
+    int slot, n, skip, apart, wsum[kAdWarps];
 };
 static_assert(sizeof(AdTile) <= 1024, "the tile's part of shared memory");
 
@@ -371,6 +376,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3, mt = warp % MT, ks = warp / MT;
     const int S = P.S, rank = S > 1 ? (int)ad_rank() : 0;
     const int job = (int)blockIdx.x / S, block = job / P.tiles, first = block * P.block_rows;
+    if (tid == 0) sh.apart = 0;
     if (!ad_find_tile<T>(P, first, min(P.block_rows, P.rows - first), job % P.tiles, sh, reinterpret_cast<unsigned short*>(sums))) return;  // (all CTAs of the cluster)
     const int n_rows = sh.n, a = sh.slot;
     const bool has = a < P.slots;
@@ -379,6 +385,8 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
     const X* bp = reinterpret_cast<const X*>(P.base);
     X* op = reinterpret_cast<X*>(P.out);
 
+    float* t32 = reinterpret_cast<float*>(t16);
+    static_assert(pieces >= 2, "t fits where its 16-bit numbers go");
     if (r_all > 0) {
         // ---- t = A x: this CTA's part of K, 64 k and more at a time through shared memory
         const int units = (P.K + 63) / 64, k_from = 64 * (int)((long long)units * rank / S), k_to = min(P.K, 64 * (int)((long long)units * (rank + 1) / S));
@@ -551,7 +559,9 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
         }
         constexpr int TPR = kAdThreads / T;  // threads of a row
         const int row = tid / TPR, c = tid % TPR;
+        constexpr bool scaled = std::is_same<W, __half>::value;
         float most = 0.f;
+        uint32_t small = ~0u;  // bits of the smallest that is not 0, times two, less one
         for (int i = 4 * c; i < r16; i += 4 * TPR) {
             float4 s = *reinterpret_cast<const float4*>(part + row * cap + i);
             if (S > 1) {
@@ -569,18 +579,45 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                 for (int p = 0; p < kAdMaxCtas; ++p)
                     if (p < S) s.x += v[p].x, s.y += v[p].y, s.z += v[p].z, s.w += v[p].w;
             }
+            if (scaled)
+                small = min(small, min(min(2 * __float_as_uint(s.x) - 1, 2 * __float_as_uint(s.y) - 1), min(2 * __float_as_uint(s.z) - 1, 2 * __float_as_uint(s.w) - 1)));
             most = fmaxf(most, fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w))));
             *reinterpret_cast<float4*>(sums + row * cap + i) = s;
         }
 #pragma unroll
         for (int o = TPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        // fp16: relative to a power of two from the row's largest on
-        float up = 1.f, down = 1.f;
-        if (std::is_same<W, __half>::value && most > 0.f && most < INFINITY) {
-            const int e = min(max((int)(__float_as_uint(most) >> 23) - 126, -120), 126);
-            up = __uint_as_float((uint32_t)(127 + e) << 23);
-            down = __uint_as_float((uint32_t)(127 - e) << 23);
+        // fp16: relative to the power of two that brings the row's largest to 2^14 .. 2^15.  Two of them are 2^-24 of a value off, but no less than 2^-25.  (Beside an
+        // infinity, which stays one, finite values are under 2^15 as well.)
+        bool far = most > 0.f && most < INFINITY && !(most >= 0x1p-100f && most < 0x1p100f);
+        float up = 1.f, down = scaled || most < INFINITY ? 1.f : 0.5f;
+        if (scaled && most > 0.f && !far) {
+            constexpr uint32_t below = Z::wide ? 20 : 23;
+            const uint32_t e = __float_as_uint(most) >> 23;  // (27 .. 226, or 255)
+            up = __uint_as_float((e - 14) << 23);
+            down = __uint_as_float((268 - e) << 23);
+            const uint32_t least = (e + 1 - below) << 23;
+            if (__builtin_expect(small < 2 * least - 1 && most < INFINITY && row < n_rows, 0)) {
+                far = S == 1;
+                if (!far)
+#pragma unroll 1
+                    for (int i = 4 * c; i < r16; i += 4 * TPR)
+#pragma unroll 1
+                        for (int j = i; j < i + 4; ++j) {
+                            if (2 * __float_as_uint(sums[row * cap + j]) - 1 >= 2 * least - 1) continue;
+                            float m = 0.f;
+#pragma unroll 4
+                            for (int p = 0; p < S; ++p) {
+                                uint32_t from;
+                                float v;
+                                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(smem_u32(part + row * cap + j)), "r"(p));
+                                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
+                                m = fmaxf(m, fabsf(v));
+                            }
+                            far |= __float_as_uint(m) < least;
+                        }
+            }
         }
+        if (far && row < n_rows) sh.apart = 1;
         if (c == 0) sh.scale[row] = up * scale;
         for (int i = 4 * c; i < r16; i += 4 * TPR) {
             const float4 s = *reinterpret_cast<const float4*>(sums + row * cap + i);
@@ -603,6 +640,15 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
         }
     }
     __syncthreads();
+    const bool apart = r_all > 0 && sh.apart;
+    if (apart) {  // t as it is, where its 16-bit numbers were
+        for (int i = tid; i < T * r16 / 4; i += kAdThreads) {
+            const int row = i / (r16 / 4), c = i % (r16 / 4) * 4;
+            *reinterpret_cast<float4*>(t32 + row * (cap + 8) + c) = *reinterpret_cast<const float4*>(sums + row * cap + c);
+        }
+        if (tid < T) sh.scale[tid] = P.scales ? __ldg(P.scales + a) : 1.f;
+        __syncthreads();
+    }
 
     // ---- out = base + B t: this CTA's part of M, FB outputs and 64 ranks at a time through shared memory
     const int units = (P.M + 31) / 32, m_from = 32 * (int)((long long)units * rank / S), m_to = min(P.M, 32 * (int)((long long)units * (rank + 1) / S));
@@ -659,10 +705,10 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
     };
     const uint32_t wm = smem_u32(stage) + (FW * ks + (lane & 7) + (lane >> 4) * 8) * wld + (lane >> 3 & 1) * 16;
     const uint32_t tm = smem_u32(t16) + (16 * mt + (lane & 15)) * pld + (lane >> 4) * 16;
-    // SK groups of sixteen ranks, whose operand of t a warp keeps (0: any number, read again)
+    // SK groups of sixteen ranks, whose operand of t a warp keeps (0: any number, read again; -1: t in fp32)
     const auto outputs = [&](auto groups_of_16) {
         constexpr int SK = decltype(groups_of_16)::value;
-        uint32_t kept[SK ? SK : 1][pieces][4];
+        uint32_t kept[SK > 0 ? SK : 1][pieces][4];
 #pragma unroll
         for (int k = 0; k < SK; ++k)
 #pragma unroll
@@ -671,13 +717,44 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
         ad_pipeline<Z::stages>(count, fill, [&](int i, int slot) {
             const uint32_t ws = wm + slot * s2;
             const unsigned char* bs = stage + slot * s2 + FB * wld;
-            const int fb = SK || chunks == 1 ? i : i / chunks, ch = SK || chunks == 1 ? 0 : i % chunks, steps = SK ? SK : min(kAdChunk, r16 - ch * kAdChunk) / 16;
+            const int fb = SK > 0 || chunks == 1 ? i : i / chunks, ch = SK > 0 || chunks == 1 ? 0 : i % chunks, steps = SK > 0 ? SK : min(kAdChunk, r16 - ch * kAdChunk) / 16;
             if (ch == 0)
 #pragma unroll
                 for (int j = 0; j < J; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
             const uint32_t tp = tm + ch * kAdChunk * 2;
+            if constexpr (SK < 0) {
+                // (four consecutive ranks of every row, as in the first product)
+                const float* tr = t32 + (16 * mt + g) * (cap + 8) + ch * kAdChunk + 4 * q;
+                const unsigned char* wr = stage + slot * s2 + (FW * ks + g) * wld + 8 * q;
+#pragma unroll 1
+                for (int k = 0; k < steps; ++k) {
+                    uint32_t hi[2][4], lo[2][4];
 #pragma unroll
-            for (int k = 0; k < (SK ? SK : kAdChunk / 16); ++k)
+                    for (int h = 0; h < 2; ++h) {
+                        const float4 y = *reinterpret_cast<const float4*>(tr + 8 * h * (cap + 8) + 16 * k);
+                        ad_split(y.x, hi[h][0], lo[h][0]);
+                        ad_split(y.y, hi[h][1], lo[h][1]);
+                        ad_split(y.z, hi[h][2], lo[h][2]);
+                        ad_split(y.w, hi[h][3], lo[h][3]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        const float4 v = ad_floats(*reinterpret_cast<const uint2*>(wr + 8 * j * wld + 32 * k), (const W*)nullptr);
+                        const uint32_t b[4] = {__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)};
+                        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            const auto& x = p ? hi : lo;
+#pragma unroll
+                            for (int e = 0; e < 4; e += 2) ad_mma_tf32(c, x[0][e], x[1][e], x[0][e + 1], x[1][e + 1], b[e], b[e + 1]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[j][e] += c[e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < (SK < 0 ? 0 : SK ? SK : kAdChunk / 16); ++k)
                 if (SK || k < steps) {
                     uint32_t w[J / 2][4];
 #pragma unroll
@@ -686,7 +763,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
                     for (int p = pieces - 1; p >= 0; --p) {
                         uint32_t t[4];
                         if constexpr (SK)
-                            t[0] = kept[k % SK][p][0], t[1] = kept[k % SK][p][1], t[2] = kept[k % SK][p][2], t[3] = kept[k % SK][p][3];
+                            t[0] = kept[k % (SK > 0 ? SK : 1)][p][0], t[1] = kept[k % (SK > 0 ? SK : 1)][p][1], t[2] = kept[k % (SK > 0 ? SK : 1)][p][2], t[3] = kept[k % (SK > 0 ? SK : 1)][p][3];
                         else
                             ad_ldm(t, tp + p * T * pld + 32 * k);
 #pragma unroll
@@ -726,14 +803,16 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             }
         });
     };
-    if (r16 == 16)
+    if (r16 == 16 && !apart)
         outputs(std::integral_constant<int, 1>());
-    else if (r16 == 32)
+    else if (r16 == 32 && !apart)
         outputs(std::integral_constant<int, 2>());
-    else if (Z::most_rank > 32 && r16 == 64)
+    else if (Z::most_rank > 32 && r16 == 64 && !apart)
         outputs(std::integral_constant<int, (Z::most_rank > 32 ? 4 : 0)>());
-    else
+    else if (!apart)
         outputs(std::integral_constant<int, 0>());
+    else
+        outputs(std::integral_constant<int, -1>());
     if (r_all > 0 && S > 1) {
         __syncwarp();
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // no CTA leaves while its part may be read
