@@ -11,7 +11,7 @@
 //           collected and sorted, the weight of all larger ones is summed exactly, and the sums tell whether the cut is there.
 //   zoom    Bins with more than 384 logits (a flat row, a large vocabulary, 16-bit logits) are divided into 512 bins again, up to four times; of equal logits
 //           as many are kept as the weight left, or the number, needs.  74 rows of 131072 logits with a deviation of 0.3 and top-p 0.9: 0.16 ms, where one
-//           CTA a row took 2.1 ms; 65536 logits of bf16 rounded to few values: under 0.15 ms and 1.1 ms.
+//           CTA a row took 2.1 ms; 80 rows of 65536 bf16 logits with seven values: 0.12 ms and 3.2 ms.
 //   neither Where more than 384 logits are equal to a small top-k's last, or four divisions were not enough, one CTA does the row by radix passes
 //           (dw_row_plain).
 // Without top-k and top-p no cut is needed: min-p's is a value that follows from the maximum.
@@ -686,9 +686,11 @@ struct DcStretch {
             if (largest >= from_l) R.mark(marks, v, i, from_l);
         });
     }
-    __device__ __forceinline__ void set_bins() {
+    // The bins of a stretch that ends with logits (`known`), or of one that may reach far down: no further then than 2.5 times the range of the threads' largest logits, unless
+    // those are all the same.
+    __device__ __forceinline__ void set_bins(bool known) {
         top_l = fminf(to_l, R.r.mx);
-        const float span = fminf(top_l - from_l, 2.5f * (R.r.mx - mn));
+        const float most = 2.5f * (R.r.mx - mn), span = fminf(top_l - from_l, !known && most > 0.f ? most : 3.402823466e38f);
         per_bin = span > 0.f ? fminf(((float)kDcBins - 1.0f) / span, 1e30f) : 1e30f;
         bin_y = -(float)R.r.c / per_bin;
     }
@@ -923,7 +925,7 @@ __device__ __noinline__ void dc_zoomed(const DrawArgs& A, int S, int n_slice, bo
     D.whole(from_all);
     D.to_l = sh.zoom.to_l, D.base = sh.zoom.base, D.base_all = sh.zoom.base_all;
     D.mark();
-    D.set_bins();
+    D.set_bins(false);  // (as they were)
     u64 total = sh.zoom.total;
     int b1 = sh.bin, b2 = sh.bin_to, n_in = sh.n_in;
     __syncthreads();
@@ -934,6 +936,7 @@ __device__ __noinline__ void dc_zoomed(const DrawArgs& A, int S, int n_slice, bo
     DcEnd end = kDcByPasses;
 #pragma unroll 1
     while (true) {
+        bool known = false;
         if (n_in > kDcList) {
             if (zooms++ == kDcZooms) {
                 dc_sync(S);  // (the histograms are being read)
@@ -946,6 +949,7 @@ __device__ __noinline__ void dc_zoomed(const DrawArgs& A, int S, int n_slice, bo
             D.base_n += dc_all(one ? sh.sums[R.lane & 7].n : 0ull, DcAdd());
             const float hi = dc_warp_max(one ? sh.top[R.lane & 7].x : -INFINITY), lo = dc_warp_min(one ? sh.top[R.lane & 7].y : INFINITY);
             D.from_l = lo, D.to_l = nextafterf(hi, INFINITY);
+            known = true;
             if (!(lo < hi)) {
                 // equal ones: as many of them as the weight or the number left needs
                 const u64 w = R.weight(lo);
@@ -953,7 +957,7 @@ __device__ __noinline__ void dc_zoomed(const DrawArgs& A, int S, int n_slice, bo
                 if (by_k && r.top_p > 0.f) total = D.base_all + m * w, P = dw_share(r.top_p, total);
                 if (r.top_p > 0.f && D.base_all >= P) {  // top-p's cut lies further up
                     if (!by_k) break;
-                    by_k = false;
+                    by_k = known = false;
                     D.whole(from_all);
                 } else {
                     if (r.top_p > 0.f) {
@@ -975,7 +979,7 @@ __device__ __noinline__ void dc_zoomed(const DrawArgs& A, int S, int n_slice, bo
             end = D.cut_at_p(b1, b2, total, P, c);
             break;
         }
-        D.set_bins();
+        D.set_bins(known);
         reinterpret_cast<uint4*>(sh.hist)[R.tid] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         D.count();
@@ -1160,7 +1164,7 @@ __global__ void __launch_bounds__(kDwThreads, 5) draw_cluster_kernel(const __gri
     DcCut c = {0, ~0ull, 0};
     DcEnd end = kDcByMinP;
     if (binned_p || binned_k) {
-        D.set_bins();
+        D.set_bins(false);
         if (!done_marks) D.mark();
         D.count();
         int b1, b2, n_in = 0;
