@@ -1048,8 +1048,8 @@ void Model::forward_rows(State& st, const StepPlan& plan, bool use_cursor) {
                                                         ws.x, ws.status);
         check_launch("embed_ln0");
     }
-    // the sessions' adapters beside a projection, added to what it gave
-    const bool adapted = std::any_of(st.adapter.begin(), st.adapter.end(), [](int32_t a) { return a >= 0; });
+    // the sessions' adapters beside a projection, added to what it gave (where a session of this step has one; others of the state may)
+    const bool adapted = std::any_of(plan.rows.begin(), plan.rows.end(), [&st](const RowMeta& r) { return st.adapted(r.slot); });
     if (adapted) LAUNCH(*this, "row_adapters") {
             row_adapters_kernel<<<(R + 255) / 256, 256, 0, stream>>>(ws.row_meta, st.adapter_dev, R, ws.row_adapter);
             check_launch("row_adapters");
