@@ -96,10 +96,20 @@ void engine_apply_adapters(cudaStream_t stream, int device, const rsv_adapters& 
         launch_adapters<float, __nv_bfloat16>(stream, device, P);
 }
 
-// First and one past the last byte of `rows` rows of `cols` elements.
-static void span(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t size, uintptr_t& lo, uintptr_t& hi) {
-    lo = (uintptr_t)p;
-    hi = lo + (uintptr_t)(((rows - 1) * ld + cols) * size);
+// Rows of `cols` elements, ld elements apart.
+struct Span {
+    const void* p;
+    int64_t cols, ld;
+};
+// Whether an element of a's rows may be one of b's: by the first and last bytes, and, for rows the same distance apart, by columns (x and out may be columns of one array).
+static bool meet(const Span& a, const Span& b, int64_t rows, int64_t size) {
+    const uintptr_t a0 = (uintptr_t)a.p, a1 = a0 + (uintptr_t)(((rows - 1) * a.ld + a.cols) * size), b0 = (uintptr_t)b.p, b1 = b0 + (uintptr_t)(((rows - 1) * b.ld + b.cols) * size);
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (a.ld != b.ld || a.ld == 0) return true;
+    const int64_t pitch = a.ld * size;
+    int64_t at = (int64_t)(b0 - a0) % pitch;  // where a row of b begins behind one of a
+    if (at < 0) at += pitch;
+    return at < a.cols * size || at + b.cols * size > pitch;
 }
 
 }  // namespace rsv
@@ -124,14 +134,10 @@ extern "C" int rsv_adapters_apply(int device, void* stream, const rsv_adapters* 
         if ((uintptr_t)x_dev % xs || (uintptr_t)base_dev % xs || (uintptr_t)out_dev % xs || (uintptr_t)ad->a % 2 || (uintptr_t)ad->b % 2 || (uintptr_t)index_dev % 4 ||
             (uintptr_t)ad->ranks % 4 || (uintptr_t)ad->scales % 4)
             throw std::runtime_error("adapters: a pointer is not aligned to its type");
-        uintptr_t o0, o1, p0, p1;
-        span(out_dev, rows, ad->M, out_stride, xs, o0, o1);
-        span(x_dev, rows, ad->K, x_stride, xs, p0, p1);
-        if (o0 < p1 && p0 < o1) throw std::runtime_error("adapters: out and x overlap");
-        if (base_dev && !(base_dev == out_dev && (base_stride == out_stride || rows == 1))) {
-            span(base_dev, rows, ad->M, base_stride, xs, p0, p1);
-            if (o0 < p1 && p0 < o1) throw std::runtime_error("adapters: out and base overlap without being the same rows");
-        }
+        const Span out = {out_dev, ad->M, out_stride};
+        if (meet(out, {x_dev, ad->K, x_stride}, rows, xs)) throw std::runtime_error("adapters: out and x overlap");
+        if (base_dev && !(base_dev == out_dev && (base_stride == out_stride || rows == 1)) && meet(out, {base_dev, ad->M, base_stride}, rows, xs))
+            throw std::runtime_error("adapters: out and base overlap without being the same rows");
         DeviceScope on(device);
         engine_apply_adapters((cudaStream_t)stream, device, *ad, xtype, x_dev, x_stride, rows, index_dev, base_dev, base_stride, out_dev, out_stride);
     });
