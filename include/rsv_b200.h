@@ -259,7 +259,7 @@ int rsv_draw_tokens(int device, void* stream, int dtype, const void* logits_dev,
 
 /* Low-rank adapters of many requests.  Slot s holds A [rank, K] in the first rank rows of a[s] ([max_rank, K], rows a_row and slots a_slot
  * elements apart) and B [M, rank] in the first rank columns of b[s] ([M, max_rank], rows b_row apart, slots b_slot); what lies behind a slot's
- * rank is never used.  dtype: RSV_F16 or RSV_BF16.  ranks[slots] NULL: max_rank each; scales[slots] NULL: 1.  max_rank <= 256, slots <= 4096. */
+ * rank is never used.  dtype: RSV_F16 or RSV_BF16.  ranks[slots] NULL: max_rank each; scales[slots] NULL: 1.  max_rank <= 256, slots <= 4096, rows <= 2^25. */
 typedef struct {
     int32_t dtype;
     int64_t slots, max_rank, K, M;

@@ -126,7 +126,7 @@ extern "C" int rsv_adapters_apply(int device, void* stream, const rsv_adapters* 
             throw std::runtime_error("adapters: K and M must be between 1 and 2^28 - 1, slots between 1 and 4096");
         if (ad->max_rank < 1 || ad->max_rank > kAdMaxRank) throw std::runtime_error("adapters: max_rank must be between 1 and 256");
         if (ad->a_row < 0 || ad->a_slot < 0 || ad->b_row < 0 || ad->b_slot < 0 || x_stride < 0 || base_stride < 0) throw std::runtime_error("adapters: negative stride");
-        if (rows < 0 || rows > lim / 64) throw std::runtime_error("adapters: rows must be between 0 and 2^25");
+        if (rows < 0 || rows > kAdMaxRows) throw std::runtime_error("adapters: rows must be between 0 and " + std::to_string(kAdMaxRows));
         if (rows == 0) return;
         if (!ad->a || !ad->b || !x_dev || !index_dev || !out_dev) throw std::runtime_error("adapters: null argument");
         if (rows > 1 && out_stride < ad->M) throw std::runtime_error("adapters: rows of out overlap");

@@ -49,6 +49,7 @@ constexpr int kAdThreads = 256;
 constexpr int kAdWarps = kAdThreads / 32;
 constexpr int kAdMaxRank = 256;
 constexpr int kAdMaxSlots = 4096;
+constexpr int kAdMaxRows = 1 << 25;  // (8192 blocks of rows with up to 4096 tiles each, as many CTAs)
 constexpr int kAdBlockRows = 4096;
 constexpr int kAdMaxCtas = 8;
 constexpr int kAdChunk = 64;  // ranks whose sums a warp holds at a time

@@ -6,6 +6,13 @@ from test_device_operator_refusals import adapters
 OUT = 1 << 28
 
 
+def test_most_rows():
+    rc, err = adapters(rows=1 << 25, x=None)
+    assert rc != 0 and "null" in err, err
+    rc, err = adapters(rows=(1 << 25) + 1, x=None)
+    assert rc != 0 and "rows must be between 0 and 33554432" in err, err
+
+
 # buffer of 128 columns: out takes 32 .. 63 (M = 32), x and base lie at some column of it
 @pytest.mark.parametrize("x_at,base_at,refused", [
     (64, 0, False), (64, 96, False), (64, None, False), (63, None, True), (0, None, True), (64, 31, True), (64, 33, True), (65, 0, True), (64 + 128, 0, False), (64, 128, False), (64, 128 + 33, True),
