@@ -268,13 +268,19 @@ class Model:
 
     def adapter_set(self, slot, layer, site, A, B, scale=1.0):
         """Adapter `slot` adds scale B (A x) to the projection `site` ("att.output" or "ffn.value") of a layer; A [rank, K], B [n_embd, rank].  A None: nothing."""
+        if site not in self.SITES:
+            raise RsvError(f"adapter_set: no site {site!r}; there are {' and '.join(self.SITES)}")
         if A is None:
             _check(native().rsv_model_adapter_set(self._h, int(slot), int(layer), self.SITES.index(site), 0, None, None, 1.0))
             return
-        a, b = _np.ascontiguousarray(A, dtype=_np.float16), _np.ascontiguousarray(B, dtype=_np.float16)
         K = self._info.num_emb if site == "att.output" else self._info.ffn_hidden
-        if site not in self.SITES or a.ndim != 2 or a.shape[1] != K or b.shape != (self._info.num_emb, a.shape[0]):
+        with _np.errstate(over="ignore"):
+            a, b = _np.ascontiguousarray(A, dtype=_np.float16), _np.ascontiguousarray(B, dtype=_np.float16)
+        if a.ndim != 2 or a.shape[1] != K or b.shape != (self._info.num_emb, a.shape[0]):
             raise RsvError(f"adapter_set: A {a.shape} and B {b.shape} do not go with {site} of {K} inputs and {self._info.num_emb} outputs")
+        for name, given, half in (("A", A, a), ("B", B, b)):
+            if (_np.isinf(half) & _np.isfinite(given)).any():
+                raise RsvError(f"adapter_set: {name} has values that float16 cannot hold (over 65504)")
         _check(native().rsv_model_adapter_set(self._h, int(slot), int(layer), self.SITES.index(site), a.shape[0], _ptr(a), _ptr(b), float(scale)))
 
     # ---- diagnostics ----
