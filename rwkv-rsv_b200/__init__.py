@@ -433,7 +433,8 @@ class Bundle:
     def infer_draw(self, tokens, params, u):
         """The next token and its log-probability, drawn with the random number u in [0, 1) after `params` (DrawParams)."""
         t, out, lp = _tokens(tokens), _np.zeros(1, dtype=_np.uint32), _np.zeros(1, dtype=_np.float32)
-        _check(native().rsv_infer_draw(self.model._h, self.state._h, _ptr(t), t.size, _c.byref(params), float(u), _ptr(out), _ptr(lp)))
+        u = min(float(u), 1 - 2.0**-24) if u < 1 else float(u)  # (doubles behind the largest float under 1 would round to 1)
+        _check(native().rsv_infer_draw(self.model._h, self.state._h, _ptr(t), t.size, _c.byref(params), u, _ptr(out), _ptr(lp)))
         return int(out[0]), float(lp[0])
 
     def infer_sample_selfloop(self, seed, n, sp):
