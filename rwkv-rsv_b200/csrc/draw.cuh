@@ -137,7 +137,7 @@ static_assert(kDwThreads == 256, "a thread per bin of a radix pass");
 // ---- a row by one CTA, from global memory -----------------------------------------------------------------
 struct DwPlainShared {
     double tab[16];
-    u64 hist[256], wsum[kDwWarps], target, total, acc;
+    u64 hist[256], wsum[kDwWarps], acc;
     uint32_t wcnt[kDwWarps], digit, cnt, best;
     float red[kDwWarps];
 };
