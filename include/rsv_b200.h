@@ -273,7 +273,8 @@ typedef struct {
 /* out[n] = base[n] + scale[s] B[s] (A[s] x[n]) with s = index_dev[n], for rows x[rows][K], base and out [rows][M] (strides in elements; xtype RSV_F32 or
  * the adapters' dtype, for all three).  A row whose index is negative (or >= slots) has no adapter: out[n] = base[n].  base is what the shared projection
  * gave, NULL counts as zeros, and it may be out itself; no other overlap of out is allowed (x, base and out may be separate columns of one array, with its row stride each).
- * Sums are fp32, rounded to out's type once. */
+ * Sums are fp32, rounded to out's type once; A x enters the second one to 2^-20 of itself or of the largest part that it is summed from (2^-17 for 16-bit rows).  fp16 values
+ * of B under 2^-14, and next to fp16 rows of A and x, enter sums as exactly as 2^-14 would. */
 int rsv_adapters_apply(int device, void* stream, const rsv_adapters* ad, int xtype, const void* x_dev, int64_t x_stride, int64_t rows,
                        const int32_t* index_dev, const void* base_dev, int64_t base_stride, void* out_dev, int64_t out_stride);
 

@@ -13,9 +13,11 @@
 // outside 2^-100 .. 2^100, has t as two tf32 numbers (2^-22 of any value) and the second product in tf32: what a rank adds keeps its precision whatever the other
 // ranks add, as it has to where outputs use few of them.  (With all tiles of that kind: one fp32 session of 2560 x 2560 11.2 us instead of 8.4, 512 rows with 64 ranks of
 // 2560 x 10240 39 instead of 25.)
+// The tensor cores line products up by the exponents of their operands, which is that of 2^-14 for all fp16 numbers below: the sums of B t (and of A x, where x is fp16) are as exact
+// as with weights of 2^-14 where those are smaller (two ranks 2^12 apart with weights of 2^-24 and 3e-5: 2^-14 of their sum off; zeros do not count, and tf32 has no such end).
 //
-// Bound by its instructions: a scheduler issues in 35 to 48 % of the cycles, four warps of it waiting for fixed latencies, and in short calls for instructions that
-// are fetched for the first time.  4096 bf16 rows, 16 adapters of 64 ranks, 2560 x 10240: 78 us, 2.6 TB/s (the second product 50 of them); 64 sessions of 10240 k with 64
+// Bound by its instructions: a scheduler issues in 34 to 53 % of the cycles, four warps of it waiting for fixed latencies, and in short calls for instructions that
+// are fetched for the first time.  4096 bf16 rows, 16 adapters of 64 ranks, 2560 x 10240: 75 us, 2.7 TB/s (the second product 50 of them); 64 sessions of 10240 k with 64
 // adapters of 16 ranks, fp32: 20 us, 1.0 TB/s; one session of 2560 x 2560: 10 us, all latency.
 #pragma once
 #include <cuda_bf16.h>
@@ -641,21 +643,12 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
         }
     }
     __syncthreads();
-    const bool apart = r_all > 0 && sh.apart;
-    if (apart) {  // t as it is, where its 16-bit numbers were
-        for (int i = tid; i < T * r16 / 4; i += kAdThreads) {
-            const int row = i / (r16 / 4), c = i % (r16 / 4) * 4;
-            *reinterpret_cast<float4*>(t32 + row * (cap + 8) + c) = *reinterpret_cast<const float4*>(sums + row * cap + c);
-        }
-        if (tid < T) sh.scale[tid] = P.scales ? __ldg(P.scales + a) : 1.f;
-        __syncthreads();
-    }
 
     // ---- out = base + B t: this CTA's part of M, FB outputs and 64 ranks at a time through shared memory
     const int units = (P.M + 31) / 32, m_from = 32 * (int)((long long)units * rank / S), m_to = min(P.M, 32 * (int)((long long)units * (rank + 1) / S));
     const int chunks = max(1, (r16 + kAdChunk - 1) / kAdChunk), rc = min(r16, kAdChunk), wld = Z::wld(rc), s2 = Z::stage2(rc);
     const int count = (max(m_to - m_from, 0) + FB - 1) / FB * chunks;
-    const float t0 = r_all ? sh.scale[16 * mt + g] : 0.f, t1 = r_all ? sh.scale[16 * mt + g + 8] : 0.f;
+    float t0 = r_all ? sh.scale[16 * mt + g] : 0.f, t1 = r_all ? sh.scale[16 * mt + g + 8] : 0.f;
     const bool have0 = 16 * mt + g < n_rows, have1 = 16 * mt + g + 8 < n_rows;
     X* o0 = op + (int64_t)sh.rows[min(16 * mt + g, n_rows - 1)] * P.ldout + m_from + FW * ks + 4 * q;  // of this stage
     X* o1 = op + (int64_t)sh.rows[min(16 * mt + g + 8, n_rows - 1)] * P.ldout + m_from + FW * ks + 4 * q;
@@ -804,6 +797,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
             }
         });
     };
+    const bool apart = r_all > 0 && sh.apart;
     if (r16 == 16 && !apart)
         outputs(std::integral_constant<int, 1>());
     else if (r16 == 32 && !apart)
@@ -812,8 +806,15 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapters_kernel(AdapterArgs P) 
         outputs(std::integral_constant<int, (Z::most_rank > 32 ? 4 : 0)>());
     else if (!apart)
         outputs(std::integral_constant<int, 0>());
-    else
+    else {  // t as it is, where its 16-bit numbers were
+        for (int i = tid; i < T * r16 / 4; i += kAdThreads) {
+            const int row = i / (r16 / 4), c = i % (r16 / 4) * 4;
+            *reinterpret_cast<float4*>(t32 + row * (cap + 8) + c) = *reinterpret_cast<const float4*>(sums + row * cap + c);
+        }
+        t0 = t1 = P.scales ? __ldg(P.scales + a) : 1.f;
+        __syncthreads();
         outputs(std::integral_constant<int, -1>());
+    }
     if (r_all > 0 && S > 1) {
         __syncwarp();
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // no CTA leaves while its part may be read

@@ -34,11 +34,12 @@ def apart(rows, K, M, most, x, w, up, down, inverse, slots=2, seed=0):
             "ranks": None, "scales": torch.rand(slots, generator=g, device="cuda") + 0.5, "index": torch.arange(rows, device="cuda", dtype=torch.int32) % slots}
 
 
-def check(d):
+def check(d, least=0.0):
+    """(least: what smaller weights of B but 0 count as in `size`.)"""
     import torch
     out = apply(d)
     want = exact(d["x"], d["index"], d["A"], d["B"], d["ranks"], d["scales"], d["base"])
-    size = exact(d["x"].abs(), d["index"], d["A"].abs(), d["B"].abs(), d["ranks"], d["scales"], d["base"].abs())
+    size = exact(d["x"].abs(), d["index"], d["A"].abs(), torch.where(d["B"] == 0, 0.0, d["B"].double().abs().clamp(min=least)), d["ranks"], d["scales"], d["base"].abs())
     xt = d["x"].dtype
     room = 2.0**-18 * size if xt == torch.float32 else 2.0**-16 * size + torch.finfo(xt).eps / 2 * want.abs() * 1.001
     room += torch.finfo(xt).smallest_normal * torch.finfo(xt).eps  # (16-bit outputs under the smallest normal one)
@@ -142,3 +143,13 @@ def test_infinities_and_nan_as_in_a_sum_of_products(x, w):
         bad.append(5)
     rest = [n for n in range(20) if n not in bad]
     assert torch.equal(got[rest], want[rest])
+
+
+@pytest.mark.parametrize("x,w", TYPES)
+@pytest.mark.parametrize("size", [2.0**-15, 2.0**-18, 2.0**-22])
+@pytest.mark.parametrize("rows,K,M,most", [(1, 2, 40, 2), (40, 64, 72, 16), (900, 64, 64, 64)])
+def test_weights_under_the_smallest_normal_fp16(rows, K, M, most, size, x, w):
+    """B of 2^-15 and less, down to 2^-24, next to ranks of other sizes: as exact as with weights of 2^-14, which is 2^-18 (2^-16) of 2^-14 |A| |x|."""
+    d = apart(rows, K, M, most, x, w, 1.0, 2.0**-8, True)
+    d["B"] = (d["B"].double() * size * 5).clamp(-4 * size, 4 * size).to(d["B"].dtype)
+    check(d, 2.0**-14 if w == "float16" else 0.0)
