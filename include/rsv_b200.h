@@ -252,7 +252,8 @@ enum { RSV_F32 = 0, RSV_F16 = 1, RSV_BF16 = 2 };
  *   - the token is the first kept one, in vocabulary order, whose running sum of w exceeds u times the sum of all kept ones.
  * T <= 0 takes the largest logit (the lowest of equal ones).  u < 0 and NaN count as 0, u >= 1 takes the last kept token.
  * tokens_dev[rows]; logprobs_dev[rows] (may be NULL) is the natural logarithm of the token's share of the kept sum.  Logits of -inf are never
- * drawn; where there is nothing else the token is 0xFFFFFFFF and the log-probability -inf; a row with a NaN gives 0xFFFFFFFF and NaN.
+ * drawn; where there is nothing else the token is 0xFFFFFFFF and the log-probability -inf; a row with a NaN gives 0xFFFFFFFF and NaN.  Where there are logits of
+ * +inf only they are drawn, as equal ones.
  * Weights and sums are whole numbers of 64 bits, so the result does not depend on how rows are split or batched.  V <= 2^22; rows <= 2^28 - 1. */
 int rsv_draw_tokens(int device, void* stream, int dtype, const void* logits_dev, int64_t rows, int64_t V, int64_t row_stride, const float* params4_dev,
                     const float* uniforms_dev, uint32_t* tokens_dev, float* logprobs_dev);
